@@ -15,11 +15,13 @@
 #include <string>
 
 #include "../../include/hkmoe.h"
+#include "bf16_rows.hpp"
 #include "gemm_fp8.hpp"
 #include "gemm_narrow.hpp"
 #include "gemm_skinny.hpp"
 #include "gemm_small.hpp"
 #include "moe_kernels.hpp"
+#include "norm_quant.hpp"
 
 #include <atomic>
 #include <cstdlib>
@@ -602,6 +604,56 @@ int launch_expert_offsets(const int32_t* block_counts, int64_t num_tokens, int32
   return check_launch("expert_offsets_kernel");
 }
 
+
+// ---------------------------------------------------------------------------
+// residual + norm + quantisation, router, adapters
+// ---------------------------------------------------------------------------
+constexpr int64_t kMaxRows = 1 << 26;  // a launch's work-items stay below 2^32 in each dimension
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int norm_chunks(int64_t cols) {  // chunks per thread: a row of up to 8192 values in one
+  const int64_t c = cols / kNormChunk;
+  return c <= kNormMaxThreads ? 1 : c <= 2 * kNormMaxThreads ? 2 : c <= 4 * kNormMaxThreads ? 4 : 8;
+}
+
+template <bool F32, NormScale SC>
+int launch_norm(const NormParams& p, hipStream_t s) {
+  const int ch = norm_chunks(p.cols);
+  const int threads = (p.cols / kNormChunk + ch * kWave - 1) / (ch * kWave) * kWave;
+  const int64_t grid = SC == NormScale::kAmax ? std::min<int64_t>(p.rows, kNormAmaxGroups) : std::min<int64_t>(p.rows, 1 << 20);
+  auto kern = ch == 1   ? rms_norm_quant_kernel<F32, SC, 1>
+              : ch == 2 ? rms_norm_quant_kernel<F32, SC, 2>
+              : ch == 4 ? rms_norm_quant_kernel<F32, SC, 4>
+                        : rms_norm_quant_kernel<F32, SC, 8>;
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, p);
+  return check_launch("rms_norm_quant_kernel");
+}
+
+template <bool F32>
+int launch_norm(const NormParams& p, int mode, hipStream_t s) {
+  if (mode == HKMOE_SCALE_BLOCK) return launch_norm<F32, NormScale::kGroup>(p, s);
+  if (mode == HKMOE_SCALE_MX) return launch_norm<F32, NormScale::kMx>(p, s);
+  if (p.scale != nullptr) return launch_norm<F32, NormScale::kStatic>(p, s);
+  int groups = 0;
+  if (p.rows > 0) {
+    HK_TRY((launch_norm<F32, NormScale::kAmax>(p, s)));
+    groups = static_cast<int>(std::min<int64_t>(p.rows, kNormAmaxGroups));
+  }
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.rows, 2048)));
+  hipLaunchKernelGGL(norm_quant_tensor_kernel<F32>, dim3(grid), dim3(256), 0, s,
+                     p.residual != nullptr ? static_cast<const void*>(p.residual_out) : p.x, p.weight, p.w_f32, p.rstd,
+                     p.amax, groups, p.rows, p.cols, p.q, static_cast<float*>(p.s));
+  return check_launch("norm_quant_tensor_kernel");
+}
+
+// Workgroups over which the adapters' narrow product splits its K steps: enough to
+// fill the chip, at least one step per wave.
+int lora_splits(int64_t rows, int64_t hidden) {
+  const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock, steps = (hidden + kRowsStep - 1) / kRowsStep;
+  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, steps / kRowsWaves));
+  return static_cast<int>(std::min(most, std::max<int64_t>(1, 512 / std::max<int64_t>(1, blocks))));
+}
 
 }  // namespace
 
@@ -1421,6 +1473,141 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
   hipLaunchKernelGGL(quant_tensor_kernel, dim3(grid), dim3(256), 0, st, x, n, amax_ws,
                      static_cast<uint8_t*>(q), s);
   return check_launch("quant_tensor_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// residual + norm + quantisation, router, adapters
+// ---------------------------------------------------------------------------
+size_t hkmoe_rms_norm_quant_workspace_size(int64_t rows, int scale_mode, int given_scale) {
+  if (rows <= 0 || scale_mode != HKMOE_SCALE_TENSOR || given_scale) return 0;
+  return align256((static_cast<size_t>(rows) + kNormAmaxGroups) * sizeof(float));
+}
+
+int hkmoe_rms_norm_quant(const void* x, const void* residual, const void* weight, int64_t rows, int64_t cols,
+                         int x_dtype, int weight_dtype, double eps, int scale_mode, const float* scale, void* q, void* s,
+                         void* residual_out, void* norm_out, void* workspace, size_t workspace_bytes,
+                         hkmoe_stream_t stream) {
+  HK_REQUIRE(rows >= 0 && cols > 0 && rows <= kMaxRows, "rms_norm_quant: bad shape rows=%lld cols=%lld",
+             (long long)rows, (long long)cols);
+  HK_REQUIRE(scale_mode == HKMOE_SCALE_TENSOR || scale_mode == HKMOE_SCALE_BLOCK || scale_mode == HKMOE_SCALE_MX,
+             "rms_norm_quant: bad scale_mode %d", scale_mode);
+  const int unit = scale_mode == HKMOE_SCALE_BLOCK ? kGroup : scale_mode == HKMOE_SCALE_MX ? 32 : kNormChunk;
+  HK_REQUIRE(cols % unit == 0 && cols <= 8 * kNormMaxThreads * kNormChunk,
+             "rms_norm_quant: cols=%lld must be a multiple of %d, at most 65536", (long long)cols, unit);
+  HK_REQUIRE((x_dtype == HKMOE_BF16 || x_dtype == HKMOE_F32) && (weight_dtype == HKMOE_BF16 || weight_dtype == HKMOE_F32),
+             "rms_norm_quant: bad dtype %d / %d", x_dtype, weight_dtype);
+  HK_REQUIRE(eps > 0 && eps < 1e30, "rms_norm_quant: eps=%g must be positive and finite", eps);
+  const bool given = scale_mode == HKMOE_SCALE_TENSOR && scale != nullptr;
+  HK_REQUIRE(scale == nullptr || given, "rms_norm_quant: a given scale is for HKMOE_SCALE_TENSOR");
+  HK_REQUIRE(weight && (rows == 0 || (x && q)) && (given || s || (rows == 0 && scale_mode != HKMOE_SCALE_TENSOR)),
+             "rms_norm_quant: null pointer");
+  HK_REQUIRE(rows == 0 || !residual == !residual_out, "rms_norm_quant: residual and residual_out come together");
+  HK_REQUIRE(aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(q) && aligned16(residual_out) &&
+                 aligned16(norm_out),
+             "rms_norm_quant: tensors must be 16-byte aligned");
+  const size_t need = hkmoe_rms_norm_quant_workspace_size(rows, scale_mode, given);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    return fail(HKMOE_ERR_WORKSPACE, "rms_norm_quant: workspace needs %zu bytes, 16-byte aligned", need);
+  if (rows == 0 && (given || scale_mode != HKMOE_SCALE_TENSOR)) return HKMOE_OK;
+  NormParams p{};
+  p.x = x;
+  p.residual = residual;
+  p.weight = weight;
+  p.residual_out = residual_out;
+  p.norm_out = static_cast<uint16_t*>(norm_out);
+  p.q = static_cast<uint8_t*>(q);
+  p.s = s;
+  p.scale = scale;
+  p.amax = static_cast<float*>(workspace);
+  p.rstd = need > 0 ? p.amax + kNormAmaxGroups : nullptr;
+  p.rows = rows;
+  p.cols = static_cast<int32_t>(cols);
+  p.w_f32 = weight_dtype == HKMOE_F32;
+  p.eps = eps;
+  auto st = static_cast<hipStream_t>(stream);
+  return x_dtype == HKMOE_F32 ? launch_norm<true>(p, scale_mode, st) : launch_norm<false>(p, scale_mode, st);
+}
+
+int hkmoe_router_logits(const void* x, const void* w, int64_t num_tokens, int32_t num_experts, int64_t hidden,
+                        float* logits, hkmoe_stream_t stream) {
+  HK_REQUIRE(num_tokens >= 0 && num_tokens <= kMaxRows && num_experts >= 1 && num_experts <= kMaxExperts,
+             "router_logits: bad shape T=%lld E=%d (1 <= E <= %d)", (long long)num_tokens, num_experts, kMaxExperts);
+  HK_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= (1 << 20),
+             "router_logits: H=%lld must be a multiple of 8, at most 2^20", (long long)hidden);
+  HK_REQUIRE(w && (num_tokens == 0 || (x && logits)), "router_logits: null pointer");
+  HK_REQUIRE(aligned16(x) && aligned16(w) && (reinterpret_cast<uintptr_t>(logits) & 3) == 0,
+             "router_logits: x and w must be 16-byte aligned");
+  if (num_tokens == 0) return HKMOE_OK;
+  RouterParams p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w), logits, num_tokens, num_experts,
+                 static_cast<int32_t>(hidden)};
+  const dim3 grid(static_cast<unsigned>((num_tokens + 15) / 16), static_cast<unsigned>((num_experts + 63) / 64));
+  hipLaunchKernelGGL((router_kernel<1, 4>), grid, dim3(kRowsWaves * 64), 0, static_cast<hipStream_t>(stream), p);
+  return check_launch("router_kernel");
+}
+
+size_t hkmoe_lora_workspace_size(int64_t rows, int64_t hidden, int32_t rank) {
+  if (rows <= 0 || hidden <= 0 || rank <= 0) return 0;
+  return align256(static_cast<size_t>(lora_splits(rows, hidden)) * rows * rank * sizeof(float));
+}
+
+int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* a, const void* b,
+                   const int32_t* ids, const float* scaling, int64_t rows, int32_t adapters, int64_t hidden, int64_t n,
+                   int32_t rank, int y_dtype, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                   hkmoe_stream_t stream) {
+  HK_REQUIRE(rows >= 0 && rows <= kMaxRows && adapters >= 1, "lora_add: bad shape rows=%lld adapters=%d",
+             (long long)rows, adapters);
+  HK_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= (1 << 20) && n > 0 && n % 8 == 0 && n <= (1 << 24),
+             "lora_add: H=%lld and N=%lld must be multiples of 8, at most 2^20 and 2^24", (long long)hidden, (long long)n);
+  HK_REQUIRE(rank > 0 && rank % 8 == 0 && rank <= kLoraMaxRank, "lora_add: rank=%d must be a multiple of 8, at most %d",
+             rank, kLoraMaxRank);
+  HK_REQUIRE(y_dtype == HKMOE_BF16 || y_dtype == HKMOE_F32, "lora_add: bad y_dtype %d", y_dtype);
+  HK_REQUIRE(a && b && (rows == 0 || (y && x && ids && out)), "lora_add: null pointer");
+  HK_REQUIRE(x_stride >= hidden && x_stride % 8 == 0 && y_stride >= n && out_stride >= n &&
+                 (y_stride * (y_dtype == HKMOE_F32 ? 4 : 2)) % 16 == 0 && (out_stride * (y_dtype == HKMOE_F32 ? 4 : 2)) % 16 == 0,
+             "lora_add: rows must be 16-byte aligned and not overlap (strides x %lld, y %lld, out %lld)",
+             (long long)x_stride, (long long)y_stride, (long long)out_stride);
+  HK_REQUIRE(aligned16(y) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(out) &&
+                 (reinterpret_cast<uintptr_t>(ids) & 3) == 0 && (reinterpret_cast<uintptr_t>(scaling) & 3) == 0,
+             "lora_add: x, y, out, a and b must be 16-byte aligned");
+  HK_REQUIRE(y != out || y_stride == out_stride, "lora_add: out in y's place needs y's row stride");
+  if (rows == 0) return HKMOE_OK;
+  const size_t need = hkmoe_lora_workspace_size(rows, hidden, rank);
+  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
+    return fail(HKMOE_ERR_WORKSPACE, "lora_add: workspace needs %zu bytes, 16-byte aligned", need);
+  LoraParams p{};
+  p.y = y;
+  p.out = out;
+  p.y_stride = y_stride;
+  p.out_stride = out_stride;
+  p.x = static_cast<const uint16_t*>(x);
+  p.x_stride = x_stride;
+  p.a = static_cast<const uint16_t*>(a);
+  p.b = static_cast<const uint16_t*>(b);
+  p.ids = ids;
+  p.scaling = scaling;
+  p.v = static_cast<float*>(workspace);
+  p.rows = rows;
+  p.adapters = adapters;
+  p.hidden = static_cast<int32_t>(hidden);
+  p.n = static_cast<int32_t>(n);
+  p.rank = rank;
+  p.splits = lora_splits(rows, hidden);
+  auto s = static_cast<hipStream_t>(stream);
+  const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock;
+  // distinct adapters a block can have, as far as a few thousand workgroups go: the
+  // others follow in the same workgroups
+  const int64_t most = std::min<int64_t>({kRowsBlock, rows, static_cast<int64_t>(adapters) + 1});
+  auto at_a_time = [&](int64_t per) { return static_cast<unsigned>(std::max<int64_t>(1, std::min(most, 4096 / (blocks * per)))); };
+  hipLaunchKernelGGL(lora_shrink_kernel, dim3(static_cast<unsigned>(blocks), at_a_time(p.splits), p.splits),
+                     dim3(kRowsWaves * 64), 0, s, p);
+  HK_TRY(check_launch("lora_shrink_kernel"));
+  const int64_t strips = (n + 255) / 256;
+  const int64_t parts = std::min<int64_t>({strips, 65535, std::max<int64_t>(1, 1024 / blocks)});
+  p.cols_per_wg = static_cast<int32_t>((strips + parts - 1) / parts * 256);
+  const dim3 grid(static_cast<unsigned>(blocks), at_a_time(parts), static_cast<unsigned>((n + p.cols_per_wg - 1) / p.cols_per_wg));
+  hipLaunchKernelGGL((y_dtype == HKMOE_F32 ? lora_expand_kernel<true, 3> : lora_expand_kernel<false, 2>), grid,
+                     dim3(kRowsWaves * 64), 0, s, p);
+  return check_launch("lora_expand_kernel");
 }
 
 // ---------------------------------------------------------------------------

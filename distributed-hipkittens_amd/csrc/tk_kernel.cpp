@@ -95,7 +95,7 @@ py::object steal(PyObject* o) {
 // a thread that then waits for the guard with the GIL held, for good.  Threads that
 // get here together each build their own and the first one to finish is kept.
 struct Names {
-  PyObject *is_contiguous, *is_cpu, *data_ptr, *shape, *dtype;
+  PyObject *is_contiguous, *is_cpu, *data_ptr, *shape, *dtype, *stride, *get_device_attr;
   PyObject* tensor_type;
   PyObject *get_device = nullptr, *raw_stream = nullptr;
   py::object torch_cuda;
@@ -109,6 +109,8 @@ const Names& names() {
   v->data_ptr = PyUnicode_InternFromString("data_ptr");
   v->shape = PyUnicode_InternFromString("shape");
   v->dtype = PyUnicode_InternFromString("dtype");
+  v->stride = PyUnicode_InternFromString("stride");
+  v->get_device_attr = PyUnicode_InternFromString("get_device");
   py::module_ torch = py::module_::import("torch");
   v->tensor_type = py::object(torch.attr("Tensor")).release().ptr();
   v->torch_cuda = torch.attr("cuda");
@@ -178,6 +180,7 @@ constexpr const char* kF8 = "torch.float8_e4m3fn";
 constexpr const char* kBf16 = "torch.bfloat16";
 constexpr const char* kF32 = "torch.float32";
 constexpr const char* kI32 = "torch.int32";
+constexpr int64_t kMaxInt = INT32_MAX;
 
 int scale_mode_of(const TensorArg& s) {
   return (s.shape.size() <= 1 && s.numel() == 1) ? HKMOE_SCALE_TENSOR : HKMOE_SCALE_BLOCK;
@@ -750,6 +753,140 @@ void dispatch_moe_mx(py::object x_q, py::object x_e8m0, py::object logits, py::o
                              bytes, current_stream()));
 }
 
+// ---------------------------------------------------------------------------
+// Residual + norm + quantisation, router, adapters.  Unlike the calls above these
+// check that every tensor lives on torch's current device, whose stream they use.
+// ---------------------------------------------------------------------------
+int64_t device_of(const py::object& obj) {
+  return steal(PyObject_CallMethodNoArgs(obj.ptr(), names().get_device_attr)).cast<int64_t>();
+}
+
+void want_current_device(std::initializer_list<std::pair<const py::object*, const char*>> ts) {
+  const Names& nm = names();
+  const int64_t cur = nm.get_device != nullptr ? steal(PyObject_CallNoArgs(nm.get_device)).cast<int64_t>()
+                                               : nm.torch_cuda.attr("current_device")().cast<int64_t>();
+  for (const auto& [obj, name] : ts)
+    if (!obj->is_none() && device_of(*obj) != cur)
+      throw std::runtime_error(std::string(name) + ": tensor must be on the current device");
+}
+
+// A 2-D tensor whose rows are contiguous: its row stride in elements.
+TensorArg as_rows(const py::object& obj, const char* name, int64_t* stride) {
+  const Names& nm = names();
+  if (!PyObject_IsInstance(obj.ptr(), nm.tensor_type)) throw std::runtime_error(std::string(name) + ": expected a torch.Tensor");
+  const py::tuple strides = steal(PyObject_CallMethodNoArgs(obj.ptr(), nm.stride)).cast<py::tuple>();
+  const py::tuple shape = steal(PyObject_GetAttr(obj.ptr(), nm.shape)).cast<py::tuple>();
+  if (shape.size() != 2) throw std::runtime_error(std::string(name) + ": expected 2-D tensor");
+  if (steal(PyObject_GetAttr(obj.ptr(), nm.is_cpu)).ptr() == Py_True)
+    throw std::runtime_error(std::string(name) + ": tensor must be on a GPU device");
+  TensorArg t;
+  for (auto s : shape) t.shape.push_back(s.cast<int64_t>());
+  if (t.shape[1] > 1 && strides[1].cast<int64_t>() != 1)
+    throw std::runtime_error(std::string(name) + ": rows must be contiguous");
+  *stride = t.shape[0] > 1 ? strides[0].cast<int64_t>() : t.shape[1];
+  t.ptr = reinterpret_cast<void*>(steal(PyObject_CallMethodNoArgs(obj.ptr(), nm.data_ptr)).cast<uintptr_t>());
+  t.dtype.name = dtype_name(steal(PyObject_GetAttr(obj.ptr(), nm.dtype)).ptr());
+  return t;
+}
+
+int float_type(const TensorArg& t, const char* name) {
+  if (t.dtype == kBf16) return HKMOE_BF16;
+  if (t.dtype == kF32) return HKMOE_F32;
+  throw std::runtime_error(std::string(name) + ": expected bfloat16 or float32, got " + t.dtype.name);
+}
+
+size_t byte_size(const TensorArg& t, const char* name) {
+  want_dtype(t, name, kU8);
+  return t.ptr ? static_cast<size_t>(t.numel()) : 0;
+}
+
+void dispatch_rms_norm_quant(py::object x_, py::object residual_, py::object weight_, double eps, int scale_mode,
+                             py::object q_, py::object s_, py::object scale_, py::object residual_out_,
+                             py::object norm_out_, py::object workspace_) {
+  auto x = as_tensor(x_, "x"), w = as_tensor(weight_, "weight"), q = as_tensor(q_, "q"), s = as_tensor_opt(s_, "s"),
+       r = as_tensor_opt(residual_, "residual"), sc = as_tensor_opt(scale_, "scale"),
+       ro = as_tensor_opt(residual_out_, "residual_out"), no = as_tensor_opt(norm_out_, "norm_out"),
+       ws = as_tensor_opt(workspace_, "workspace");
+  want_current_device({{&x_, "x"}, {&weight_, "weight"}, {&q_, "q"}, {&s_, "s"}, {&residual_, "residual"}, {&scale_, "scale"},
+                       {&residual_out_, "residual_out"}, {&norm_out_, "norm_out"}, {&workspace_, "workspace"}});
+  want_dim(x, "x", 2);
+  const int xt = float_type(x, "x"), wt = float_type(w, "weight");
+  const int64_t rows = x.shape[0], cols = x.shape[1];
+  if (w.numel() != cols) throw std::runtime_error("weight must be [C]");
+  want_dtype(q, "q", kF8);
+  if (q.shape != x.shape) throw std::runtime_error("q must be [R, C]");
+  if (residual_.is_none() != residual_out_.is_none())
+    throw std::runtime_error("residual and residual_out come together");
+  if (!residual_.is_none()) {
+    want_dtype(r, "residual", x.dtype.name);
+    want_dtype(ro, "residual_out", x.dtype.name);
+    if (r.shape != x.shape || ro.shape != x.shape) throw std::runtime_error("residual and residual_out must be [R, C]");
+  }
+  if (!norm_out_.is_none()) {
+    want_dtype(no, "norm_out", kBf16);
+    if (no.shape != x.shape) throw std::runtime_error("norm_out must be [R, C]");
+  }
+  want_dtype(sc, "scale", kF32);
+  if (!scale_.is_none() && sc.numel() != 1) throw std::runtime_error("scale must hold one value");
+  if (scale_.is_none() && s_.is_none()) throw std::runtime_error("s: expected a torch.Tensor");
+  if (scale_mode == HKMOE_SCALE_MX) {
+    want_dtype(s, "s", kU8);
+    if (s.numel() != rows * (cols / 32)) throw std::runtime_error("s must be [R, C/32]");
+  } else if (!s_.is_none()) {
+    want_dtype(s, "s", kF32);
+    if (s.numel() != (scale_mode == HKMOE_SCALE_BLOCK ? rows * (cols / 128) : 1))
+      throw std::runtime_error("s must be [R, C/128], or one value with HKMOE_SCALE_TENSOR");
+  }
+  check(hkmoe_rms_norm_quant(x.ptr, r.ptr, w.ptr, rows, cols, xt, wt, eps, scale_mode, static_cast<const float*>(sc.ptr),
+                             q.ptr, s.ptr, ro.ptr, no.ptr, ws.ptr, byte_size(ws, "workspace"), current_stream()));
+}
+
+void dispatch_router_logits(py::object x_, py::object w_, py::object logits_) {
+  auto x = as_tensor(x_, "x"), w = as_tensor(w_, "w"), l = as_tensor(logits_, "logits");
+  want_current_device({{&x_, "x"}, {&w_, "w"}, {&logits_, "logits"}});
+  want_dtype(x, "x", kBf16);
+  want_dtype(w, "w", kBf16);
+  want_dtype(l, "logits", kF32);
+  want_dim(x, "x", 2);
+  want_dim(w, "w", 2);
+  want_dim(l, "logits", 2);
+  if (w.shape[1] != x.shape[1]) throw std::runtime_error("x must be [T, H] and w [E, H]");
+  if (l.shape[0] != x.shape[0] || l.shape[1] != w.shape[0]) throw std::runtime_error("logits must be [T, E]");
+  if (w.shape[0] > kMaxInt) throw std::runtime_error("w: too many experts");
+  check(hkmoe_router_logits(x.ptr, w.ptr, x.shape[0], static_cast<int32_t>(w.shape[0]), x.shape[1],
+                            static_cast<float*>(l.ptr), current_stream()));
+}
+
+void dispatch_lora_add(py::object y_, py::object x_, py::object a_, py::object b_, py::object ids_, py::object scaling_,
+                       py::object out_, py::object workspace_) {
+  int64_t ys = 0, xs = 0, os = 0;
+  auto y = as_rows(y_, "y", &ys), x = as_rows(x_, "x", &xs), o = as_rows(out_, "out", &os);
+  auto a = as_tensor(a_, "a"), b = as_tensor(b_, "b"), i = as_tensor(ids_, "ids"), sc = as_tensor_opt(scaling_, "scaling"),
+       ws = as_tensor_opt(workspace_, "workspace");
+  want_current_device({{&y_, "y"}, {&x_, "x"}, {&a_, "a"}, {&b_, "b"}, {&ids_, "ids"}, {&scaling_, "scaling"}, {&out_, "out"},
+                       {&workspace_, "workspace"}});
+  const int yt = float_type(y, "y");
+  want_dtype(o, "out", y.dtype.name);
+  if (o.dtype != y.dtype.name) throw std::runtime_error("out must have y's dtype");
+  for (const auto& [t, name] : {std::pair(&x, "x"), std::pair(&a, "a"), std::pair(&b, "b")})
+    if (t->dtype != kBf16) throw std::runtime_error(std::string(name) + ": expected dtype torch.bfloat16");
+  if (i.dtype != kI32) throw std::runtime_error("ids: expected dtype torch.int32");
+  want_dtype(sc, "scaling", kF32);
+  want_dim(a, "a", 3);
+  want_dim(b, "b", 3);
+  const int64_t rows = y.shape[0], n = y.shape[1], adapters = a.shape[0], rank = a.shape[1], hidden = a.shape[2];
+  if (x.shape[0] != rows || x.shape[1] != hidden) throw std::runtime_error("x must be [T, H]");
+  if (b.shape[0] != adapters || b.shape[1] != n || b.shape[2] != rank)
+    throw std::runtime_error("a must be [L, R, H] and b [L, N, R]");
+  if (o.shape != y.shape) throw std::runtime_error("out must be [T, N]");
+  if (i.numel() != rows) throw std::runtime_error("ids must be [T]");
+  if (!scaling_.is_none() && sc.numel() != adapters) throw std::runtime_error("scaling must be [L]");
+  if (adapters > kMaxInt || rank > kMaxInt) throw std::runtime_error("a: too many adapters or ranks");
+  check(hkmoe_lora_add(y.ptr, ys, x.ptr, xs, a.ptr, b.ptr, static_cast<const int32_t*>(i.ptr),
+                       static_cast<const float*>(sc.ptr), rows, static_cast<int32_t>(adapters), hidden, n,
+                       static_cast<int32_t>(rank), yt, o.ptr, os, ws.ptr, byte_size(ws, "workspace"), current_stream()));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(tk_kernel, m) {
@@ -802,6 +939,19 @@ PYBIND11_MODULE(tk_kernel, m) {
         py::arg("out"), py::arg("workspace"), py::arg("packed") = true);
   m.def("dispatch_gemm_mx", &dispatch_gemm_mx, "C = A . B^T with 1x32 e8m0 scales (packed words)",
         py::arg("A"), py::arg("scale_a"), py::arg("B"), py::arg("scale_b"), py::arg("C"));
+  m.def("dispatch_rms_norm_quant", &dispatch_rms_norm_quant,
+        "residual_out = x + residual; q, s = the e4m3 operand of its rms norm (and the bf16 norm)", py::arg("x"),
+        py::arg("residual"), py::arg("weight"), py::arg("eps"), py::arg("scale_mode"), py::arg("q"), py::arg("s"),
+        py::arg("scale") = py::none(), py::arg("residual_out") = py::none(), py::arg("norm_out") = py::none(),
+        py::arg("workspace") = py::none());
+  m.def("dispatch_router_logits", &dispatch_router_logits, "logits = x . w^T (bf16 in, fp32 out)", py::arg("x"),
+        py::arg("w"), py::arg("logits"));
+  m.def("dispatch_lora_add", &dispatch_lora_add, "out = y + scaling[ids] (x A[ids]^T) B[ids]^T", py::arg("y"),
+        py::arg("x"), py::arg("a"), py::arg("b"), py::arg("ids"), py::arg("scaling"), py::arg("out"),
+        py::arg("workspace"));
+  m.def("rms_norm_quant_workspace_size", &hkmoe_rms_norm_quant_workspace_size, py::arg("rows"), py::arg("scale_mode"),
+        py::arg("given_scale"));
+  m.def("lora_workspace_size", &hkmoe_lora_workspace_size, py::arg("rows"), py::arg("hidden"), py::arg("rank"));
   m.def("moe_workspace_size", &moe_workspace_size);
   m.def("set_narrow", [](int cus, int max_rows, int wide_share) { check(hkmoe_set_narrow(cus, max_rows, wide_share)); },
         "narrow path of dispatch_moe: workgroups (0 = off), largest expert it takes, wide-GEMM CU share",

@@ -13,6 +13,11 @@ Entry points
   hkmoe.moe_forward_steps   the same layer one kernel at a time, returning
                             every intermediate (for parity tests)
   hkmoe.quant_*             device quantisers (per-tensor, 1x128, 128x128)
+  hkmoe.rms_norm_quant      residual + norm + e4m3 operand in one pass
+  hkmoe.router_logits       the router's product
+  hkmoe.lora_add            adapters of many requests beside a projection
+  hkmoe.MoEBlock            norm, router and layer; hkmoe.LoraLinear: projection
+                            and adapters
 """
 import os
 import sys
@@ -32,6 +37,7 @@ except ImportError as exc:  # pragma: no cover - exercised only on a broken tree
 from .layer import (MoELayer, moe_forward, moe_forward_steps, pack_weights,  # noqa: E402
                     quant_block, quant_group, quant_tensor, gemm_fp8, quant_mx, mx_pack_scales, gemm_mx,
                     mx_pack_weight_scales, moe_forward_mx_steps, MoELayerMX)
+from .block import LoraLinear, MoEBlock, lora_add, rms_norm_quant, router_logits  # noqa: E402
 
 LIB_PATH = os.path.join(_PKG_ROOT, "libhkmoe.so")
 SCALE_TENSOR = tk_kernel.SCALE_TENSOR
@@ -39,5 +45,6 @@ SCALE_BLOCK = tk_kernel.SCALE_BLOCK
 
 __all__ = ["tk_kernel", "MoELayer", "moe_forward", "moe_forward_steps", "pack_weights", "quant_block",
            "quant_group", "quant_tensor", "gemm_fp8", "quant_mx", "mx_pack_scales", "gemm_mx",
-           "mx_pack_weight_scales", "moe_forward_mx_steps", "MoELayerMX", "LIB_PATH",
+           "mx_pack_weight_scales", "moe_forward_mx_steps", "MoELayerMX", "rms_norm_quant", "router_logits",
+           "lora_add", "LoraLinear", "MoEBlock", "LIB_PATH",
            "SCALE_TENSOR", "SCALE_BLOCK"]

@@ -404,6 +404,60 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
                        float* amax_ws, hkmoe_stream_t stream);
 
 /*
+ * What stands between a residual stream and the FP8 products.  No reference
+ * counterpart (the reference has no norm, router or adapters).  All tensors are
+ * row-major and 16-byte aligned, rows at most 2^26; no entry point reads an output.
+ *
+ * hkmoe_rms_norm_quant: the residual's addition, the norm and the e4m3 operand.
+ *     r = x + residual, rounded to x's type (written to residual_out)
+ *     rstd = fl32(1 / sqrt(mean_j r_j^2 + eps)), mean and root in 64 bits
+ *     n_j = fl32(fl32(r_j * rstd) * weight_j)
+ *   x, residual, residual_out [R, C] bf16 or fp32 (x_dtype; residual and
+ *   residual_out both NULL: r = x; residual_out may be x or residual itself),
+ *   weight [C] bf16 or fp32, q [R, C] e4m3, norm_out NULL or n as bf16 [R, C].
+ *     HKMOE_SCALE_BLOCK   s [R, C/128] fp32, C % 128 == 0   (as hkmoe_quant_group)
+ *     HKMOE_SCALE_MX      s [R, C/32] e8m0, C % 32 == 0     (as hkmoe_quant_mx)
+ *     HKMOE_SCALE_TENSOR  C % 8 == 0; scale NULL: s [1] = scale of max |n|, with the
+ *                         workspace below; else *scale (device, positive and finite)
+ *                         is used, values past 448 scale saturate, and s is unused.
+ *   C <= 65536.  Scales and bytes are those of the quantisers above for n, bit
+ *   for bit, non-finite n included.  R = 0 writes nothing but s of
+ *   HKMOE_SCALE_TENSOR without a given scale (1).
+ *
+ * hkmoe_router_logits: logits [T, E] fp32 = x [T, H] . w [E, H]^T, bf16 operands,
+ *   fp32 sums: the logits of hkmoe_route_topk and the layers.  H % 8 == 0,
+ *   H <= 2^20, 1 <= E <= 1024.
+ *
+ * hkmoe_lora_add: out[t] = y[t] + scaling[l] * (x[t] A_l^T) B_l^T with l = ids[t],
+ *   the low-rank adapters of a batch's requests beside a projection that computed y.
+ *   Rows whose id is outside [0, adapters) have none: out[t] = y[t].
+ *   y [T, N] and out [T, N] bf16 or fp32 (y_dtype), x [T, H] bf16, their rows y_stride,
+ *   out_stride and x_stride elements apart (16-byte multiples; slices of wider buffers);
+ *   a [adapters, rank, H], b [adapters, N, rank] bf16 contiguous, ids [T] int32,
+ *   scaling [adapters] fp32 or NULL (1).  out may be y itself (with its stride; rows
+ *   without an adapter are then not touched) and overlaps nothing else.
+ *   H % 8 == 0, N % 8 == 0, rank % 8 == 0, rank <= 256, H <= 2^20, N <= 2^24; pad
+ *   smaller ranks with zeros.  v = x A_l^T is kept to 2^-17 (fp32 y: 2^-25) of its
+ *   value; an infinite value of A or B gives an infinity or a NaN.
+ *   workspace: hkmoe_lora_workspace_size(T, H, rank) bytes, not shared by calls that
+ *   overlap in time.
+ * Results are deterministic, but the sums' order follows from the shapes: a row's last
+ * bits may differ with the number of rows beside it.
+ */
+size_t hkmoe_rms_norm_quant_workspace_size(int64_t rows, int scale_mode, int given_scale);
+int hkmoe_rms_norm_quant(const void* x, const void* residual, const void* weight, int64_t rows, int64_t cols,
+                         int x_dtype, int weight_dtype, double eps, int scale_mode, const float* scale, void* q, void* s,
+                         void* residual_out, void* norm_out, void* workspace, size_t workspace_bytes,
+                         hkmoe_stream_t stream);
+int hkmoe_router_logits(const void* x, const void* w, int64_t num_tokens, int32_t num_experts, int64_t hidden,
+                        float* logits, hkmoe_stream_t stream);
+size_t hkmoe_lora_workspace_size(int64_t rows, int64_t hidden, int32_t rank);
+int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* a, const void* b,
+                   const int32_t* ids, const float* scaling, int64_t rows, int32_t adapters, int64_t hidden, int64_t n,
+                   int32_t rank, int y_dtype, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                   hkmoe_stream_t stream);
+
+/*
  * MX (microscaling) FP8: e4m3 elements with one e8m0 exponent per row and
  * 32-element K block.  An e8m0 byte s stands for 2^(s - 127).
  *

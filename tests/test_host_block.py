@@ -1,0 +1,134 @@
+"""Norm, router and adapters: what the host refuses, and what it launches (no GPU)."""
+import ctypes
+import os
+
+import pytest
+
+import hip_host
+
+P = ctypes.c_void_p(0x1000)  # never dereferenced: validation fails first
+ODD = ctypes.c_void_p(0x1008)
+i64, i32, dbl, size = ctypes.c_int64, ctypes.c_int32, ctypes.c_double, ctypes.c_size_t
+
+
+@pytest.fixture(scope="module")
+def lib():
+    lib = ctypes.CDLL(os.environ.get("HKMOE_LIB") or hip_host.LIB)
+    lib.hkmoe_last_error.restype = ctypes.c_char_p
+    lib.hkmoe_lora_workspace_size.restype = size
+    lib.hkmoe_rms_norm_quant_workspace_size.restype = size
+    return lib
+
+
+def _norm(lib, x=P, residual=None, weight=P, rows=4, cols=256, xt=0, wt=0, eps=1e-6, mode=1, scale=None, q=P, s=P,
+          residual_out=None, norm=None, ws=None, ws_bytes=0):
+    return lib.hkmoe_rms_norm_quant(x, residual, weight, i64(rows), i64(cols), xt, wt, dbl(eps), mode, scale, q, s,
+                                    residual_out, norm, ws, size(ws_bytes), None)
+
+
+@pytest.mark.parametrize("bad,says", [
+    (dict(x=None), "null"), (dict(weight=None), "null"), (dict(q=None), "null"), (dict(s=None), "null"),
+    (dict(rows=-1), "shape"), (dict(cols=0), "shape"), (dict(rows=1 << 27), "shape"), (dict(cols=200), "multiple of 128"),
+    (dict(cols=40, mode=2), "multiple of 32"), (dict(cols=4, mode=0), "multiple of 8"), (dict(cols=65664), "65536"),
+    (dict(xt=2), "dtype"), (dict(wt=5), "dtype"), (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"),
+    (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"), (dict(mode=3), "scale_mode"),
+    (dict(scale=P), "given scale"), (dict(residual=P), "together"), (dict(residual_out=P), "together"),
+    (dict(x=ODD), "aligned"), (dict(q=ODD), "aligned"), (dict(norm=ODD), "aligned"), (dict(weight=ODD), "aligned")])
+def test_norm_refusals(lib, bad, says):
+    assert _norm(lib, **bad) == 1
+    assert says in lib.hkmoe_last_error().decode()
+
+
+def test_norm_workspace(lib):
+    need = lib.hkmoe_rms_norm_quant_workspace_size(i64(4), 0, 0)
+    assert need >= 4 * 4 and lib.hkmoe_rms_norm_quant_workspace_size(i64(4), 0, 1) == 0
+    assert lib.hkmoe_rms_norm_quant_workspace_size(i64(4), 1, 0) == 0
+    assert _norm(lib, mode=0) == 4 and _norm(lib, mode=0, ws=P, ws_bytes=need - 1) == 4
+    assert _norm(lib, mode=0, ws=ODD, ws_bytes=need) == 4
+
+
+def test_norm_no_rows_takes_null_buffers(lib):
+    assert _norm(lib, rows=0, x=None, q=None, s=None) == 0
+    assert _norm(lib, rows=0, x=None, q=None, s=None, mode=0, scale=P) == 0
+    assert _norm(lib, rows=0, x=None, q=None, s=None, mode=0) == 1  # its scale is still an output
+
+
+@pytest.mark.parametrize("bad,says", [
+    (dict(x=None), "null"), (dict(w=None), "null"), (dict(logits=None), "null"), (dict(t=-1), "shape"),
+    (dict(e=0), "shape"), (dict(e=1025), "shape"), (dict(h=0), "multiple of 8"), (dict(h=12), "multiple of 8"),
+    (dict(h=(1 << 20) + 8), "2^20"), (dict(x=ODD), "aligned"), (dict(w=ODD), "aligned"), (dict(t=1 << 27), "shape")])
+def test_router_refusals(lib, bad, says):
+    a = dict(x=P, w=P, t=4, e=8, h=64, logits=P)
+    a.update(bad)
+    assert lib.hkmoe_router_logits(a["x"], a["w"], i64(a["t"]), i32(a["e"]), i64(a["h"]), a["logits"], None) == 1
+    assert says in lib.hkmoe_last_error().decode()
+
+
+def _lora(lib, y=P, ys=64, x=P, xs=256, a=P, b=P, ids=P, scaling=None, rows=4, adapters=2, h=256, n=64, r=8, yt=0, out=P,
+          os_=64, ws=P, ws_bytes=1 << 40):
+    return lib.hkmoe_lora_add(y, i64(ys), x, i64(xs), a, b, ids, scaling, i64(rows), i32(adapters), i64(h), i64(n), i32(r), yt,
+                              out, i64(os_), ws, size(ws_bytes), None)
+
+
+@pytest.mark.parametrize("bad,says", [
+    (dict(y=None), "null"), (dict(x=None), "null"), (dict(a=None), "null"), (dict(b=None), "null"), (dict(ids=None), "null"),
+    (dict(out=None), "null"), (dict(rows=-1), "shape"), (dict(rows=1 << 27), "shape"), (dict(adapters=0), "shape"),
+    (dict(h=12), "multiples of 8"), (dict(n=60), "multiples of 8"), (dict(n=0), "multiples of 8"), (dict(r=12), "rank"),
+    (dict(r=0), "rank"), (dict(r=264), "rank"), (dict(yt=2), "y_dtype"), (dict(xs=248), "strides"), (dict(xs=260), "strides"),
+    (dict(ys=56), "strides"), (dict(ys=68), "strides"), (dict(os_=60), "strides"), (dict(yt=1, ys=66), "strides"),
+    (dict(os_=72), "row stride"), (dict(y=ODD), "aligned"), (dict(x=ODD), "aligned"), (dict(out=ODD), "aligned"),
+    (dict(a=ODD), "aligned"), (dict(b=ODD), "aligned"), (dict(ids=ctypes.c_void_p(0x1002)), "aligned")])
+def test_lora_refusals(lib, bad, says):
+    assert _lora(lib, **bad) == 1
+    assert says in lib.hkmoe_last_error().decode()
+
+
+def test_lora_workspace(lib):
+    need = lib.hkmoe_lora_workspace_size(i64(4), i64(256), i32(8))
+    assert need >= 4 * 8 * 4 and lib.hkmoe_lora_workspace_size(i64(0), i64(256), i32(8)) == 0
+    assert _lora(lib, ws=None) == 4 and _lora(lib, ws_bytes=need - 1) == 4 and _lora(lib, ws=ODD) == 4
+    assert _lora(lib, rows=0, y=None, x=None, ids=None, out=None, ws=None, ws_bytes=0) == 0
+
+
+def test_python_refuses_cpu_tensors():
+    import torch
+    hkmoe = pytest.importorskip("hkmoe")
+    x = torch.zeros((4, 256), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        hkmoe.rms_norm_quant(x, x[0])
+    with pytest.raises(RuntimeError):
+        hkmoe.router_logits(x, x)
+    with pytest.raises(RuntimeError):
+        hkmoe.lora_add(x, x, x[None], x[None], torch.zeros(4, dtype=torch.int32))
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    return hip_host.build_fake(str(tmp_path_factory.mktemp("hip")))
+
+
+def test_grids_stay_in_range(fake):
+    """The largest sizes that are taken launch with every dimension below 2^32 work-items."""
+    out = hip_host.run(fake, """
+        size, dbl = ctypes.c_size_t, ctypes.c_double
+        big, st = 1 << 26, vp(5)
+        lib.hkmoe_lora_workspace_size.restype = size
+        for rows in (1, 64, 5000, big):
+            for cols in (8, 128, 65536):
+                for mode in (0, 1, 2):
+                    if mode and cols == 8: continue
+                    assert lib.hkmoe_rms_norm_quant(P, None, P, i64(rows), i64(cols), 0, 0, dbl(1e-6), mode, None, P, P, None,
+                                                    None, P, size(1 << 50), st) == 0
+            for e in (1, 256, 1024):
+                assert lib.hkmoe_router_logits(P, P, i64(rows), i32(e), i64(4096), P, st) == 0
+            for n in (8, 4096, 1 << 24):
+                for yt in (0, 1):
+                    assert lib.hkmoe_lora_add(P, i64(n), P, i64(256), P, P, P, None, i64(rows), i32(1000), i64(256), i64(n),
+                                              i32(16), yt, P, i64(n), P, size(1 << 50), st) == 0
+        for line in log(): print(line)
+    """)
+    launches = [l for l in out if l.startswith("launch")]
+    assert launches and all(l.endswith("stream=5") for l in launches)
+    for l in launches:
+        grid = int(l.split("grid=")[1].split()[0])
+        assert 1 <= grid and grid * (1024 if "norm" in l else 256) < 1 << 32, l
