@@ -647,11 +647,58 @@ int launch_norm(const NormParams& p, int mode, hipStream_t s) {
   return check_launch("norm_quant_tensor_kernel");
 }
 
+template <typename P>
+int launch_router_panel(const RouterParams& p, hipStream_t s) {
+  static bool attr_set[kMaxDevices] = {false};
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  auto kern = router_panel_kernel<P>;
+  if (dev >= 0 && dev < kMaxDevices && !attr_set[dev]) {
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, P::kLds);
+    if (err != hipSuccess) return fail(HKMOE_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(err));
+    attr_set[dev] = true;
+  }
+  const int64_t rt = (p.rows + P::BM - 1) / P::BM, ct = (p.experts + P::BN - 1) / P::BN;
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((rt + 7) / 8 * 8 * ct)), dim3(P::kWaves * 64), P::kLds, s, p,
+                     static_cast<int>(rt), static_cast<int>(ct));
+  return check_launch("router_panel_kernel");
+}
+
+template <int MT, int NT, int WAVES, int DEPTH>
+int launch_router(const RouterParams& p, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((p.rows + 16 * MT - 1) / (16 * MT)), static_cast<unsigned>((p.experts + 16 * NT - 1) / (16 * NT)));
+  hipLaunchKernelGGL((router_kernel<MT, NT, WAVES, DEPTH>), grid, dim3(WAVES * 64), 0, s, p);
+  return check_launch("router_kernel");
+}
+
+int launch_router(const RouterParams& p, hipStream_t s) {
+  const int64_t tiles = (p.rows + 15) / 16 * ((p.experts + 15) / 16);
+  if (tiles <= 512) return launch_router<1, 1, 16, 4>(p, s);
+  if (tiles <= 2048) return launch_router<1, 4, 8, 2>(p, s);
+  return launch_router_panel<Panel<64, 128, 2, 4, 4>>(p, s);
+}
+
+template <bool F32, int TERMS>
+int launch_lora_expand(const LoraParams& p, dim3 grid, hipStream_t s) {
+  static bool attr_set[kMaxDevices] = {false};
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  auto kern = lora_expand_kernel<F32, TERMS>;
+  if (dev >= 0 && dev < kMaxDevices && !attr_set[dev]) {
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                               lora_lds_bytes(kLoraMaxRank, TERMS));
+    if (err != hipSuccess) return fail(HKMOE_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(err));
+    attr_set[dev] = true;
+  }
+  hipLaunchKernelGGL(kern, grid, dim3(kLoraWaves * 64), lora_lds_bytes(p.rank, TERMS), s, p);
+  return check_launch("lora_expand_kernel");
+}
+
 // Workgroups over which the adapters' narrow product splits its K steps: enough to
 // fill the chip, at least one step per wave.
 int lora_splits(int64_t rows, int64_t hidden) {
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock, steps = (hidden + kRowsStep - 1) / kRowsStep;
-  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, steps / kRowsWaves));
+  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, steps / kLoraWaves));
   return static_cast<int>(std::min(most, std::max<int64_t>(1, 512 / std::max<int64_t>(1, blocks))));
 }
 
@@ -1540,9 +1587,7 @@ int hkmoe_router_logits(const void* x, const void* w, int64_t num_tokens, int32_
   if (num_tokens == 0) return HKMOE_OK;
   RouterParams p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w), logits, num_tokens, num_experts,
                  static_cast<int32_t>(hidden)};
-  const dim3 grid(static_cast<unsigned>((num_tokens + 15) / 16), static_cast<unsigned>((num_experts + 63) / 64));
-  hipLaunchKernelGGL((router_kernel<1, 4>), grid, dim3(kRowsWaves * 64), 0, static_cast<hipStream_t>(stream), p);
-  return check_launch("router_kernel");
+  return launch_router(p, static_cast<hipStream_t>(stream));
 }
 
 size_t hkmoe_lora_workspace_size(int64_t rows, int64_t hidden, int32_t rank) {
@@ -1594,20 +1639,16 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
   p.splits = lora_splits(rows, hidden);
   auto s = static_cast<hipStream_t>(stream);
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock;
-  // distinct adapters a block can have, as far as a few thousand workgroups go: the
-  // others follow in the same workgroups
-  const int64_t most = std::min<int64_t>({kRowsBlock, rows, static_cast<int64_t>(adapters) + 1});
-  auto at_a_time = [&](int64_t per) { return static_cast<unsigned>(std::max<int64_t>(1, std::min(most, 4096 / (blocks * per)))); };
-  hipLaunchKernelGGL(lora_shrink_kernel, dim3(static_cast<unsigned>(blocks), at_a_time(p.splits), p.splits),
-                     dim3(kRowsWaves * 64), 0, s, p);
+  const unsigned grid_x = static_cast<unsigned>(blocks <= 8 ? blocks : (blocks + 7) / 8 * 8);
+  // parts of a block's adapters: one per row as far as two workgroups per CU go
+  auto parts = [&](int64_t per) { return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(kRowsBlock, 1024 / (blocks * per)))); };
+  hipLaunchKernelGGL((rank <= 16 ? lora_shrink_kernel<1> : rank <= 32 ? lora_shrink_kernel<2> : lora_shrink_kernel<4>),
+                     dim3(grid_x, parts(p.splits), p.splits), dim3(kLoraWaves * 64), 0, s, p);
   HK_TRY(check_launch("lora_shrink_kernel"));
-  const int64_t strips = (n + 255) / 256;
-  const int64_t parts = std::min<int64_t>({strips, 65535, std::max<int64_t>(1, 1024 / blocks)});
-  p.cols_per_wg = static_cast<int32_t>((strips + parts - 1) / parts * 256);
-  const dim3 grid(static_cast<unsigned>(blocks), at_a_time(parts), static_cast<unsigned>((n + p.cols_per_wg - 1) / p.cols_per_wg));
-  hipLaunchKernelGGL((y_dtype == HKMOE_F32 ? lora_expand_kernel<true, 3> : lora_expand_kernel<false, 2>), grid,
-                     dim3(kRowsWaves * 64), 0, s, p);
-  return check_launch("lora_expand_kernel");
+  const int64_t strips = (n + 255) / 256, cols = std::min<int64_t>({strips, 65535, std::max<int64_t>(1, 512 / blocks)});
+  p.cols_per_wg = static_cast<int32_t>((strips + cols - 1) / cols * 256);
+  const dim3 grid(grid_x, parts(cols), static_cast<unsigned>((n + p.cols_per_wg - 1) / p.cols_per_wg));
+  return y_dtype == HKMOE_F32 ? launch_lora_expand<true, 3>(p, grid, s) : launch_lora_expand<false, 2>(p, grid, s);
 }
 
 // ---------------------------------------------------------------------------
