@@ -118,72 +118,137 @@ struct Panel {
   static constexpr int kLoads = (BM + BN) / 8 / kWaves;  // DMA instructions per wave and step
   static constexpr int kStage = (BM + BN) * 2 * kRowsStep;
   static constexpr int kLds = STAGES * kStage;
-  static_assert((BM + BN) % (8 * kWaves) == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "tile");
-  static_assert(STAGES >= 2 && STAGES <= 4, "small_wait_stage covers at most 3 newer stages");
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "tile");
+  static_assert(STAGES >= 2 && (STAGES - 1) * kLoads <= 63, "ring depth, vmcnt range");
 };
 
-// acc += the tile over K steps s0 .. s1 - 1.  row_of(i): row i of the BM rows of x, then of
-// the BN rows of w (16-byte aligned; rows past the last may repeat a valid one).  Every wave of the workgroup calls it; on return all
-// are done with smem.
-template <typename P, typename RowOf>
-__device__ __forceinline__ void panel_product(uint8_t* smem, RowOf row_of, int K, int s0, int s1, f32x4 (&acc)[P::MT][P::NT]) {
+// vmcnt wait that leaves this wave's loads of the newest `newer` (at most MOST) stages in
+// flight, L loads each, then a barrier: every wave's loads of the older ones are in LDS, and
+// every wave's LDS reads are done.  The compiler's own s_waitcnt (simm16: vmcnt in bits 0-3
+// and 14-15, lgkmcnt in 8-11), so that it knows the fragments read so far to be complete
+// and adds no lgkmcnt(0) between the next step's reads and this step's products (55 us
+// with one, 8192x7168x256).
+template <int L, int MOST>
+__device__ __forceinline__ void panel_wait(int newer) {
+  if constexpr (MOST > 0) {
+    if (newer < MOST) return panel_wait<L, MOST - 1>(newer);
+  }
+  constexpr int kVm = L * MOST;
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((kVm & 15) | (kVm >> 4) << 14 | 0x70);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// acc += the tile over K steps s0 .. s1 - 1.  x, w: bases that the whole workgroup shares;
+// x_off(i), w_off(i): byte offset from them (below 2^32 - 2^22, a multiple of 16) of row i
+// of the BM rows and of the BN columns; rows past the last may repeat a valid one.
+// Step kt's products run beside the LDS reads of step kt + 1 (two register sets) and the DMA
+// of the steps after it.  Every wave of the workgroup calls it; on return all are done with
+// smem.
+template <typename P, typename XOff, typename WOff>
+__device__ __forceinline__ void panel_product(uint8_t* smem, const uint16_t* x, XOff x_off, const uint16_t* w, WOff w_off, int K,
+                                              int s0, int s1, f32x4 (&acc)[P::MT][P::NT]) {
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, lg = lane >> 4, wm = wave / P::WN, wn = wave % P::WN;
-  const uint16_t* src[P::kLoads];
-  int off[P::kLoads];  // K offset of this lane's chunk in a step
+  constexpr int kAhead = P::STAGES - 1, kXLoads = P::BM / 8 / P::kWaves;
+  const i32x4 x_srd = make_srd(x, 0xffffffffu), w_srd = make_srd(w, 0xffffffffu);
+  uint32_t off[P::kLoads];
+  int chunk[P::kLoads];  // this lane's chunk of a step
 #pragma unroll
-  for (int i = 0; i < P::kLoads; ++i) {
-    const int r = 8 * (wave + P::kWaves * i) + (lane >> 3);
-    off[i] = 8 * ((lane & 7) ^ swz(r));
-    src[i] = row_of(r) + off[i];
+  for (int u = 0; u < P::kLoads; ++u) {
+    const int r = 8 * (wave + P::kWaves * u) + (lane >> 3);
+    chunk[u] = (lane & 7) ^ swz(r);
+    off[u] = (u < kXLoads ? x_off(r) : w_off(r - P::BM)) + 16 * chunk[u];
   }
   const int n = s1 - s0;
-  auto issue = [&](int i) __attribute__((always_inline)) {
+  // DMA of step i.  The last one of K % 64 != 0 takes the step's first chunk in the place of
+  // those past the row; their products are cut below.
+  auto issue = [&](int i, auto ragged) __attribute__((always_inline)) {
     uint8_t* st = smem + (i % P::STAGES) * P::kStage;
     const int k0 = (s0 + i) * kRowsStep;
-    const bool ragged = k0 + kRowsStep > K;
 #pragma unroll
     for (int u = 0; u < P::kLoads; ++u) {
-      const uint16_t* at = src[u] + k0;
-      if (ragged && k0 + off[u] >= K) at = src[u] - off[u];  // past the row: any of its chunks, zeroed below
-      __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(at)),
-                                       reinterpret_cast<HK_LDS void*>(reinterpret_cast<uintptr_t>(st + (wave + P::kWaves * u) * 1024)),
-                                       16, 0, 0);
+      uint32_t at = off[u];
+      if constexpr (decltype(ragged)::value) {
+        if (k0 + 8 * chunk[u] >= K) at -= 16 * chunk[u];
+      }
+      load_lds_16B(u < kXLoads ? x_srd : w_srd, st + (wave + P::kWaves * u) * 1024, static_cast<int>(at), 2 * k0);
     }
   };
-  const int pre = min(P::STAGES - 1, n);
-  for (int i = 0; i < pre; ++i) issue(i);
   const int fx = swz(l16);
-  for (int i = 0; i < n; ++i) {
-    small_wait_stage<P::kLoads>(min(P::STAGES - 2, n - 1 - i));
-    if (i + P::STAGES - 1 < n) issue(i + P::STAGES - 1);  // into the slot that every wave has read
-    const uint8_t* st = smem + (i % P::STAGES) * P::kStage;
+  struct Frags {
     bf16x8 a[2][P::MT], b[2][P::NT];
+  };
+  auto read = [&](int i, Frags& f) __attribute__((always_inline)) {
+    const uint8_t* st = smem + (i % P::STAGES) * P::kStage;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int slot = ((4 * h + lg) ^ fx) * 16;
 #pragma unroll
-      for (int j = 0; j < P::MT; ++j) a[h][j] = *reinterpret_cast<const bf16x8*>(st + (16 * (wm * P::MT + j) + l16) * 128 + slot);
+      for (int j = 0; j < P::MT; ++j) f.a[h][j] = *reinterpret_cast<const bf16x8*>(st + (16 * (wm * P::MT + j) + l16) * 128 + slot);
 #pragma unroll
-      for (int j = 0; j < P::NT; ++j) b[h][j] = *reinterpret_cast<const bf16x8*>(st + (P::BM + 16 * (wn * P::NT + j) + l16) * 128 + slot);
+      for (int j = 0; j < P::NT; ++j) f.b[h][j] = *reinterpret_cast<const bf16x8*>(st + (P::BM + 16 * (wn * P::NT + j) + l16) * 128 + slot);
     }
-    if ((s0 + i + 1) * kRowsStep > K) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if ((s0 + i) * kRowsStep + 32 * h + 8 * lg >= K) {
-#pragma unroll
-          for (int j = 0; j < P::MT; ++j) a[h][j] = zero_bf16x8();
-#pragma unroll
-          for (int j = 0; j < P::NT; ++j) b[h][j] = zero_bf16x8();
-        }
-      }
-    }
+  };
+  auto mma = [&](const Frags& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int j = 0; j < P::MT; ++j)
 #pragma unroll
-        for (int l = 0; l < P::NT; ++l) acc[j][l] = mfma_bf16_16x16x32(a[h][j], b[h][l], acc[j][l]);
+        for (int l = 0; l < P::NT; ++l) acc[j][l] = mfma_bf16_16x16x32(f.a[h][j], f.b[h][l], acc[j][l]);
+  };
+  // K's last step, K % 64 != 0: both operands 0 past K
+  auto cut = [&](int i, Frags& f) __attribute__((always_inline)) {
+    if ((s0 + i + 1) * kRowsStep <= K) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if ((s0 + i) * kRowsStep + 32 * h + 8 * lg < K) continue;
+#pragma unroll
+      for (int j = 0; j < P::MT; ++j) f.a[h][j] = zero_bf16x8();
+#pragma unroll
+      for (int j = 0; j < P::NT; ++j) f.b[h][j] = zero_bf16x8();
+    }
+  };
+  if (n > 0) {
+    const int pre = min(kAhead, n);
+    for (int i = 0; i < pre; ++i) issue(i, std::true_type{});
+    panel_wait<P::kLoads, kAhead - 1>(pre - 1);
+    Frags f0, f1;
+    read(0, f0);
+    // Step i: DMA of step i + kAhead into the slot of step i - 1 (its reads are complete at
+    // step i - 1's barrier), step i + 1's fragments, step i's products.
+    auto step_full = [&](int i, Frags& cur, Frags& next) __attribute__((always_inline)) {
+      issue(i + kAhead, std::false_type{});
+      panel_wait<P::kLoads, kAhead - 1>(kAhead - 1);
+      read(i + 1, next);
+      __builtin_amdgcn_sched_barrier(0);
+      mma(cur);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](int i, Frags& cur, Frags& next) __attribute__((always_inline)) {
+      if (i + kAhead < n) issue(i + kAhead, std::true_type{});
+      if (i + 1 < n) {
+        panel_wait<P::kLoads, kAhead - 1>(min(kAhead - 1, n - 2 - i));
+        read(i + 1, next);
+      } else {
+        cut(i, cur);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      mma(cur);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    int i = 0;
+    for (; i + 2 + kAhead < n; i += 2) {  // the DMA of all but K's last step
+      step_full(i, f0, f1);
+      step_full(i + 1, f1, f0);
+    }
+    for (; i + 1 < n; i += 2) {
+      step(i, f0, f1);
+      step(i + 1, f1, f0);
+    }
+    if (i < n) step(i, f0, f1);
   }
   __syncthreads();
 }
@@ -231,11 +296,11 @@ __global__ __launch_bounds__(P::kWaves * 64) void router_panel_kernel(RouterPara
   const int col0 = ct * P::BN;
   const int lane = lane_id(), wave = threadIdx.x >> 6;
   f32x4 acc[P::MT][P::NT] = {};
-  auto row_of = [&](int i) __attribute__((always_inline)) {
-    return i < P::BM ? p.x + min(row0 + i, p.rows - 1) * p.hidden
-                     : p.w + static_cast<int64_t>(min(col0 + i - P::BM, p.experts - 1)) * p.hidden;
-  };
-  panel_product<P>(smem, row_of, p.hidden, 0, (p.hidden + kRowsStep - 1) / kRowsStep, acc);
+  const int last = static_cast<int>(min(static_cast<int64_t>(P::BM), p.rows - row0)) - 1;
+  const uint32_t pitch = 2 * static_cast<uint32_t>(p.hidden);  // H <= 2^20: 64 rows, 1024 experts stay below 2^32
+  panel_product<P>(
+      smem, p.x + row0 * p.hidden, [&](int i) { return min(i, last) * pitch; }, p.w,
+      [&](int i) { return min(col0 + i, p.experts - 1) * pitch; }, p.hidden, 0, (p.hidden + kRowsStep - 1) / kRowsStep, acc);
 #pragma unroll
   for (int j = 0; j < P::MT; ++j)
 #pragma unroll
@@ -357,11 +422,11 @@ __device__ __forceinline__ void lora_shrink_panel(const LoraParams& p, int64_t t
   const int s0 = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
   const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
   f32x4 acc[P::MT][P::NT] = {};
-  auto row_of = [&](int i) __attribute__((always_inline)) {
-    return i < P::BM ? p.x + (t0 + list[min(i, n - 1)]) * p.x_stride
-                     : p.a + (static_cast<int64_t>(id) * p.rank + min(r0 + i - P::BM, p.rank - 1)) * p.hidden;
-  };
-  panel_product<P>(smem, row_of, p.hidden, s0, s1, acc);
+  // the host keeps 64 rows of x and the ranks of an adapter below 2^32 bytes
+  panel_product<P>(
+      smem, p.x + t0 * p.x_stride, [&](int i) { return list[min(i, n - 1)] * static_cast<uint32_t>(2 * p.x_stride); },
+      p.a + static_cast<int64_t>(id) * p.rank * p.hidden,
+      [&](int i) { return min(r0 + i, p.rank - 1) * static_cast<uint32_t>(2 * p.hidden); }, p.hidden, s0, s1, acc);
   float* v = p.v + (split * p.rows + t0) * p.rank;
 #pragma unroll
   for (int j = 0; j < P::MT; ++j)
@@ -415,56 +480,74 @@ __device__ __forceinline__ void split_bf16(float v, uint16_t (&t)[TERMS]) {
 
 constexpr int kLoraPad = 8;  // LDS row pitch: off a multiple of the banks' width, 16-byte aligned
 constexpr int lora_pitch(int rank) { return (rank + 31) / 32 * 32 + kLoraPad; }
-constexpr int lora_lds_bytes(int rank, int terms) { return terms * kRowsBlock * lora_pitch(rank) * 2; }
 
-// out of one adapter's rows, two tiles of 16 at a time.  The operands are swapped (B rows
-// first), and result row 4g + i of column tile jt is column 16g + 4jt + i: a lane then
-// holds 16 adjacent columns of one row, and a wave whole 128-byte lines of it (bf16).  y
-// comes in while the products run and is added last.  ONE: the rank fits one step of 64,
-// and B is read once for all the rows.
-template <bool F32, int TERMS, bool ONE>
+// A wave's 16 x 64 products on their way from operand order to rows, fp32.
+constexpr int kLoraTilePitch = 68;
+constexpr int lora_lds_bytes(int rank, int terms) {
+  return terms * kRowsBlock * lora_pitch(rank) * 2 + kLoraWaves * 16 * kLoraTilePitch * 4;
+}
+
+// 16 bytes of y / out.  NT: more than the L2s hold, touched once: 8192x4096 bf16 read and
+// written in these pieces 26 us, with plain accesses 38; straight from operand order, 16
+// rows of 64 bytes an access, 43.
+template <bool NT>
+__device__ __forceinline__ uint4 lora_load(const void* p) {
+  if constexpr (NT) return ld_nt16(p);
+  return *static_cast<const uint4*>(p);
+}
+template <bool NT>
+__device__ __forceinline__ void lora_store(void* p, uint4 v) {
+  if constexpr (NT) st_nt16(p, v);
+  else *static_cast<uint4*>(p) = v;
+}
+
+// out of one adapter's rows, two tiles of 16 at a time, a wave 64 columns.  With B as the
+// first operand a lane holds 4 adjacent columns of one row; the wave turns the tile round in
+// LDS, so that y and out are accessed in whole 128-byte lines (fp32: two), the fp32 sum
+// rounded once.  ONE: the rank fits one step of 64, and B is read once for all the rows.
+template <bool F32, int TERMS, bool NT, bool ONE>
 __device__ __forceinline__ void lora_expand_rows(const LoraParams& p, int64_t t0, int id, int n, const int* list,
-                                                 const uint16_t* vt, int c_begin, int c_end) {
+                                                 const uint16_t* vt, float* tiles, int c_begin, int c_end) {
+  using T = std::conditional_t<F32, float, uint16_t>;
+  constexpr int kPer = 16 / sizeof(T), kLanes = 64 / kPer;      // values per piece, pieces per row
+  constexpr int kRows = 64 / kLanes, kPieces = 16 / kRows;      // rows per access, accesses per tile
   const int lane = lane_id(), wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-  const int pitch = lora_pitch(p.rank);
+  const int pitch = lora_pitch(p.rank), yr = lane / kLanes, yc = (lane % kLanes) * kPer;
   const uint16_t* bm = p.b + static_cast<int64_t>(id) * p.n * p.rank;
+  float* tile = tiles + wave * 16 * kLoraTilePitch;
+  // every lane loads (past the last row or column a valid place again): a load under a
+  // branch is waited for before the next one
+  auto row_of = [&](int i0, int i, int u) __attribute__((always_inline)) {
+    return t0 + list[min(i0 + 16 * i + kRows * u + yr, n - 1)];
+  };
+  auto load_y = [&](int col0, int i0, uint4 (&y)[2][kPieces]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u)
+        y[i][u] = lora_load<NT>(static_cast<const T*>(p.y) + row_of(i0, i, u) * p.y_stride + min(col0 + yc, c_end - kPer));
+  };
+  uint4 y[2][kPieces], y_next[2][kPieces];
+  load_y(c_begin + 64 * wave, 0, y);
   for (int col0 = c_begin + 64 * wave; col0 < c_end; col0 += 64 * kLoraWaves) {
-    const int n_lane = col0 + 16 * g;
-    const bool live[2] = {n_lane < c_end, n_lane + 8 < c_end};  // c_end % 8 == 0
+    const bool live = col0 + yc < c_end;  // c_end is a multiple of 8
     const uint16_t* br[4];
 #pragma unroll
-    for (int jt = 0; jt < 4; ++jt)
-      br[jt] = bm + static_cast<int64_t>(min(col0 + 16 * (m >> 2) + 4 * jt + (m & 3), c_end - 1)) * p.rank;
+    for (int jt = 0; jt < 4; ++jt) br[jt] = bm + static_cast<int64_t>(min(col0 + 16 * jt + m, c_end - 1)) * p.rank;
     bf16x8 b[2][4];
     auto load_b = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = k0 + 32 * h + 8 * g;
+        const int k = min(k0 + 32 * h + 8 * g, p.rank - 8);  // past the rank v is 0
 #pragma unroll
-        for (int jt = 0; jt < 4; ++jt) b[h][jt] = k < p.rank ? *reinterpret_cast<const bf16x8*>(br[jt] + k) : zero_bf16x8();
+        for (int jt = 0; jt < 4; ++jt) b[h][jt] = *reinterpret_cast<const bf16x8*>(br[jt] + k);
       }
     };
     if constexpr (ONE) load_b(0);
     for (int i0 = 0; i0 < n; i0 += 32) {
-      int64_t row[2];
-      uint4 y[2][F32 ? 4 : 2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        row[i] = t0 + list[min(i0 + 16 * i + m, n - 1)];
-        if (i0 + 16 * i + m < n) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!live[h]) continue;
-            if constexpr (F32) {
-              const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.y) + row[i] * p.y_stride + n_lane + 8 * h);
-              y[i][2 * h] = src[0];
-              y[i][2 * h + 1] = src[1];
-            } else {
-              y[i][h] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.y) + row[i] * p.y_stride + n_lane + 8 * h);
-            }
-          }
-        }
-      }
+      // the next pair's y ahead of this one's stores, which a later load would wait for
+      const bool more = i0 + 32 < n;
+      load_y(more ? col0 : col0 + 64 * kLoraWaves, more ? i0 + 32 : 0, y_next);
       f32x4 acc[2][4] = {};
       for (int k0 = 0; k0 < (ONE ? 1 : p.rank); k0 += 64) {
         if constexpr (!ONE) load_b(k0);
@@ -483,36 +566,67 @@ __device__ __forceinline__ void lora_expand_rows(const LoraParams& p, int64_t t0
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (i0 + 16 * i + m < n) {
+        // the wave's own LDS accesses are done in order
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!live[h]) continue;
-            if constexpr (F32) {
-              f32x4* dst = reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + row[i] * p.out_stride + n_lane + 8 * h);
-              dst[0] = __builtin_bit_cast(f32x4, y[i][2 * h]) + acc[i][2 * h];
-              dst[1] = __builtin_bit_cast(f32x4, y[i][2 * h + 1]) + acc[i][2 * h + 1];
-            } else {
-              const uint32_t w[4] = {y[i][h].x, y[i][h].y, y[i][h].z, y[i][h].w};
-              uint32_t o[4];
+        for (int jt = 0; jt < 4; ++jt) *reinterpret_cast<f32x4*>(tile + m * kLoraTilePitch + 16 * jt + 4 * g) = acc[i][jt];
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                o[e] = pack_bf16x2(__uint_as_float(w[e] << 16) + acc[i][2 * h + e / 2][2 * (e & 1)],
-                                   __uint_as_float(w[e] & 0xffff0000u) + acc[i][2 * h + e / 2][2 * (e & 1) + 1]);
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row[i] * p.out_stride + n_lane + 8 * h) =
-                  uint4{o[0], o[1], o[2], o[3]};
-            }
+        for (int u = 0; u < kPieces; ++u) {
+          const f32x4* src = reinterpret_cast<const f32x4*>(tile + (kRows * u + yr) * kLoraTilePitch + yc);
+          uint4 o;
+          if constexpr (F32) {
+            o = __builtin_bit_cast(uint4, __builtin_bit_cast(f32x4, y[i][u]) + src[0]);
+          } else {
+            const f32x4 lo = src[0], hi = src[1];
+            auto add = [](uint32_t w, float c0, float c1) {
+              return pack_bf16x2(__uint_as_float(w << 16) + c0, __uint_as_float(w & 0xffff0000u) + c1);
+            };
+            o = uint4{add(y[i][u].x, lo[0], lo[1]), add(y[i][u].y, lo[2], lo[3]), add(y[i][u].z, hi[0], hi[1]),
+                      add(y[i][u].w, hi[2], hi[3])};
           }
+          if (live && i0 + 16 * i + kRows * u + yr < n)
+            lora_store<NT>(static_cast<T*>(p.out) + row_of(i0, i, u) * p.out_stride + col0 + yc, o);
         }
+        __builtin_amdgcn_wave_barrier();
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) y[i][u] = y_next[i][u];
+    }
+  }
+}
+
+// out = y for the listed rows, eight 16-byte loads in flight per thread.
+template <bool F32, bool NT>
+__device__ __forceinline__ void lora_copy_rows(const LoraParams& p, int64_t t0, int n, const int* list, int c_begin, int c_end) {
+  using T = std::conditional_t<F32, float, uint16_t>;
+  constexpr int kPer = 16 / sizeof(T), kFlight = 8, kThreads = kLoraWaves * 64;
+  const int chunks = (c_end - c_begin) / kPer, total = n * chunks;
+  for (int e0 = threadIdx.x; e0 < total; e0 += kFlight * kThreads) {
+    uint4 v[kFlight];
+    auto at = [&](int e, int64_t stride) __attribute__((always_inline)) {
+      const int i = e / chunks;
+      return (t0 + list[i]) * stride + c_begin + (e - i * chunks) * kPer;
+    };
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      v[u] = lora_load<NT>(static_cast<const T*>(p.y) + at(min(e0 + u * kThreads, total - 1), p.y_stride));
+    }
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const int e = e0 + u * kThreads;
+      if (e < total) lora_store<NT>(static_cast<T*>(p.out) + at(e, p.out_stride), v[u]);
     }
   }
 }
 
 // grid: (row blocks, parts of a block's adapters, column parts).  The rows without an
 // adapter are a group of their own, copied unless out is y.
-template <bool F32, int TERMS>
-__global__ __launch_bounds__(kLoraWaves * 64, 3) void lora_expand_kernel(LoraParams p) {
-  extern __shared__ __align__(16) uint16_t vt[];  // [TERMS][kRowsBlock][pitch]
+template <bool F32, int TERMS, bool NT>
+__global__ __launch_bounds__(kLoraWaves * 64, F32 ? 2 : 3) void lora_expand_kernel(LoraParams p) {
+  extern __shared__ __align__(16) float tiles[];  // [waves][16][pitch], then v's terms
+  uint16_t* vt = reinterpret_cast<uint16_t*>(tiles + kLoraWaves * 16 * kLoraTilePitch);  // [TERMS][kRowsBlock][pitch]
   __shared__ int list[kRowsBlock];
   const int64_t blk = lora_block(p), t0 = blk * kRowsBlock;
   if (blk < 0) return;
@@ -520,16 +634,7 @@ __global__ __launch_bounds__(kLoraWaves * 64, 3) void lora_expand_kernel(LoraPar
   const int c_begin = blockIdx.z * p.cols_per_wg, c_end = min(c_begin + p.cols_per_wg, p.n);
   lora_groups(id, __ballot(p.y != p.out ? id >= -1 : id >= 0), blockIdx.y, gridDim.y, list, [&](int gid, int n) {
     if (gid < 0) {
-      constexpr int kPer = F32 ? 4 : 8;  // values of 16 bytes
-      const int chunks = (c_end - c_begin) / kPer;
-      for (int i = 0; i < n; ++i) {
-        const int64_t t = t0 + list[i];
-        for (int c = threadIdx.x; c < chunks; c += kLoraWaves * 64) {
-          const int64_t at = c_begin + c * kPer;
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.y) + (t * p.y_stride + at) * (16 / kPer));
-          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + (t * p.out_stride + at) * (16 / kPer)) = *src;
-        }
-      }
+      lora_copy_rows<F32, NT>(p, t0, n, list, c_begin, c_end);
       return;
     }
     // v of the rows, the splits summed in order and scaled, as bf16 terms; 0 past the rank
@@ -538,18 +643,20 @@ __global__ __launch_bounds__(kLoraWaves * 64, 3) void lora_expand_kernel(LoraPar
     for (int e = threadIdx.x; e < n * quads; e += kLoraWaves * 64) {
       const int i = e / quads, r = 4 * (e - i * quads);
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (r < p.rank) {
-        const float* src = p.v + (t0 + list[i]) * p.rank + r;
-        for (int s = 0; s < p.splits; s += 8) {  // the loads of eight splits at once
-          f32x4 part[8];
+      const float* src = p.v + (t0 + list[i]) * p.rank + min(r, p.rank - 4);
+      auto add = [&](int s, auto many) __attribute__((always_inline)) {  // their loads in flight together
+        constexpr int kMany = decltype(many)::value;
+        f32x4 part[kMany];
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            part[u] = s + u < p.splits ? *reinterpret_cast<const f32x4*>(src + (s + u) * p.rows * p.rank) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < kMany; ++u) part[u] = *reinterpret_cast<const f32x4*>(src + min(s + u, p.splits - 1) * p.rows * p.rank);
 #pragma unroll
-          for (int u = 0; u < 8; ++u) v += part[u];
-        }
-        v *= c;
-      }
+        for (int u = 0; u < kMany; ++u)
+          if (s + u < p.splits) v += part[u];
+      };
+      if (p.splits <= 4) add(0, std::integral_constant<int, 4>{});
+      else for (int s = 0; s < p.splits; s += 8) add(s, std::integral_constant<int, 8>{});
+      v *= c;
+      if (r >= p.rank) v = f32x4{0.f, 0.f, 0.f, 0.f};
       uint16_t t16[4][TERMS];
 #pragma unroll
       for (int u = 0; u < 4; ++u) split_bf16<TERMS>(v[u], t16[u]);
@@ -560,9 +667,9 @@ __global__ __launch_bounds__(kLoraWaves * 64, 3) void lora_expand_kernel(LoraPar
     }
     __syncthreads();
     if (p.rank <= 64)
-      lora_expand_rows<F32, TERMS, true>(p, t0, gid, n, list, vt, c_begin, c_end);
+      lora_expand_rows<F32, TERMS, NT, true>(p, t0, gid, n, list, vt, tiles, c_begin, c_end);
     else
-      lora_expand_rows<F32, TERMS, false>(p, t0, gid, n, list, vt, c_begin, c_end);
+      lora_expand_rows<F32, TERMS, NT, false>(p, t0, gid, n, list, vt, tiles, c_begin, c_end);
   });
 }
 

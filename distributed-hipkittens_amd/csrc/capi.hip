@@ -678,12 +678,14 @@ int launch_router(const RouterParams& p, hipStream_t s) {
   return launch_router_panel<Panel<64, 128, 2, 4, 4>>(p, s);
 }
 
-template <bool F32, int TERMS>
+constexpr int64_t kLoraCached = 16 << 20;  // bytes of y up to which its accesses go through the L2s
+
+template <bool F32, int TERMS, bool NT>
 int launch_lora_expand(const LoraParams& p, dim3 grid, hipStream_t s) {
   static bool attr_set[kMaxDevices] = {false};
   int dev = 0;
   (void)hipGetDevice(&dev);
-  auto kern = lora_expand_kernel<F32, TERMS>;
+  auto kern = lora_expand_kernel<F32, TERMS, NT>;
   if (dev >= 0 && dev < kMaxDevices && !attr_set[dev]) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                lora_lds_bytes(kLoraMaxRank, TERMS));
@@ -698,8 +700,8 @@ int launch_lora_expand(const LoraParams& p, dim3 grid, hipStream_t s) {
 // fill the chip, at least one step per wave.
 int lora_splits(int64_t rows, int64_t hidden) {
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock, steps = (hidden + kRowsStep - 1) / kRowsStep;
-  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, steps / kLoraWaves));
-  return static_cast<int>(std::min(most, std::max<int64_t>(1, 512 / std::max<int64_t>(1, blocks))));
+  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, steps / (2 * kLoraWaves)));
+  return static_cast<int>(std::min(most, std::max<int64_t>(1, 400 / std::max<int64_t>(1, blocks))));
 }
 
 }  // namespace
@@ -1607,9 +1609,9 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
              rank, kLoraMaxRank);
   HK_REQUIRE(y_dtype == HKMOE_BF16 || y_dtype == HKMOE_F32, "lora_add: bad y_dtype %d", y_dtype);
   HK_REQUIRE(a && b && (rows == 0 || (y && x && ids && out)), "lora_add: null pointer");
-  HK_REQUIRE(x_stride >= hidden && x_stride % 8 == 0 && y_stride >= n && out_stride >= n &&
+  HK_REQUIRE(x_stride >= hidden && x_stride % 8 == 0 && x_stride <= (1 << 25) && y_stride >= n && out_stride >= n &&
                  (y_stride * (y_dtype == HKMOE_F32 ? 4 : 2)) % 16 == 0 && (out_stride * (y_dtype == HKMOE_F32 ? 4 : 2)) % 16 == 0,
-             "lora_add: rows must be 16-byte aligned and not overlap (strides x %lld, y %lld, out %lld)",
+             "lora_add: rows must be 16-byte aligned and not overlap, x's at most 2^25 apart (strides x %lld, y %lld, out %lld)",
              (long long)x_stride, (long long)y_stride, (long long)out_stride);
   HK_REQUIRE(aligned16(y) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(out) &&
                  (reinterpret_cast<uintptr_t>(ids) & 3) == 0 && (reinterpret_cast<uintptr_t>(scaling) & 3) == 0,
@@ -1648,7 +1650,9 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
   const int64_t strips = (n + 255) / 256, cols = std::min<int64_t>({strips, 65535, std::max<int64_t>(1, 512 / blocks)});
   p.cols_per_wg = static_cast<int32_t>((strips + cols - 1) / cols * 256);
   const dim3 grid(grid_x, parts(cols), static_cast<unsigned>((n + p.cols_per_wg - 1) / p.cols_per_wg));
-  return y_dtype == HKMOE_F32 ? launch_lora_expand<true, 3>(p, grid, s) : launch_lora_expand<false, 2>(p, grid, s);
+  const bool nt = rows * n * (y_dtype == HKMOE_F32 ? 4 : 2) > kLoraCached;
+  if (y_dtype == HKMOE_F32) return nt ? launch_lora_expand<true, 3, true>(p, grid, s) : launch_lora_expand<true, 3, false>(p, grid, s);
+  return nt ? launch_lora_expand<false, 2, true>(p, grid, s) : launch_lora_expand<false, 2, false>(p, grid, s);
 }
 
 // ---------------------------------------------------------------------------

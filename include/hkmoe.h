@@ -432,7 +432,8 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
  *   the low-rank adapters of a batch's requests beside a projection that computed y.
  *   Rows whose id is outside [0, adapters) have none: out[t] = y[t].
  *   y [T, N] and out [T, N] bf16 or fp32 (y_dtype), x [T, H] bf16, their rows y_stride,
- *   out_stride and x_stride elements apart (16-byte multiples; slices of wider buffers);
+ *   out_stride and x_stride elements apart (16-byte multiples; slices of wider buffers;
+ *   x_stride <= 2^25);
  *   a [adapters, rank, H], b [adapters, N, rank] bf16 contiguous, ids [T] int32,
  *   scaling [adapters] fp32 or NULL (1).  out may be y itself (with its stride; rows
  *   without an adapter are then not touched) and overlaps nothing else.
