@@ -11,6 +11,7 @@
 // the result holds rows 4 (l / 16) + 0..3, column l % 16.
 #pragma once
 
+#include "gemm_skinny.hpp"
 #include "gemm_small.hpp"
 
 namespace hkmoe {
@@ -264,24 +265,114 @@ struct RouterParams {
   int32_t experts, hidden;
 };
 
-// One workgroup per tile of [16 MT, 16 NT] logits, K split over its waves.
-template <int MT, int NT, int WAVES, int DEPTH>
-__global__ __launch_bounds__(WAVES * 64) void router_kernel(RouterParams p) {
-  __shared__ float red[WAVES * MT * NT * 256];
-  const int64_t row0 = blockIdx.x * static_cast<int64_t>(16 * MT);
-  const int col0 = blockIdx.y * 16 * NT;
-  const int lane = lane_id(), wave = threadIdx.x >> 6;
-  const uint16_t* xr[MT];
-  const uint16_t* wr[NT];
+// Few rows or few tiles: one workgroup per tile of [16 MT, 16 NT] logits, K split over its NW
+// waves, each streaming its steps through an LDS ring of its own, DEPTH steps deep (whole
+// 128-byte lines, no barrier in the loop); the partial tiles are summed in wave order.
+template <int MT_, int NT_, int NW_, int DEPTH_>
+struct Strip {
+  static constexpr int MT = MT_, NT = NT_, NW = NW_, DEPTH = DEPTH_;
+  static constexpr int kStep = (MT + NT) * 2048, kRing = NW * DEPTH * kStep, kLd = 16 * NT + 4;
+  static constexpr int kPart = NW * 16 * MT * kLd * 4, kLds = kRing > kPart ? kRing : kPart;
+  static constexpr int kLoads = 2 * (MT + NT);  // DMA instructions per step
+  static_assert((MT == 1 || MT == 2) && (NT == 1 || NT == 2 || NT == 4), "tile");
+  static_assert(DEPTH >= 2 && kLoads * (DEPTH - 1) <= 63 && kLds <= kSkMaxLds, "ring depth, vmcnt range");
+};
+
+template <typename S>
+__global__ __launch_bounds__(S::NW * 64) void router_strip_kernel(RouterParams p) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int64_t row0 = blockIdx.x * static_cast<int64_t>(16 * S::MT);
+  const int col0 = blockIdx.y * 16 * S::NT;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l16 = lane & 15, lg = lane >> 4, ld_row = lane >> 3;
+  const int K = p.hidden, steps = (K + kRowsStep - 1) / kRowsStep;
+  const int mine = (steps - wave + S::NW - 1) / S::NW;  // this wave's steps (0: none)
+  const i32x4 x_srd = make_srd(p.x + row0 * K, 0xffffffffu), w_srd = make_srd(p.w, 0xffffffffu);
+  const int last = static_cast<int>(min(static_cast<int64_t>(16 * S::MT), p.rows - row0)) - 1;
+  // instruction u fills ring rows 8u .. 8u + 7, of x and then of w; the lane fetches the
+  // chunk that lands swizzled.  Rows past the last repeat it (never stored).
+  uint32_t off[S::kLoads];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xr[i] = p.x + min(row0 + 16 * i + (lane & 15), p.rows - 1) * p.hidden;
+  for (int u = 0; u < S::kLoads; ++u) {
+    const int r = 8 * u + ld_row;
+    off[u] = static_cast<uint32_t>(u < 2 * S::MT ? min(r, last) : min(col0 + r - 16 * S::MT, p.experts - 1)) * (2 * static_cast<uint32_t>(K)) +
+             16 * ((lane & 7) ^ swz(r));
+  }
+  uint8_t* ring = smem + wave * S::DEPTH * S::kStep;
+  // Steps past the last one go through empty descriptors (no memory traffic), so the loads
+  // in flight stay a constant count.  K's last step, K % 64 != 0, takes its first chunk in
+  // the place of those past the row; their products are cut below.
+  auto issue = [&](int i, int slot) __attribute__((always_inline)) {
+    const bool in = i < mine;
+    const int k0 = in ? (wave + S::NW * i) * kRowsStep : 0;
+    i32x4 xs = x_srd, ws = w_srd;
+    xs.z = in ? xs.z : 0;
+    ws.z = in ? ws.z : 0;
 #pragma unroll
-  for (int j = 0; j < NT; ++j) wr[j] = p.w + static_cast<int64_t>(min(col0 + 16 * j + (lane & 15), p.experts - 1)) * p.hidden;
-  f32x4 acc[MT][NT] = {};
-  rows_product<MT, NT, DEPTH>(xr, wr, p.hidden, wave, WAVES, (p.hidden + kRowsStep - 1) / kRowsStep, acc);
-  rows_reduce<MT, NT, WAVES>(acc, red, [&](int r, int c, float v) {
+    for (int u = 0; u < S::kLoads; ++u) {
+      uint32_t at = off[u];
+      if (k0 + kRowsStep > K) {
+        const int chunk = (lane & 7) ^ swz(8 * u + ld_row);
+        if (k0 + 8 * chunk >= K) at -= 16 * chunk;
+      }
+      load_lds_16B(u < 2 * S::MT ? xs : ws, ring + slot * S::kStep + u * 1024, static_cast<int>(at), 2 * k0);
+    }
+  };
+  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring)) + l16 * 128;
+  const uint32_t lo_off = (lg ^ swz(l16)) << 4, hi_off = ((lg + 4) ^ swz(l16)) << 4;
+  f32x4 acc[S::MT][S::NT] = {};
+#pragma unroll
+  for (int u = 0; u < S::DEPTH; ++u) issue(u, u);
+  int slot = 0;
+  for (int i = 0; i < mine; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads * (S::DEPTH - 1)) : "memory");
+    const uint32_t lo = base + slot * S::kStep + lo_off, hi = base + slot * S::kStep + hi_off;
+    i32x8 a[S::MT], b[S::NT];
+    if constexpr (S::MT == 1) sk_frag<0>(lo, hi, a[0]);
+    else sk_frag2<0>(lo, hi, a[0], a[1]);
+    if constexpr (S::NT == 1) {
+      sk_frag<S::MT * 2048>(lo, hi, b[0]);
+    } else {
+      sk_frag2<S::MT * 2048>(lo, hi, b[0], b[1]);
+      if constexpr (S::NT == 4) sk_frag2<(S::MT + 2) * 2048>(lo, hi, b[2], b[3]);
+    }
+    issue(i + S::DEPTH, slot);  // this wave has read the slot
+    __builtin_amdgcn_sched_barrier(0);
+    const int k0 = (wave + S::NW * i) * kRowsStep;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool cut = k0 + 32 * h + 8 * lg >= K;
+      bf16x8 ah[S::MT], bh[S::NT];
+#pragma unroll
+      for (int j = 0; j < S::MT; ++j) ah[j] = cut ? zero_bf16x8() : __builtin_bit_cast(bf16x8, h ? a[j].hi : a[j].lo);
+#pragma unroll
+      for (int j = 0; j < S::NT; ++j) bh[j] = cut ? zero_bf16x8() : __builtin_bit_cast(bf16x8, h ? b[j].hi : b[j].lo);
+#pragma unroll
+      for (int j = 0; j < S::MT; ++j)
+#pragma unroll
+        for (int l = 0; l < S::NT; ++l) acc[j][l] = mfma_bf16_16x16x32(ah[j], bh[l], acc[j][l]);
+    }
+    slot = slot == S::DEPTH - 1 ? 0 : slot + 1;
+  }
+  // every wave's DMA has landed before the partial tiles overwrite the rings
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int j = 0; j < S::MT; ++j)
+#pragma unroll
+    for (int l = 0; l < S::NT; ++l)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) part[(wave * 16 * S::MT + 16 * j + 4 * lg + r) * S::kLd + 16 * l + l16] = acc[j][l][r];
+  __syncthreads();
+  for (int e = threadIdx.x; e < 256 * S::MT * S::NT; e += S::NW * 64) {
+    const int r = e / (16 * S::NT), c = e % (16 * S::NT);
+    float v = part[r * S::kLd + c];
+#pragma unroll
+    for (int w = 1; w < S::NW; ++w) v += part[(w * 16 * S::MT + r) * S::kLd + c];
     if (row0 + r < p.rows && col0 + c < p.experts) p.logits[(row0 + r) * p.experts + col0 + c] = v;
-  });
+  }
 }
 
 // Many rows: one workgroup per panel tile.  The column tiles of a row tile run side by

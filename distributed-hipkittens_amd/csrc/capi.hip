@@ -608,7 +608,7 @@ int launch_expert_offsets(const int32_t* block_counts, int64_t num_tokens, int32
 // ---------------------------------------------------------------------------
 // residual + norm + quantisation, router, adapters
 // ---------------------------------------------------------------------------
-constexpr int64_t kMaxRows = 1 << 26;  // a launch's work-items stay below 2^32 in each dimension
+constexpr int64_t kMaxRows = 1 << 24;  // a launch's work-items stay below 2^32 in each dimension
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -647,34 +647,60 @@ int launch_norm(const NormParams& p, int mode, hipStream_t s) {
   return check_launch("norm_quant_tensor_kernel");
 }
 
-template <typename P>
-int launch_router_panel(const RouterParams& p, hipStream_t s) {
-  static bool attr_set[kMaxDevices] = {false};
+template <typename K>
+int raise_lds(K kern, int bytes, bool (&done)[kMaxDevices]) {
   int dev = 0;
   (void)hipGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices || done[dev]) return HKMOE_OK;
+  const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != hipSuccess) return fail(HKMOE_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(err));
+  done[dev] = true;
+  return HKMOE_OK;
+}
+
+template <typename P>
+int launch_router_panel(const RouterParams& p, hipStream_t s) {
+  static bool done[kMaxDevices] = {false};
   auto kern = router_panel_kernel<P>;
-  if (dev >= 0 && dev < kMaxDevices && !attr_set[dev]) {
-    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, P::kLds);
-    if (err != hipSuccess) return fail(HKMOE_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(err));
-    attr_set[dev] = true;
-  }
+  HK_TRY(raise_lds(kern, P::kLds, done));
   const int64_t rt = (p.rows + P::BM - 1) / P::BM, ct = (p.experts + P::BN - 1) / P::BN;
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>((rt + 7) / 8 * 8 * ct)), dim3(P::kWaves * 64), P::kLds, s, p,
                      static_cast<int>(rt), static_cast<int>(ct));
   return check_launch("router_panel_kernel");
 }
 
-template <int MT, int NT, int WAVES, int DEPTH>
-int launch_router(const RouterParams& p, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>((p.rows + 16 * MT - 1) / (16 * MT)), static_cast<unsigned>((p.experts + 16 * NT - 1) / (16 * NT)));
-  hipLaunchKernelGGL((router_kernel<MT, NT, WAVES, DEPTH>), grid, dim3(WAVES * 64), 0, s, p);
-  return check_launch("router_kernel");
+template <typename S>
+int launch_router_strip(const RouterParams& p, hipStream_t s) {
+  static bool done[kMaxDevices] = {false};
+  auto kern = router_strip_kernel<S>;
+  HK_TRY(raise_lds(kern, S::kLds, done));
+  const dim3 grid(static_cast<unsigned>((p.rows + 16 * S::MT - 1) / (16 * S::MT)),
+                  static_cast<unsigned>((p.experts + 16 * S::NT - 1) / (16 * S::NT)));
+  hipLaunchKernelGGL(kern, grid, dim3(S::NW * 64), S::kLds, s, p);
+  return check_launch("router_strip_kernel");
 }
 
+// The router's kernel: the cheapest by estimated time (us), rounds of 256 workgroups x (start
+// + K steps x time per step), fitted to launches in a row on 21 shapes (T 1 .. 16384, E 8 ..
+// 512, H 1024 .. 7168), on each of which it picks the fastest:
+//   64x128x4096    strips 16x16 7.4, 32x32 9.9, panels 64x64 16.0, 64x128 22.0
+//   1024x256x7168  38.4, 15.3, 26.4, 36.5
+//   4096x256x7168  157, 56.6, 27.4, 37.2
+//   8192x256x7168  301, 146, 43.3, 39.0
 int launch_router(const RouterParams& p, hipStream_t s) {
-  const int64_t tiles = (p.rows + 15) / 16 * ((p.experts + 15) / 16);
-  if (tiles <= 512) return launch_router<1, 1, 16, 4>(p, s);
-  if (tiles <= 2048) return launch_router<1, 4, 8, 2>(p, s);
+  const double steps = static_cast<double>((p.hidden + kRowsStep - 1) / kRowsStep);
+  auto rounds = [&](int64_t rows, int64_t cols) {
+    const int64_t tiles = (p.rows + rows - 1) / rows * ((p.experts + cols - 1) / cols);
+    return static_cast<double>((tiles + 255) / 256);
+  };
+  const double t11 = 1.3 + rounds(16, 16) * (2.2 + 0.0625 * steps), t12 = 1.3 + rounds(16, 32) * (2.8 + 0.075 * steps),
+               t22 = 1.3 + rounds(32, 32) * (2.6 + 0.0975 * steps),
+               t64 = 2.0 + steps * (0.075 + 0.15 * rounds(64, 64)), t128 = 2.0 + steps * 0.335 * rounds(64, 128);
+  const double best = std::min({t11, t12, t22, t64, t128});
+  if (best == t11) return launch_router_strip<Strip<1, 1, 8, 4>>(p, s);
+  if (best == t12) return launch_router_strip<Strip<1, 2, 8, 3>>(p, s);
+  if (best == t22) return launch_router_strip<Strip<2, 2, 8, 2>>(p, s);
+  if (best == t64) return launch_router_panel<Panel<64, 64, 2, 2, 4>>(p, s);
   return launch_router_panel<Panel<64, 128, 2, 4, 4>>(p, s);
 }
 
@@ -682,16 +708,9 @@ constexpr int64_t kLoraCached = 16 << 20;  // bytes of y up to which its accesse
 
 template <bool F32, int TERMS, bool NT>
 int launch_lora_expand(const LoraParams& p, dim3 grid, hipStream_t s) {
-  static bool attr_set[kMaxDevices] = {false};
-  int dev = 0;
-  (void)hipGetDevice(&dev);
+  static bool done[kMaxDevices] = {false};
   auto kern = lora_expand_kernel<F32, TERMS, NT>;
-  if (dev >= 0 && dev < kMaxDevices && !attr_set[dev]) {
-    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               lora_lds_bytes(kLoraMaxRank, TERMS));
-    if (err != hipSuccess) return fail(HKMOE_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(err));
-    attr_set[dev] = true;
-  }
+  HK_TRY(raise_lds(kern, lora_lds_bytes(kLoraMaxRank, TERMS), done));
   hipLaunchKernelGGL(kern, grid, dim3(kLoraWaves * 64), lora_lds_bytes(p.rank, TERMS), s, p);
   return check_launch("lora_expand_kernel");
 }

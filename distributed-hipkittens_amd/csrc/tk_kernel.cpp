@@ -757,36 +757,57 @@ void dispatch_moe_mx(py::object x_q, py::object x_e8m0, py::object logits, py::o
 // Residual + norm + quantisation, router, adapters.  Unlike the calls above these
 // check that every tensor lives on torch's current device, whose stream they use.
 // ---------------------------------------------------------------------------
-int64_t device_of(const py::object& obj) {
-  return steal(PyObject_CallMethodNoArgs(obj.ptr(), names().get_device_attr)).cast<int64_t>();
+// torch's current device and its current stream.
+struct Current {
+  int64_t device;
+  hkmoe_stream_t stream;
+};
+Current current() {
+  const Names& nm = names();
+  if (nm.raw_stream == nullptr)
+    return Current{nm.torch_cuda.attr("current_device")().cast<int64_t>(), current_stream()};
+  const py::object dev = steal(PyObject_CallNoArgs(nm.get_device));
+  return Current{PyLong_AsLongLong(dev.ptr()),
+                 reinterpret_cast<hkmoe_stream_t>(PyLong_AsSize_t(steal(PyObject_CallOneArg(nm.raw_stream, dev.ptr())).ptr()))};
 }
 
-void want_current_device(std::initializer_list<std::pair<const py::object*, const char*>> ts) {
+// A torch.Tensor of the current device; `stride` (2-D tensors only): its rows need only be
+// contiguous by themselves, and this is the distance between them in elements.
+TensorArg as_current(const py::object& obj, const char* name, const Current& cur, int64_t* stride = nullptr) {
   const Names& nm = names();
-  const int64_t cur = nm.get_device != nullptr ? steal(PyObject_CallNoArgs(nm.get_device)).cast<int64_t>()
-                                               : nm.torch_cuda.attr("current_device")().cast<int64_t>();
-  for (const auto& [obj, name] : ts)
-    if (!obj->is_none() && device_of(*obj) != cur)
-      throw std::runtime_error(std::string(name) + ": tensor must be on the current device");
-}
-
-// A 2-D tensor whose rows are contiguous: its row stride in elements.
-TensorArg as_rows(const py::object& obj, const char* name, int64_t* stride) {
-  const Names& nm = names();
-  if (!PyObject_IsInstance(obj.ptr(), nm.tensor_type)) throw std::runtime_error(std::string(name) + ": expected a torch.Tensor");
-  const py::tuple strides = steal(PyObject_CallMethodNoArgs(obj.ptr(), nm.stride)).cast<py::tuple>();
-  const py::tuple shape = steal(PyObject_GetAttr(obj.ptr(), nm.shape)).cast<py::tuple>();
-  if (shape.size() != 2) throw std::runtime_error(std::string(name) + ": expected 2-D tensor");
-  if (steal(PyObject_GetAttr(obj.ptr(), nm.is_cpu)).ptr() == Py_True)
-    throw std::runtime_error(std::string(name) + ": tensor must be on a GPU device");
+  PyObject* o = obj.ptr();
+  if (reinterpret_cast<PyObject*>(Py_TYPE(o)) != nm.tensor_type && PyObject_IsInstance(o, nm.tensor_type) != 1) {
+    PyErr_Clear();
+    throw std::runtime_error(std::string(name) + ": expected a torch.Tensor");
+  }
   TensorArg t;
-  for (auto s : shape) t.shape.push_back(s.cast<int64_t>());
-  if (t.shape[1] > 1 && strides[1].cast<int64_t>() != 1)
-    throw std::runtime_error(std::string(name) + ": rows must be contiguous");
-  *stride = t.shape[0] > 1 ? strides[0].cast<int64_t>() : t.shape[1];
-  t.ptr = reinterpret_cast<void*>(steal(PyObject_CallMethodNoArgs(obj.ptr(), nm.data_ptr)).cast<uintptr_t>());
-  t.dtype.name = dtype_name(steal(PyObject_GetAttr(obj.ptr(), nm.dtype)).ptr());
+  const py::object shape = steal(PyObject_GetAttr(o, nm.shape));
+  for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(shape.ptr()); ++k)
+    t.shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(shape.ptr(), k)));
+  const bool flat = steal(PyObject_CallMethodNoArgs(o, nm.is_contiguous)).ptr() == Py_True;
+  if (stride != nullptr) {
+    if (t.shape.size() != 2) throw std::runtime_error(std::string(name) + ": expected 2-D tensor");
+    *stride = t.shape[1];
+    if (!flat) {
+      const py::tuple st = steal(PyObject_CallMethodNoArgs(o, nm.stride)).cast<py::tuple>();
+      if (t.shape[1] > 1 && st[1].cast<int64_t>() != 1)
+        throw std::runtime_error(std::string(name) + ": rows must be contiguous");
+      if (t.shape[0] > 1) *stride = st[0].cast<int64_t>();
+    }
+  } else if (!flat) {
+    throw std::runtime_error(std::string(name) + ": tensor must be contiguous");
+  }
+  const int64_t dev = PyLong_AsLongLong(steal(PyObject_CallMethodNoArgs(o, nm.get_device_attr)).ptr());
+  if (dev < 0) throw std::runtime_error(std::string(name) + ": tensor must be on a GPU device");
+  if (dev != cur.device) throw std::runtime_error(std::string(name) + ": tensor must be on the current device");
+  t.ptr = PyLong_AsVoidPtr(steal(PyObject_CallMethodNoArgs(o, nm.data_ptr)).ptr());
+  t.dtype.name = dtype_name(steal(PyObject_GetAttr(o, nm.dtype)).ptr());
+  if (PyErr_Occurred()) throw py::error_already_set();
   return t;
+}
+
+TensorArg as_current_opt(const py::object& obj, const char* name, const Current& cur) {
+  return obj.is_none() ? TensorArg{} : as_current(obj, name, cur);
 }
 
 int float_type(const TensorArg& t, const char* name) {
@@ -803,12 +824,11 @@ size_t byte_size(const TensorArg& t, const char* name) {
 void dispatch_rms_norm_quant(py::object x_, py::object residual_, py::object weight_, double eps, int scale_mode,
                              py::object q_, py::object s_, py::object scale_, py::object residual_out_,
                              py::object norm_out_, py::object workspace_) {
-  auto x = as_tensor(x_, "x"), w = as_tensor(weight_, "weight"), q = as_tensor(q_, "q"), s = as_tensor_opt(s_, "s"),
-       r = as_tensor_opt(residual_, "residual"), sc = as_tensor_opt(scale_, "scale"),
-       ro = as_tensor_opt(residual_out_, "residual_out"), no = as_tensor_opt(norm_out_, "norm_out"),
-       ws = as_tensor_opt(workspace_, "workspace");
-  want_current_device({{&x_, "x"}, {&weight_, "weight"}, {&q_, "q"}, {&s_, "s"}, {&residual_, "residual"}, {&scale_, "scale"},
-                       {&residual_out_, "residual_out"}, {&norm_out_, "norm_out"}, {&workspace_, "workspace"}});
+  const Current cur = current();
+  auto x = as_current(x_, "x", cur), w = as_current(weight_, "weight", cur), q = as_current(q_, "q", cur),
+       s = as_current_opt(s_, "s", cur), r = as_current_opt(residual_, "residual", cur), sc = as_current_opt(scale_, "scale", cur),
+       ro = as_current_opt(residual_out_, "residual_out", cur), no = as_current_opt(norm_out_, "norm_out", cur),
+       ws = as_current_opt(workspace_, "workspace", cur);
   want_dim(x, "x", 2);
   const int xt = float_type(x, "x"), wt = float_type(w, "weight");
   const int64_t rows = x.shape[0], cols = x.shape[1];
@@ -838,15 +858,14 @@ void dispatch_rms_norm_quant(py::object x_, py::object residual_, py::object wei
       throw std::runtime_error("s must be [R, C/128], or one value with HKMOE_SCALE_TENSOR");
   }
   check(hkmoe_rms_norm_quant(x.ptr, r.ptr, w.ptr, rows, cols, xt, wt, eps, scale_mode, static_cast<const float*>(sc.ptr),
-                             q.ptr, s.ptr, ro.ptr, no.ptr, ws.ptr, byte_size(ws, "workspace"), current_stream()));
+                             q.ptr, s.ptr, ro.ptr, no.ptr, ws.ptr, byte_size(ws, "workspace"), cur.stream));
 }
 
 void dispatch_router_logits(py::object x_, py::object w_, py::object logits_) {
-  auto x = as_tensor(x_, "x"), w = as_tensor(w_, "w"), l = as_tensor(logits_, "logits");
-  want_current_device({{&x_, "x"}, {&w_, "w"}, {&logits_, "logits"}});
-  want_dtype(x, "x", kBf16);
-  want_dtype(w, "w", kBf16);
-  want_dtype(l, "logits", kF32);
+  const Current cur = current();
+  auto x = as_current(x_, "x", cur), w = as_current(w_, "w", cur), l = as_current(logits_, "logits", cur);
+  if (x.dtype != kBf16 || w.dtype != kBf16) throw std::runtime_error("x and w: expected dtype torch.bfloat16");
+  if (l.dtype != kF32) throw std::runtime_error("logits: expected dtype torch.float32");
   want_dim(x, "x", 2);
   want_dim(w, "w", 2);
   want_dim(l, "logits", 2);
@@ -854,17 +873,16 @@ void dispatch_router_logits(py::object x_, py::object w_, py::object logits_) {
   if (l.shape[0] != x.shape[0] || l.shape[1] != w.shape[0]) throw std::runtime_error("logits must be [T, E]");
   if (w.shape[0] > kMaxInt) throw std::runtime_error("w: too many experts");
   check(hkmoe_router_logits(x.ptr, w.ptr, x.shape[0], static_cast<int32_t>(w.shape[0]), x.shape[1],
-                            static_cast<float*>(l.ptr), current_stream()));
+                            static_cast<float*>(l.ptr), cur.stream));
 }
 
 void dispatch_lora_add(py::object y_, py::object x_, py::object a_, py::object b_, py::object ids_, py::object scaling_,
                        py::object out_, py::object workspace_) {
   int64_t ys = 0, xs = 0, os = 0;
-  auto y = as_rows(y_, "y", &ys), x = as_rows(x_, "x", &xs), o = as_rows(out_, "out", &os);
-  auto a = as_tensor(a_, "a"), b = as_tensor(b_, "b"), i = as_tensor(ids_, "ids"), sc = as_tensor_opt(scaling_, "scaling"),
-       ws = as_tensor_opt(workspace_, "workspace");
-  want_current_device({{&y_, "y"}, {&x_, "x"}, {&a_, "a"}, {&b_, "b"}, {&ids_, "ids"}, {&scaling_, "scaling"}, {&out_, "out"},
-                       {&workspace_, "workspace"}});
+  const Current cur = current();
+  auto y = as_current(y_, "y", cur, &ys), x = as_current(x_, "x", cur, &xs), o = as_current(out_, "out", cur, &os),
+       a = as_current(a_, "a", cur), b = as_current(b_, "b", cur), i = as_current(ids_, "ids", cur),
+       sc = as_current_opt(scaling_, "scaling", cur), ws = as_current_opt(workspace_, "workspace", cur);
   const int yt = float_type(y, "y");
   want_dtype(o, "out", y.dtype.name);
   if (o.dtype != y.dtype.name) throw std::runtime_error("out must have y's dtype");
@@ -884,7 +902,7 @@ void dispatch_lora_add(py::object y_, py::object x_, py::object a_, py::object b
   if (adapters > kMaxInt || rank > kMaxInt) throw std::runtime_error("a: too many adapters or ranks");
   check(hkmoe_lora_add(y.ptr, ys, x.ptr, xs, a.ptr, b.ptr, static_cast<const int32_t*>(i.ptr),
                        static_cast<const float*>(sc.ptr), rows, static_cast<int32_t>(adapters), hidden, n,
-                       static_cast<int32_t>(rank), yt, o.ptr, os, ws.ptr, byte_size(ws, "workspace"), current_stream()));
+                       static_cast<int32_t>(rank), yt, o.ptr, os, ws.ptr, byte_size(ws, "workspace"), cur.stream));
 }
 
 }  // namespace

@@ -24,7 +24,6 @@ def rms_norm_quant(x, weight, residual=None, scales="group", scale=None, eps=1e-
     new residual stream x + residual in x's type (x itself without a residual,
     ``residual_out`` where given: it may be x or residual); n the norm in bf16
     with ``with_norm``, else None."""
-    _check_dev(x, weight, residual, scale)
     if scales not in _MODES:
         raise RuntimeError(f"rms_norm_quant: scales must be one of {sorted(_MODES)}, got {scales!r}")
     if x.dim() != 2:
@@ -57,7 +56,6 @@ def rms_norm_quant(x, weight, residual=None, scales="group", scale=None, eps=1e-
 
 def router_logits(x, w, out=None):
     """fp32 [T, E] router logits of bf16 x [T, H] and the router's bf16 weight w [E, H]."""
-    _check_dev(x, w, out)
     if out is None:
         out = x.new_empty((x.shape[0], w.shape[0]), dtype=torch.float32)
     tk_kernel.dispatch_router_logits(x, w, out)
@@ -72,11 +70,14 @@ def lora_add(y, x, a, b, ids, scaling=None, out=None, workspace=None):
     buffers; a [L, R, H], b [L, N, R] bf16; ids int32 [T]; scaling fp32 [L].
     ``out`` may be y itself (in place).  ``workspace``: uint8, at least
     tk_kernel.lora_workspace_size(T, H, R) bytes, allocated per call if None."""
-    _check_dev(y, x, a, b, ids, scaling, out)
+    if a.dim() != 3:
+        raise RuntimeError("lora_add: a must be [L, R, H]")
     if out is None:
-        out = y.new_empty(y.shape)
-    if workspace is None and y.shape[0] > 0:
-        workspace = x.new_empty((tk_kernel.lora_workspace_size(x.shape[0], a.shape[2], a.shape[1]),), dtype=torch.uint8)
+        out = _like(y, y.dtype)
+    if workspace is None:
+        _, rank, hidden = a.shape
+        need = tk_kernel.lora_workspace_size(y.shape[0], hidden, rank)
+        workspace = a.new_empty((need,), dtype=torch.uint8) if need else None
     tk_kernel.dispatch_lora_add(y, x, a, b, ids, scaling, out, workspace)
     return out
 

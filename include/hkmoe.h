@@ -406,7 +406,7 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
 /*
  * What stands between a residual stream and the FP8 products.  No reference
  * counterpart (the reference has no norm, router or adapters).  All tensors are
- * row-major and 16-byte aligned, rows at most 2^26; no entry point reads an output.
+ * row-major and 16-byte aligned, rows at most 2^24; no entry point reads an output.
  *
  * hkmoe_rms_norm_quant: the residual's addition, the norm and the e4m3 operand.
  *     r = x + residual, rounded to x's type (written to residual_out)

@@ -111,7 +111,7 @@ def test_grids_stay_in_range(fake):
     """The largest sizes that are taken launch with every dimension below 2^32 work-items."""
     out = hip_host.run(fake, """
         size, dbl = ctypes.c_size_t, ctypes.c_double
-        big, st = 1 << 26, vp(5)
+        big, st = 1 << 24, vp(5)
         lib.hkmoe_lora_workspace_size.restype = size
         for rows in (1, 64, 5000, big):
             for cols in (8, 128, 65536):
@@ -131,4 +131,4 @@ def test_grids_stay_in_range(fake):
     assert launches and all(l.endswith("stream=5") for l in launches)
     for l in launches:
         grid = int(l.split("grid=")[1].split()[0])
-        assert 1 <= grid and grid * (1024 if "norm" in l else 256) < 1 << 32, l
+        assert 1 <= grid and grid * (1024 if "norm" in l else 512) < 1 << 32, l
