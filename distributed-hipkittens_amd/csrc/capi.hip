@@ -681,23 +681,25 @@ int launch_router_strip(const RouterParams& p, hipStream_t s) {
 }
 
 // The router's kernel: the cheapest by estimated time (us), rounds of 256 workgroups x (start
-// + K steps x time per step), fitted to launches in a row on 21 shapes (T 1 .. 16384, E 8 ..
-// 512, H 1024 .. 7168), on each of which it picks the fastest:
-//   64x128x4096    strips 16x16 7.4, 32x32 9.9, panels 64x64 16.0, 64x128 22.0
-//   1024x256x7168  38.4, 15.3, 26.4, 36.5
-//   4096x256x7168  157, 56.6, 27.4, 37.2
-//   8192x256x7168  301, 146, 43.3, 39.0
+// + K steps x time per step), fitted to launches in a row on 22 shapes (T 1 .. 16384, E 8 ..
+// 512, H 1024 .. 7168), on 21 of which it picks the fastest (5000x4096x16: 4% off):
+//                  strips 16x16, 16x32, 32x32, panels 64x64, 64x128
+//   64x4096x128     6.0    8.5    9.8   14.6   19.2
+//   512x7168x256   17.1   13.2   15.3   24.1   32.2
+//   1024x7168x256  31.6   24.3   15.8   24.0   32.0
+//   4096x7168x256 148.4   94.7   56.8   25.3   32.3
+//   8192x7168x256 280.1  183.7  145.7   42.5   34.3
 int launch_router(const RouterParams& p, hipStream_t s) {
   const double steps = static_cast<double>((p.hidden + kRowsStep - 1) / kRowsStep);
   auto rounds = [&](int64_t rows, int64_t cols) {
     const int64_t tiles = (p.rows + rows - 1) / rows * ((p.experts + cols - 1) / cols);
     return static_cast<double>((tiles + 255) / 256);
   };
-  const double t11 = 1.3 + rounds(16, 16) * (2.2 + 0.0625 * steps), t12 = 1.3 + rounds(16, 32) * (2.8 + 0.075 * steps),
+  const double t11 = 1.3 + rounds(16, 16) * (2.0 + 0.047 * steps), t12 = 1.3 + rounds(16, 32) * (2.8 + 0.075 * steps),
                t22 = 1.3 + rounds(32, 32) * (2.6 + 0.0975 * steps),
                t64 = 2.0 + steps * (0.075 + 0.15 * rounds(64, 64)), t128 = 2.0 + steps * 0.335 * rounds(64, 128);
   const double best = std::min({t11, t12, t22, t64, t128});
-  if (best == t11) return launch_router_strip<Strip<1, 1, 8, 4>>(p, s);
+  if (best == t11) return launch_router_strip<Strip<1, 1, 16, 2>>(p, s);
   if (best == t12) return launch_router_strip<Strip<1, 2, 8, 3>>(p, s);
   if (best == t22) return launch_router_strip<Strip<2, 2, 8, 2>>(p, s);
   if (best == t64) return launch_router_panel<Panel<64, 64, 2, 2, 4>>(p, s);

@@ -180,6 +180,7 @@ constexpr const char* kF8 = "torch.float8_e4m3fn";
 constexpr const char* kBf16 = "torch.bfloat16";
 constexpr const char* kF32 = "torch.float32";
 constexpr const char* kI32 = "torch.int32";
+constexpr const char* kU8 = "torch.uint8";
 constexpr int64_t kMaxInt = INT32_MAX;
 
 int scale_mode_of(const TensorArg& s) {
@@ -565,7 +566,6 @@ void dispatch_quant_tensor(py::object x, py::object q, py::object s, py::object 
 
 // MX (e8m0 1x32) operands: raw exponents are uint8 [R, C/32]; packed
 // exponent words are int32 [C/128, R64] (R64 = R rounded up to 64).
-constexpr const char* kU8 = "torch.uint8";
 
 int64_t round64(int64_t r) { return (r + 63) / 64 * 64; }
 
@@ -757,6 +757,54 @@ void dispatch_moe_mx(py::object x_q, py::object x_e8m0, py::object logits, py::o
 // Residual + norm + quantisation, router, adapters.  Unlike the calls above these
 // check that every tensor lives on torch's current device, whose stream they use.
 // ---------------------------------------------------------------------------
+// The part of the DLPack 1.x exchange interface (a capsule that a tensor type offers as
+// __dlpack_c_exchange_api__) which describes a tensor in place: one C call and 50 ns, where
+// its Python attributes take 450.
+struct DlTensor {
+  void* data;
+  int32_t device_type, device_id;
+  int32_t ndim;
+  uint8_t code, bits;
+  uint16_t lanes;
+  int64_t *shape, *strides;  // the tensor's own
+  uint64_t byte_offset;
+};
+struct DlExchange {
+  uint32_t major, minor;
+  void *prev, *allocate, *managed_from_object, *managed_to_object;
+  int (*describe)(void* object, DlTensor* out);  // 0, or -1 with a Python error
+};
+constexpr int32_t kDlRocm = 10;
+
+// torch.Tensor's, null where torch offers none (then the attributes are read).
+const DlExchange* exchange() {
+  static bool looked = false;  // with the GIL held, as names()
+  static const DlExchange* kept = nullptr;
+  if (looked) return kept;
+  py::object cap = py::reinterpret_steal<py::object>(PyObject_GetAttrString(names().tensor_type, "__dlpack_c_exchange_api__"));
+  if (cap && PyCapsule_IsValid(cap.ptr(), "dlpack_exchange_api")) {
+    const auto* api = static_cast<const DlExchange*>(PyCapsule_GetPointer(cap.ptr(), "dlpack_exchange_api"));
+    if (api->major == 1 && api->describe != nullptr) {
+      kept = api;
+      cap.release();  // held for good, as names() are
+    }
+  }
+  PyErr_Clear();
+  looked = true;
+  return kept;
+}
+
+const char* dl_dtype(const DlTensor& d) {
+  if (d.lanes == 1) {
+    if (d.code == 4 && d.bits == 16) return kBf16;
+    if (d.code == 2 && d.bits == 32) return kF32;
+    if (d.code == 10 && d.bits == 8) return kF8;
+    if (d.code == 0 && d.bits == 32) return kI32;
+    if (d.code == 1 && d.bits == 8) return kU8;
+  }
+  return "another type";
+}
+
 // torch's current device and its current stream.
 struct Current {
   int64_t device;
@@ -781,6 +829,40 @@ TensorArg as_current(const py::object& obj, const char* name, const Current& cur
     throw std::runtime_error(std::string(name) + ": expected a torch.Tensor");
   }
   TensorArg t;
+  if (const DlExchange* dl = exchange()) {
+    DlTensor d;
+    if (dl->describe(o, &d) != 0) {
+      PyErr_Clear();
+      throw std::runtime_error(std::string(name) + ": expected a dense tensor");
+    }
+    const size_t nd = static_cast<size_t>(d.ndim);
+    int64_t want = 1;
+    bool flat = true, empty = false;
+    for (size_t k = 0; k < nd; ++k) {
+      t.shape.push_back(d.shape[k]);
+      empty |= d.shape[k] == 0;
+    }
+    for (size_t k = nd; k-- > 0;) {
+      flat &= d.strides == nullptr || d.shape[k] == 1 || d.strides[k] == want;
+      want *= d.shape[k];
+    }
+    flat |= empty;
+    if (stride != nullptr) {
+      if (nd != 2) throw std::runtime_error(std::string(name) + ": expected 2-D tensor");
+      *stride = d.shape[1];
+      if (!flat) {
+        if (d.shape[1] > 1 && d.strides[1] != 1) throw std::runtime_error(std::string(name) + ": rows must be contiguous");
+        if (d.shape[0] > 1) *stride = d.strides[0];
+      }
+    } else if (!flat) {
+      throw std::runtime_error(std::string(name) + ": tensor must be contiguous");
+    }
+    if (d.device_type != kDlRocm) throw std::runtime_error(std::string(name) + ": tensor must be on a GPU device");
+    if (d.device_id != cur.device) throw std::runtime_error(std::string(name) + ": tensor must be on the current device");
+    t.ptr = static_cast<uint8_t*>(d.data) + d.byte_offset;
+    t.dtype.name = dl_dtype(d);
+    return t;
+  }
   const py::object shape = steal(PyObject_GetAttr(o, nm.shape));
   for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(shape.ptr()); ++k)
     t.shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(shape.ptr(), k)));
