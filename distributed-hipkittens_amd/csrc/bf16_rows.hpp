@@ -768,4 +768,73 @@ __global__ __launch_bounds__(kLoraWaves * 64, F32 ? 2 : 3) void lora_expand_kern
   });
 }
 
+// Few rows: one workgroup per row and 256 CPT columns, CPT columns per thread, plain fp32
+// products (v needs no terms).  What bounds a handful of rows is the chain of memory accesses
+// and the instructions between them, and here two accesses follow the row's id: v, B and y
+// together, then the store.  Each row reads its adapter's B, from the L2s where rows share it.
+constexpr int kLoraSmallRank = 64;  // CPT columns take ranks up to 64 / CPT
+template <bool F32, int CPT>
+__global__ __launch_bounds__(256) void lora_expand_small_kernel(LoraParams p) {
+  using T = std::conditional_t<F32, float, uint16_t>;
+  constexpr int kChunks = kLoraSmallRank / 8 / CPT;  // of 8 ranks
+  __shared__ __align__(16) float vs[kLoraSmallRank];
+  const int64_t t = blockIdx.x;
+  const int c0 = blockIdx.y * 256 * CPT + threadIdx.x;
+  const int id = p.ids[t];
+  const T* yr = static_cast<const T*>(p.y) + t * p.y_stride;
+  T* out = static_cast<T*>(p.out) + t * p.out_stride;
+  T y[CPT];
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) y[c] = yr[min(c0 + 256 * c, p.n - 1)];
+  if (id < 0 || id >= p.adapters) {
+#pragma unroll
+    for (int c = 0; c < CPT; ++c)
+      if (p.y != p.out && c0 + 256 * c < p.n) out[c0 + 256 * c] = y[c];
+    return;
+  }
+  uint4 b[CPT][kChunks];
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+    const uint16_t* br = p.b + (static_cast<int64_t>(id) * p.n + min(c0 + 256 * c, p.n - 1)) * p.rank;
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k)
+      if (8 * k < p.rank) b[c][k] = *reinterpret_cast<const uint4*>(br + 8 * k);
+  }
+  if (static_cast<int>(threadIdx.x) < p.rank) {
+    const float* src = p.v + t * p.rank + threadIdx.x;
+    float v = 0.0f;
+    for (int s = 0; s < p.splits; s += 8) {
+      float part[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) part[u] = src[min(s + u, p.splits - 1) * p.rows * p.rank];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (s + u < p.splits) v += part[u];
+    }
+    vs[threadIdx.x] = p.scaling != nullptr ? v * p.scaling[id] : v;
+  }
+  __syncthreads();
+  float d[CPT] = {};
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) {
+    if (8 * k < p.rank) {
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) {
+        const uint32_t w[4] = {b[c][k].x, b[c][k].y, b[c][k].z, b[c][k].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          d[c] = __builtin_fmaf(vs[8 * k + 2 * e], __uint_as_float(w[e] << 16), d[c]);
+          d[c] = __builtin_fmaf(vs[8 * k + 2 * e + 1], __uint_as_float(w[e] & 0xffff0000u), d[c]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+    if (c0 + 256 * c >= p.n) continue;
+    if constexpr (F32) out[c0 + 256 * c] = y[c] + d[c];
+    else out[c0 + 256 * c] = static_cast<uint16_t>(bf16_rne_bits(bf16_bits_to_f32(y[c]) + d[c]));
+  }
+}
+
 }  // namespace hkmoe

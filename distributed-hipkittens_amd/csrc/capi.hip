@@ -706,6 +706,25 @@ int launch_router(const RouterParams& p, hipStream_t s) {
   return launch_router_panel<Panel<64, 128, 2, 4, 4>>(p, s);
 }
 
+// Rows x rank up to which each row reads its own B (lora_expand_small_kernel), for ranks to 32 and
+// to 64.  Both launches, us, N = 4096, as a graph: rows shuffled over 64 adapters / in
+// segments of 4 or 8, small kernel against matrix instruction
+//   512 x 16    13.7 / 10.3,  62 / 11.3        2048 x 16  36 / 21,  180 / 16
+//   4096 x 16   84 / 34,     284 / 26
+//   128 x 64    21 / 17,      26 / 12          256 x 64   34 / 27,   45 / 14
+// The small kernel's loss on segments is bounded, the other's on shuffled rows is not.
+constexpr int64_t kLoraSmallWork = 32768, kLoraSmallWork64 = 8192;
+// Rows x columns up to which a thread takes one column (both launches, rank 16, 64x4096: 9.2 us
+// with one, 9.6 with four; 512x4096: 17.1, 13.7).
+constexpr int64_t kLoraNarrow = 1 << 18;
+
+template <bool F32, int CPT>
+int launch_lora_small(const LoraParams& p, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(p.rows), static_cast<unsigned>((p.n + 256 * CPT - 1) / (256 * CPT)));
+  hipLaunchKernelGGL((lora_expand_small_kernel<F32, CPT>), grid, dim3(256), 0, s, p);
+  return check_launch("lora_expand_small_kernel");
+}
+
 constexpr int64_t kLoraCached = 16 << 20;  // bytes of y up to which its accesses go through the L2s
 
 template <bool F32, int TERMS, bool NT>
@@ -1663,11 +1682,18 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
   auto s = static_cast<hipStream_t>(stream);
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock;
   const unsigned grid_x = static_cast<unsigned>(blocks <= 8 ? blocks : (blocks + 7) / 8 * 8);
-  // parts of a block's adapters: one per row as far as two workgroups per CU go
-  auto parts = [&](int64_t per) { return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(kRowsBlock, 1024 / (blocks * per)))); };
+  // parts of a block's adapters: one for each it can have, as far as four workgroups per CU go
+  const int64_t most = std::min<int64_t>(kRowsBlock, static_cast<int64_t>(adapters) + 1);
+  auto parts = [&](int64_t per) { return static_cast<unsigned>(std::max<int64_t>(1, std::min(most, 1024 / (blocks * per)))); };
   hipLaunchKernelGGL((rank <= 16 ? lora_shrink_kernel<1> : rank <= 32 ? lora_shrink_kernel<2> : lora_shrink_kernel<4>),
                      dim3(grid_x, parts(p.splits), p.splits), dim3(kLoraWaves * 64), 0, s, p);
   HK_TRY(check_launch("lora_shrink_kernel"));
+  if (rank <= kLoraSmallRank && rows * rank <= (rank <= 32 ? kLoraSmallWork : kLoraSmallWork64)) {
+    const bool f32 = y_dtype == HKMOE_F32;
+    if (rank > 32 || rows * n <= kLoraNarrow) return f32 ? launch_lora_small<true, 1>(p, s) : launch_lora_small<false, 1>(p, s);
+    if (rank > 16) return f32 ? launch_lora_small<true, 2>(p, s) : launch_lora_small<false, 2>(p, s);
+    return f32 ? launch_lora_small<true, 4>(p, s) : launch_lora_small<false, 4>(p, s);
+  }
   const int64_t strips = (n + 255) / 256, cols = std::min<int64_t>({strips, 65535, std::max<int64_t>(1, 512 / blocks)});
   p.cols_per_wg = static_cast<int32_t>((strips + cols - 1) / cols * 256);
   const dim3 grid(grid_x, parts(cols), static_cast<unsigned>((n + p.cols_per_wg - 1) / p.cols_per_wg));

@@ -259,6 +259,27 @@ def test_lora_many(hk, t, adapters, how):
     _lora_case(hk, t, 128, 320, 16, adapters, how)
 
 
+@pytest.mark.parametrize("t,r", [(1, 72), (15, 136), (16, 72), (17, 72), (33, 256), (63, 72), (64, 136), (65, 72), (130, 72),
+                                 (204, 40), (205, 40), (257, 64), (1024, 32), (1025, 32), (2049, 16)])
+@pytest.mark.parametrize("how", ["none", "one", "mixed", "segments", "out of range"])
+def test_lora_matrix_rows(hk, t, r, how):
+    """Ranks and row counts on both sides of the matrix instruction's share."""
+    _lora_case(hk, t, 72, 264, r, 5, how, bf16=(t + r) % 2 == 0, wide=8 if t % 3 else 0, in_place=t % 4 == 1)
+
+
+@pytest.mark.parametrize("n", [8, 56, 64, 72, 248, 256, 264, 520, 1032, 4104])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_lora_matrix_columns(hk, n, bf16):
+    _lora_case(hk, 70, 64, n, 72, 4, "mixed", bf16=bf16, wide=16, in_place=bf16)
+
+
+@pytest.mark.parametrize("t,n,r,bf16", [(2100, 4104, 16, True), (2100, 2056, 24, False), (1100, 8200, 72, True)])
+def test_lora_large_outputs(hk, t, n, r, bf16):
+    """Outputs past what the caches hold."""
+    _lora_case(hk, t, 64, n, r, 6, "segments", bf16=bf16)
+    _lora_case(hk, t, 64, n, r, 6, "mixed", bf16=bf16, in_place=True)
+
+
 def test_lora_far_offsets(hk):
     """An adapter whose weights lie past 2^31 values, and far rows of strided x, y and out."""
     l, r, h, n = 140, 256, 65536, 512
