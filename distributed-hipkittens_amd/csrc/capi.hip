@@ -1643,8 +1643,8 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
                    hkmoe_stream_t stream) {
   HK_REQUIRE(rows >= 0 && rows <= kMaxRows && adapters >= 1, "lora_add: bad shape rows=%lld adapters=%d",
              (long long)rows, adapters);
-  HK_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= (1 << 20) && n > 0 && n % 8 == 0 && n <= (1 << 24),
-             "lora_add: H=%lld and N=%lld must be multiples of 8, at most 2^20 and 2^24", (long long)hidden, (long long)n);
+  HK_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= (1 << 20) && n > 0 && n % 8 == 0 && n <= (1 << 23),
+             "lora_add: H=%lld and N=%lld must be multiples of 8, at most 2^20 and 2^23", (long long)hidden, (long long)n);
   HK_REQUIRE(rank > 0 && rank % 8 == 0 && rank <= kLoraMaxRank, "lora_add: rank=%d must be a multiple of 8, at most %d",
              rank, kLoraMaxRank);
   HK_REQUIRE(y_dtype == HKMOE_BF16 || y_dtype == HKMOE_F32, "lora_add: bad y_dtype %d", y_dtype);

@@ -406,7 +406,8 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
 /*
  * What stands between a residual stream and the FP8 products.  No reference
  * counterpart (the reference has no norm, router or adapters).  All tensors are
- * row-major and 16-byte aligned, rows at most 2^24; no entry point reads an output.
+ * row-major and 16-byte aligned, rows at most 2^24; outputs overlap nothing but what is
+ * said below.
  *
  * hkmoe_rms_norm_quant: the residual's addition, the norm and the e4m3 operand.
  *     r = x + residual, rounded to x's type (written to residual_out)
@@ -437,7 +438,7 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
  *   a [adapters, rank, H], b [adapters, N, rank] bf16 contiguous, ids [T] int32,
  *   scaling [adapters] fp32 or NULL (1).  out may be y itself (with its stride; rows
  *   without an adapter are then not touched) and overlaps nothing else.
- *   H % 8 == 0, N % 8 == 0, rank % 8 == 0, rank <= 256, H <= 2^20, N <= 2^24; pad
+ *   H % 8 == 0, N % 8 == 0, rank % 8 == 0, rank <= 256, H <= 2^20, N <= 2^23; pad
  *   smaller ranks with zeros.  v = x A_l^T is kept to 2^-17 (fp32 y: 2^-25) of its
  *   value; an infinite value of A or B gives an infinity or a NaN.
  *   workspace: hkmoe_lora_workspace_size(T, H, rank) bytes, not shared by calls that

@@ -73,7 +73,7 @@ def _lora(lib, y=P, ys=64, x=P, xs=256, a=P, b=P, ids=P, scaling=None, rows=4, a
 @pytest.mark.parametrize("bad,says", [
     (dict(y=None), "null"), (dict(x=None), "null"), (dict(a=None), "null"), (dict(b=None), "null"), (dict(ids=None), "null"),
     (dict(out=None), "null"), (dict(rows=-1), "shape"), (dict(rows=1 << 27), "shape"), (dict(adapters=0), "shape"),
-    (dict(h=12), "multiples of 8"), (dict(n=60), "multiples of 8"), (dict(n=0), "multiples of 8"), (dict(r=12), "rank"),
+    (dict(h=12), "multiples of 8"), (dict(n=60), "multiples of 8"), (dict(n=0), "multiples of 8"), (dict(n=(1 << 23) + 8, ys=1 << 24, os_=1 << 24), "2^23"), (dict(xs=(1 << 25) + 8), "2^25"), (dict(r=12), "rank"),
     (dict(r=0), "rank"), (dict(r=264), "rank"), (dict(yt=2), "y_dtype"), (dict(xs=248), "strides"), (dict(xs=260), "strides"),
     (dict(ys=56), "strides"), (dict(ys=68), "strides"), (dict(os_=60), "strides"), (dict(yt=1, ys=66), "strides"),
     (dict(os_=72), "row stride"), (dict(y=ODD), "aligned"), (dict(x=ODD), "aligned"), (dict(out=ODD), "aligned"),
@@ -121,7 +121,7 @@ def test_grids_stay_in_range(fake):
                                                     None, P, size(1 << 50), st) == 0
             for e in (1, 256, 1024):
                 assert lib.hkmoe_router_logits(P, P, i64(rows), i32(e), i64(4096), P, st) == 0
-            for n in (8, 4096, 1 << 24):
+            for n in (8, 4096, 1 << 23):
                 for yt in (0, 1):
                     assert lib.hkmoe_lora_add(P, i64(n), P, i64(256), P, P, P, None, i64(rows), i32(1000), i64(256), i64(n),
                                               i32(16), yt, P, i64(n), P, size(1 << 50), st) == 0
