@@ -107,7 +107,7 @@ __device__ __forceinline__ void rows_reduce(const f32x4 (&acc)[MT][NT], float* r
 //
 // A load in operand order touches 16 rows of 64 bytes, and a CU gets a third of its
 // rate from such loads (8192x7168 rows against 64 columns: 37 us straight into
-// registers, of which 17 for the columns alone).  So the rows of both operands come in
+// registers, 29 through LDS).  So the rows of both operands come in
 // whole 128-byte lines by global->LDS DMA, K steps of 64 in a ring of STAGES, swizzled
 // (chunk c of row r at slot c ^ swz(r)) so that the fragment reads spread over the banks.
 // WM x WN waves, each with MT x NT tiles of 16x16 outputs.
@@ -127,8 +127,8 @@ struct Panel {
 // flight, L loads each, then a barrier: every wave's loads of the older ones are in LDS, and
 // every wave's LDS reads are done.  The compiler's own s_waitcnt (simm16: vmcnt in bits 0-3
 // and 14-15, lgkmcnt in 8-11), so that it knows the fragments read so far to be complete
-// and adds no lgkmcnt(0) between the next step's reads and this step's products (55 us
-// with one, 8192x7168x256).
+// and adds no lgkmcnt(0) between the next step's reads and this step's products
+// (8192x7168x256 from the Infinity Cache 46 us, with the reads ahead of the products 42).
 template <int L, int MOST>
 __device__ __forceinline__ void panel_wait(int newer) {
   if constexpr (MOST > 0) {
@@ -381,6 +381,7 @@ __global__ __launch_bounds__(S::NW * 64) void router_strip_kernel(RouterParams p
 
 // Many rows: one workgroup per panel tile.  The column tiles of a row tile run side by
 // side on one XCD (workgroups go round-robin over the 8), so x comes from HBM once.
+// 8192x7168x256: 52 us, 2.5 TB/s and 580 TFLOP/s, bound by what a CU takes in (24 KiB a step).
 template <typename P>
 __global__ __launch_bounds__(P::kWaves * 64) void router_panel_kernel(RouterParams p, int row_tiles, int col_tiles) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -417,6 +418,7 @@ __global__ __launch_bounds__(P::kWaves * 64) void router_panel_kernel(RouterPara
 // the requests of a decode batch each find their workgroup, with no sorted order
 // to build first.  Two launches: the narrow product v = x A_l^T (its K split over
 // `splits` workgroups, each writing its own fp32 partial sums), then y + c_l v B_l^T.
+// 8192 rows, 7168 -> 64 -> 4096, bf16: 32 us (22 at a copy's rate) and 44 (28).
 // ---------------------------------------------------------------------------
 struct LoraParams {
   const void* y;

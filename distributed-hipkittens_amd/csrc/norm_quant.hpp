@@ -15,7 +15,8 @@
 // Bound by HBM: per value it reads x and the residual and writes the residual, one
 // byte and, where asked for, the bf16 norm.  One workgroup per row, the row in
 // registers between the sum and the quantisation (8 values a chunk, 16-byte
-// loads), so each value is read once.
+// loads), so each value is read once.  8192x7168 bf16 with a residual, groups and the bf16
+// norm: 117 us, 4.5 TB/s (a copy: 4.7).
 #pragma once
 
 #include "common.hpp"

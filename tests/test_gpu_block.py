@@ -252,6 +252,13 @@ def test_lora_ranks(hk, r, bf16):
     _lora_case(hk, 40, 512, 136, r, 4, "mixed", bf16=bf16, scaled=r % 16 == 0)
 
 
+@pytest.mark.parametrize("h", [8, 72, 120, 1000, 4096])
+@pytest.mark.parametrize("r", [8, 16, 24, 32, 40, 64, 72, 200])
+def test_lora_panels(hk, h, r):
+    """More than 16 rows of an adapter: every rank tile, ragged and whole K."""
+    _lora_case(hk, 90, h, 72, r, 2, "one", bf16=r % 16 == 0)
+
+
 @pytest.mark.parametrize("t,adapters,how", [(64, 70, "mixed"), (256, 300, "mixed"), (2000, 3, "segments"),
                                             (5000, 64, "segments"), (1500, 200, "mixed")])
 def test_lora_many(hk, t, adapters, how):
@@ -446,6 +453,23 @@ def test_on_another_stream(hk):
         got = chain(late, res, ids)
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_streams_at_once(hk):
+    """Calls that overlap in time: each takes its workspace from the allocator."""
+    chains, sets = [_Chain(hk, "mx"), _Chain(hk, "tensor")], [_inputs(8), _inputs(9)]
+    want = [[v.clone() for v in c(*s)] for c, s in zip(chains, sets)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in chains]
+    got = [[], []]
+    for _ in range(10):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(chains[k](*sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for g in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[k]))
 
 
 def test_same_bits_every_time(hk):

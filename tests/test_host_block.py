@@ -132,3 +132,55 @@ def test_grids_stay_in_range(fake):
     for l in launches:
         grid = int(l.split("grid=")[1].split()[0])
         assert 1 <= grid and grid * (1024 if "norm" in l else 512) < 1 << 32, l
+
+
+STAND_IN = hip_host.BINDING + """
+torch.cuda.current_device = lambda: 0
+class T(Tensor):
+    def __init__(self, shape, dtype="torch.bfloat16", dev=0, strides=None):
+        Tensor.__init__(self, shape, dtype)
+        flat, n = [], 1
+        for s in reversed(self.shape):
+            flat.insert(0, n)
+            n *= s
+        self.dev, self.flat, self.strides = dev, tuple(flat), strides or tuple(flat)
+    def is_contiguous(self): return self.strides == self.flat
+    def stride(self): return self.strides
+    def get_device(self): return self.dev
+f32, u8, i32 = "torch.float32", "torch.uint8", "torch.int32"
+def lora(y=T([4, 64]), x=T([4, 256]), a=T([2, 8, 256]), b=T([2, 64, 8]), ids=T([4], i32), scaling=None, out=T([4, 64]),
+         ws=T([1 << 20], u8)):
+    tk_kernel.dispatch_lora_add(y, x, a, b, ids, scaling, out, ws)
+def refused(fn):
+    try:
+        fn()
+    except RuntimeError as e:
+        print("refused:", e)
+    else:
+        print("taken")
+"""
+
+
+def test_tensors_through_their_attributes(fake):
+    """A torch without the exchange interface: the same checks, on the attributes."""
+    out = hip_host.run(fake, STAND_IN + """
+lora()
+lora(y=T([4, 64], strides=(192, 1)), out=T([4, 64], strides=(192, 1)), x=T([4, 256], strides=(512, 1)))
+tk_kernel.dispatch_router_logits(T([4, 64]), T([8, 64]), T([4, 8], f32))
+tk_kernel.dispatch_rms_norm_quant(T([4, 256]), None, T([256]), 1e-6, 1, T([4, 256], "torch.float8_e4m3fn"), T([4, 2], f32))
+for line in log(): print(line)
+refused(lambda: lora(x=T([4, 256], dev=1)))
+refused(lambda: lora(x=T([4, 256], dev=-1)))
+refused(lambda: lora(y=T([4, 64], strides=(1, 4))))
+refused(lambda: lora(a=T([2, 8, 256], strides=(1, 2, 16))))
+refused(lambda: lora(ids=T([4], f32)))
+refused(lambda: lora(y=[1, 2]))
+refused(lambda: tk_kernel.dispatch_router_logits(T([4, 64], strides=(128, 1)), T([8, 64]), T([4, 8], f32)))
+""")
+    launches = [l for l in out if l.startswith("launch")]
+    assert len(launches) == 6 and all(l.endswith("stream=7") for l in launches), out
+    said = [l for l in out if l.startswith("refused")]
+    wanted = ["x: tensor must be on the current device", "x: tensor must be on a GPU device", "y: rows must be contiguous",
+              "a: tensor must be contiguous", "ids: expected dtype torch.int32", "y: expected a torch.Tensor",
+              "x: tensor must be contiguous"]
+    assert [s.split(": ", 1)[1] for s in said] == wanted and "taken" not in out
