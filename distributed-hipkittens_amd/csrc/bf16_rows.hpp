@@ -433,19 +433,20 @@ struct LoraParams {
   float* v;              // [splits][T][R]
   int64_t rows;
   int32_t adapters, hidden, n, rank, splits, cols_per_wg;  // cols_per_wg: a multiple of 256
+  const int32_t* perm;        // [T] rows by adapter, null: row blocks as they come
+  const i32x4* items;         // (adapter or -1, first place in perm, rows)
+  const int32_t* item_count;
 };
 
 constexpr int kLoraWaves = 4;
 constexpr int kLoraMaxRank = 256;
 
-// The row block of a workgroup: each XCD (workgroups are dealt to them in turn) takes a run
-// of blocks, so that the adapters of its segments stay in its L2.  The grid is a multiple
-// of 8 wide; -1 past the last block.
-__device__ __forceinline__ int64_t lora_block(const LoraParams& p) {
-  const int64_t blocks = (p.rows + kRowsBlock - 1) / kRowsBlock;
-  if (blocks <= 8) return blockIdx.x < blocks ? blockIdx.x : -1;
-  const int64_t per = gridDim.x / 8, blk = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  return blk < blocks ? blk : -1;
+// Workgroup `bid` of a grid that is a multiple of 8 wide, as a place among `count`: each XCD
+// (workgroups are dealt to them in turn) takes a run of places, so that the adapters of its
+// rows stay in its L2.  -1 past the last.
+__device__ __forceinline__ int64_t xcd_run(int64_t bid, int64_t count) {
+  const int64_t per = (count + 7) / 8, at = (bid & 7) * per + (bid >> 3);
+  return (bid >> 3) < per && at < count ? at : -1;
 }
 
 // This lane's adapter of row block `blk`: -1 for rows without one, -2 past the end.
@@ -459,31 +460,177 @@ __device__ __forceinline__ int lora_id(const LoraParams& p, int64_t blk) {
   return id;
 }
 
-// Calls `f(id, n)` for this part's adapters among the block's `live` rows, with their n
-// rows listed in `list` (LDS), in order.  With a part per row a part owns the adapter whose
-// first row is its own: one step, however many adapters there are; with fewer parts it
-// owns every parts-th adapter, so that two adapters of a block are two workgroups'.
-// Uniform over the workgroup: every wave holds the same ids.
+// Calls `f(id, n, t0)` for each group of rows of one adapter that is this workgroup's: its n
+// (at most 64) rows are t0 + list[0 .. n - 1] (list: LDS).  `bare`: the rows without an
+// adapter are a group, too (id < 0).  With a plan the workgroup's group is an item of it.
+// Without one it takes adapters of its row block, in order of their first rows: with a part
+// (blockIdx.y) per row the one whose first row is the part's own, which is one step, however
+// many adapters there are; with fewer parts every parts-th, so that two adapters of a block are
+// two workgroups'.  Uniform over the workgroup: every wave holds the same ids.
 template <typename F>
-__device__ __forceinline__ void lora_groups(int id, uint64_t live, int part, int parts, int* list, F f) {
+__device__ __forceinline__ void lora_groups(const LoraParams& p, bool bare, int* list, F f) {
   const int lane = lane_id();
+  const bool planned = p.items != nullptr;
+  int64_t at, t0 = 0;
+  uint64_t live = 0, todo = 0;
+  int id = 0, turn = 0;
+  const int part = blockIdx.y, parts = gridDim.y;
   const bool by_row = parts >= kRowsBlock;
-  uint64_t todo = by_row ? live & (1ull << part) : live;
-  int turn = by_row ? part : 0;
-  while (todo != 0) {
-    const int first = __builtin_ctzll(todo);
-    const int gid = __builtin_amdgcn_readlane(id, first);
-    const uint64_t rows = __ballot(id == gid) & live;
-    todo &= ~rows;
-    if ((rows & ((1ull << first) - 1)) != 0) continue;  // by row: not its first
-    const bool mine = turn == part;
-    if (!by_row) turn = turn + 1 == parts ? 0 : turn + 1;
-    if (!mine) continue;
-    __syncthreads();  // the list's last user is done
-    if (threadIdx.x < 64 && (rows >> lane & 1)) list[__builtin_popcountll(rows & ((1ull << lane) - 1))] = lane;
-    __syncthreads();
-    f(gid, __builtin_popcountll(rows));
+  if (planned) {
+    at = xcd_run(blockIdx.x, *p.item_count);
+    todo = 1;
+  } else {
+    const int64_t blocks = (p.rows + kRowsBlock - 1) / kRowsBlock;
+    at = blocks <= 8 ? blockIdx.x : xcd_run(blockIdx.x, blocks);
   }
+  if (at < 0) return;
+  if (!planned) {
+    t0 = at * kRowsBlock;
+    id = lora_id(p, at);
+    live = __ballot(id >= (bare ? -1 : 0));
+    todo = by_row ? live & (1ull << part) : live;
+    turn = by_row ? part : 0;
+  }
+  while (todo != 0) {
+    int gid, n;
+    if (planned) {
+      const i32x4 item = p.items[at];
+      gid = item.x;
+      n = item.z;
+      if (gid < 0 && !bare) return;
+      if (static_cast<int>(threadIdx.x) < n) list[threadIdx.x] = p.perm[item.y + threadIdx.x];
+      todo = 0;
+    } else {
+      const int first = __builtin_ctzll(todo);
+      gid = __builtin_amdgcn_readlane(id, first);
+      const uint64_t rows = __ballot(id == gid) & live;
+      todo &= ~rows;
+      if ((rows & ((1ull << first) - 1)) != 0) continue;  // by row: not its first
+      const bool mine = turn == part;
+      if (!by_row) turn = turn + 1 == parts ? 0 : turn + 1;
+      if (!mine) continue;
+      n = __builtin_popcountll(rows);
+      __syncthreads();  // the list's last user is done
+      if (threadIdx.x < 64 && (rows >> lane & 1)) list[__builtin_popcountll(rows & ((1ull << lane) - 1))] = lane;
+    }
+    __syncthreads();
+    f(gid, n, t0);
+  }
+}
+
+// The plan: rows sorted by adapter (stable, so that a row's group, and with it the order of its
+// sums, is the same every time), in items of at most 64 rows.  Without it every block of a
+// shuffled batch reads every adapter (1078 rows over 24 adapters, 5672 -> 72 -> 896: 143 us
+// without).  One workgroup; each of its 16 waves counts and places a run of rows, 64 at a
+// time, one step per distinct adapter among them.  LDS: counts [16][bins], places [bins], item
+// places [bins], bins = adapters + 1 (the last: none).
+constexpr int kPlanWaves = 16, kPlanBins = 2048, kPlanRows = 65536;
+constexpr int lora_plan_lds(int bins) { return (kPlanWaves + 2) * bins * 4; }
+constexpr int64_t lora_plan_items(int64_t rows, int64_t adapters) {  // at most
+  return rows / kRowsBlock + (rows < adapters + 1 ? rows : adapters + 1);
+}
+
+__global__ __launch_bounds__(kPlanWaves * 64) void lora_plan_kernel(const int32_t* __restrict__ ids, int rows, int adapters,
+                                                                    int32_t* __restrict__ perm, i32x4* __restrict__ items,
+                                                                    int32_t* __restrict__ item_count) {
+  extern __shared__ int counts[];
+  __shared__ uint64_t sums[kPlanWaves];
+  const int bins = adapters + 1, tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int* start = counts + kPlanWaves * bins;
+  int* item_start = start + bins;
+  int* mine = counts + wave * bins;
+  for (int b = lane; b < bins; b += 64) mine[b] = 0;
+  const int per = (rows + 64 * kPlanWaves - 1) / (64 * kPlanWaves) * 64, end = min(rows, (wave + 1) * per);
+  // f(t0, b, m, first): the rows of mask m among 64 from t0 are bin b's.  The ids of eight
+  // times 64 rows are loaded at once, and once for both passes where a wave has no more.
+  constexpr int kFlight = 8;
+  int bins8[kFlight];
+  auto load = [&](int t8) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const int id = ids[min(t8 + 64 * u + lane, rows - 1)];
+      bins8[u] = id < 0 || id >= adapters ? adapters : id;
+    }
+  };
+  load(wave * per);
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    for (int t8 = wave * per; t8 < end; t8 += 64 * kFlight) {
+      if (per > 64 * kFlight) load(t8);
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        uint64_t todo = __ballot(t8 + 64 * u + lane < end);
+        while (todo != 0) {
+          const int first = __builtin_ctzll(todo);
+          const int b = __builtin_amdgcn_readlane(bins8[u], first);
+          const uint64_t m = __ballot(bins8[u] == b) & todo;
+          todo &= ~m;
+          f(t8 + 64 * u, b, m, lane == first);
+        }
+      }
+    }
+  };
+  each([&](int, int b, uint64_t m, bool first) {
+    if (first) mine[b] += __builtin_popcountll(m);
+  });
+  __syncthreads();
+  // two bins per thread: the waves' places within a bin, the bins' places and items
+  static_assert(kPlanBins <= 2 * 64 * kPlanWaves, "bins per thread");
+  uint64_t v[2] = {0, 0};  // rows, items << 32
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int b = 2 * tid + u;
+    if (b < bins) {
+      int n = 0, c[kPlanWaves];
+#pragma unroll
+      for (int w = 0; w < kPlanWaves; ++w) c[w] = counts[w * bins + b];
+#pragma unroll
+      for (int w = 0; w < kPlanWaves; ++w) {
+        counts[w * bins + b] = n;
+        n += c[w];
+      }
+      v[u] = static_cast<uint64_t>((n + kRowsBlock - 1) / kRowsBlock) << 32 | static_cast<uint32_t>(n);
+    }
+  }
+  uint64_t incl = v[0] + v[1];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t up = __shfl_up(static_cast<unsigned long long>(incl), o, kWave);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  uint64_t at = incl - v[0] - v[1], all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    if (w < wave) at += sums[w];
+    all += sums[w];
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int b = 2 * tid + u;
+    if (b < bins) {
+      start[b] = static_cast<int>(at);
+      item_start[b] = static_cast<int>(at >> 32);
+    }
+    at += v[u];
+  }
+  __syncthreads();
+  const int n_items = static_cast<int>(all >> 32);
+  if (tid == 0) *item_count = n_items;
+  for (int i = tid; i < n_items; i += 64 * kPlanWaves) {
+    int b = 0, past = bins;  // the last bin whose first item is not past i
+    while (past - b > 1) {
+      const int mid = (b + past) >> 1;
+      if (item_start[mid] <= i) b = mid; else past = mid;
+    }
+    const int first = start[b] + (i - item_start[b]) * kRowsBlock;
+    items[i] = i32x4{b == adapters ? -1 : b, first, min(kRowsBlock, (b + 1 < bins ? start[b + 1] : rows) - first), 0};
+  }
+  each([&](int t0, int b, uint64_t m, bool first) {
+    const int to = start[b] + mine[b];
+    if (m >> lane & 1) perm[to + __builtin_popcountll(m & ((1ull << lane) - 1))] = t0 + lane;
+    if (first) mine[b] += __builtin_popcountll(m);
+  });
 }
 
 // v[split] of up to 16 MT rows of adapter `id` and 16 NT ranks from r0.
@@ -519,7 +666,7 @@ __device__ __forceinline__ void lora_shrink_panel(const LoraParams& p, int64_t t
   const int s0 = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
   const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
   f32x4 acc[P::MT][P::NT] = {};
-  // the host keeps 64 rows of x and the ranks of an adapter below 2^32 bytes
+  // the host keeps 64 rows of x (with a plan: all) and the ranks of an adapter below 2^32 bytes
   panel_product<P>(
       smem, p.x + t0 * p.x_stride, [&](int i) { return list[min(i, n - 1)] * static_cast<uint32_t>(2 * p.x_stride); },
       p.a + static_cast<int64_t>(id) * p.rank * p.hidden,
@@ -538,7 +685,8 @@ __device__ __forceinline__ void lora_shrink_panel(const LoraParams& p, int64_t t
     }
 }
 
-// grid: (row blocks, parts of a block's adapters, splits).  16 NT ranks at a time.
+// grid: (row blocks, parts of a block's adapters, splits), or (items, 1, splits).  16 NT ranks
+// at a time.
 template <int NT>
 __global__ __launch_bounds__(kLoraWaves * 64) void lora_shrink_kernel(LoraParams p) {
   using P = Panel<kRowsBlock, NT == 4 ? 64 : 32, NT == 4 ? 2 : 4, NT == 4 ? 2 : 1, 4>;
@@ -546,15 +694,12 @@ __global__ __launch_bounds__(kLoraWaves * 64) void lora_shrink_kernel(LoraParams
   __shared__ __attribute__((aligned(1024))) uint8_t smem[P::kLds > kRed ? P::kLds : kRed];
   float* red = reinterpret_cast<float*>(smem);
   __shared__ int list[kRowsBlock];
-  const int64_t blk = lora_block(p);
-  if (blk < 0) return;
-  const int id = lora_id(p, blk);
-  lora_groups(id, __ballot(id >= 0), blockIdx.y, gridDim.y, list, [&](int gid, int n) {
+  lora_groups(p, false, list, [&](int gid, int n, int64_t t0) {
     for (int r0 = 0; r0 < p.rank; r0 += 16 * NT) {
       if (n > 16)
-        lora_shrink_panel<P>(p, blk * kRowsBlock, gid, n, list, r0, smem);
+        lora_shrink_panel<P>(p, t0, gid, n, list, r0, smem);
       else
-        lora_shrink_tile<1, NT, 4>(p, blk * kRowsBlock, gid, n, list, r0, red);
+        lora_shrink_tile<1, NT, 4>(p, t0, gid, n, list, r0, red);
     }
   });
 }
@@ -718,18 +863,15 @@ __device__ __forceinline__ void lora_copy_rows(const LoraParams& p, int64_t t0, 
   }
 }
 
-// grid: (row blocks, parts of a block's adapters, column parts).  The rows without an
+// grid: (row blocks, parts of a block's adapters, column parts), or (items, 1, column parts).  The rows without an
 // adapter are a group of their own, copied unless out is y.
 template <bool F32, int TERMS, bool NT>
 __global__ __launch_bounds__(kLoraWaves * 64, F32 ? 2 : 3) void lora_expand_kernel(LoraParams p) {
   extern __shared__ __align__(16) float tiles[];  // [waves][16][pitch], then v's terms
   uint16_t* vt = reinterpret_cast<uint16_t*>(tiles + kLoraWaves * 16 * kLoraTilePitch);  // [TERMS][kRowsBlock][pitch]
   __shared__ int list[kRowsBlock];
-  const int64_t blk = lora_block(p), t0 = blk * kRowsBlock;
-  if (blk < 0) return;
-  const int id = lora_id(p, blk);
   const int c_begin = blockIdx.z * p.cols_per_wg, c_end = min(c_begin + p.cols_per_wg, p.n);
-  lora_groups(id, __ballot(p.y != p.out ? id >= -1 : id >= 0), blockIdx.y, gridDim.y, list, [&](int gid, int n) {
+  lora_groups(p, p.y != p.out, list, [&](int gid, int n, int64_t t0) {
     if (gid < 0) {
       lora_copy_rows<F32, NT>(p, t0, n, list, c_begin, c_end);
       return;

@@ -736,12 +736,31 @@ int launch_lora_expand(const LoraParams& p, dim3 grid, hipStream_t s) {
   return check_launch("lora_expand_kernel");
 }
 
+// Workspace: the narrow product's partial sums, then the plan (perm, items, their count).
+size_t lora_plan_bytes(int64_t rows) {
+  if (rows <= kRowsBlock || rows > kPlanRows) return 0;
+  return align256(rows * 4) + align256(lora_plan_items(rows, kPlanBins - 1) * 16) + 256;
+}
+
 // Workgroups over which the adapters' narrow product splits its K steps: enough to
 // fill the chip, at least one step per wave.
 int lora_splits(int64_t rows, int64_t hidden) {
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock, steps = (hidden + kRowsStep - 1) / kRowsStep;
   const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, steps / (2 * kLoraWaves)));
   return static_cast<int>(std::min(most, std::max<int64_t>(1, 400 / std::max<int64_t>(1, blocks))));
+}
+
+size_t lora_partials(int64_t rows, int64_t hidden, int32_t rank) {
+  return align256(static_cast<size_t>(lora_splits(rows, hidden)) * rows * rank * sizeof(float));
+}
+
+// Bytes of A that the row blocks could read, each adapter in each block, from which the rows
+// are sorted first: the plan's launch costs about 4 us.
+constexpr int64_t kLoraPlanBytes = 32ll << 20;
+bool lora_planned(int64_t rows, int64_t x_stride, int32_t adapters, int64_t hidden, int32_t rank) {
+  const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock;
+  return blocks > 1 && rows <= kPlanRows && adapters < kPlanBins && 2 * rows * x_stride < (1ll << 32) - (1 << 22) &&
+         blocks * std::min<int64_t>(adapters, kRowsBlock) * rank * hidden * 2 > kLoraPlanBytes;
 }
 
 }  // namespace
@@ -1634,7 +1653,7 @@ int hkmoe_router_logits(const void* x, const void* w, int64_t num_tokens, int32_
 
 size_t hkmoe_lora_workspace_size(int64_t rows, int64_t hidden, int32_t rank) {
   if (rows <= 0 || hidden <= 0 || rank <= 0) return 0;
-  return align256(static_cast<size_t>(lora_splits(rows, hidden)) * rows * rank * sizeof(float));
+  return lora_partials(rows, hidden, rank) + lora_plan_bytes(rows);
 }
 
 int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* a, const void* b,
@@ -1681,10 +1700,25 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
   p.splits = lora_splits(rows, hidden);
   auto s = static_cast<hipStream_t>(stream);
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock;
-  const unsigned grid_x = static_cast<unsigned>(blocks <= 8 ? blocks : (blocks + 7) / 8 * 8);
+  const bool planned = lora_planned(rows, x_stride, adapters, hidden, rank);
+  const int64_t places = planned ? lora_plan_items(rows, adapters) : blocks;
+  const unsigned grid_x = static_cast<unsigned>(!planned && blocks <= 8 ? blocks : (places + 7) / 8 * 8);
+  if (planned) {
+    static bool done[kMaxDevices] = {false};
+    HK_TRY(raise_lds(lora_plan_kernel, lora_plan_lds(kPlanBins), done));
+    auto* perm = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + lora_partials(rows, hidden, rank));
+    auto* items = reinterpret_cast<i32x4*>(reinterpret_cast<uint8_t*>(perm) + align256(rows * 4));
+    auto* count = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(items) + align256(lora_plan_items(rows, kPlanBins - 1) * 16));
+    hipLaunchKernelGGL(lora_plan_kernel, dim3(1), dim3(kPlanWaves * 64), lora_plan_lds(adapters + 1), s, ids,
+                       static_cast<int>(rows), adapters, perm, items, count);
+    HK_TRY(check_launch("lora_plan_kernel"));
+    p.perm = perm;
+    p.items = items;
+    p.item_count = count;
+  }
   // parts of a block's adapters: one for each it can have, as far as four workgroups per CU go
   const int64_t most = std::min<int64_t>(kRowsBlock, static_cast<int64_t>(adapters) + 1);
-  auto parts = [&](int64_t per) { return static_cast<unsigned>(std::max<int64_t>(1, std::min(most, 1024 / (blocks * per)))); };
+  auto parts = [&](int64_t per) { return static_cast<unsigned>(planned ? 1 : std::max<int64_t>(1, std::min(most, 1024 / (blocks * per)))); };
   hipLaunchKernelGGL((rank <= 16 ? lora_shrink_kernel<1> : rank <= 32 ? lora_shrink_kernel<2> : lora_shrink_kernel<4>),
                      dim3(grid_x, parts(p.splits), p.splits), dim3(kLoraWaves * 64), 0, s, p);
   HK_TRY(check_launch("lora_shrink_kernel"));

@@ -287,6 +287,25 @@ def test_lora_large_outputs(hk, t, n, r, bf16):
     _lora_case(hk, t, 64, n, r, 6, "mixed", bf16=bf16, in_place=True)
 
 
+@pytest.mark.parametrize("how", ["none", "one", "mixed", "segments", "out of range"])
+@pytest.mark.parametrize("t,adapters,r,h", [(65, 200, 128, 2048), (130, 64, 64, 2048), (1000, 20, 72, 1032), (1029, 64, 16, 1048),
+                                            (2500, 2047, 8, 1024), (2500, 2048, 8, 1024), (66, 65, 256, 2056)])
+def test_lora_sorted_first(hk, t, adapters, r, h, how):
+    """Batches whose rows are sorted by adapter first (and, at 2048 adapters, just not)."""
+    _lora_case(hk, t, h, 72, r, adapters, how, bf16=t % 2 == 0, in_place=t % 4 == 2)
+
+
+def test_lora_sorted_first_same_bits(hk):
+    """The groups, and with them the order of each row's sums, are the same every time."""
+    rng = np.random.default_rng(11)
+    y, x, a, b, c = _lora_data(rng, 1500, 2048, 264, 64, 40, False)
+    args = [_dev(y, F32), _dev(x, BF16), _dev(a, BF16), _dev(b, BF16),
+            torch.from_numpy(rng.integers(-1, 40, 1500).astype(np.int32)).cuda(), torch.from_numpy(c).cuda()]
+    first = hk.lora_add(*args)
+    for _ in range(20):
+        assert torch.equal(hk.lora_add(*args), first)
+
+
 def test_lora_far_offsets(hk):
     """An adapter whose weights lie past 2^31 values, and far rows of strided x, y and out."""
     l, r, h, n = 140, 256, 65536, 512
