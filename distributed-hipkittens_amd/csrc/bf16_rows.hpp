@@ -522,10 +522,11 @@ __device__ __forceinline__ void lora_groups(const LoraParams& p, bool bare, int*
 // sums, is the same every time), in items of at most 64 rows.  Without it every block of a
 // shuffled batch reads every adapter (1078 rows over 24 adapters, 5672 -> 72 -> 896: 143 us
 // without).  One workgroup; each of its 16 waves counts and places a run of rows, 64 at a
-// time, one step per distinct adapter among them.  LDS: counts [16][bins], places [bins], item
-// places [bins], bins = adapters + 1 (the last: none).
-constexpr int kPlanWaves = 16, kPlanBins = 2048, kPlanRows = 65536;
-constexpr int lora_plan_lds(int bins) { return (kPlanWaves + 2) * bins * 4; }
+// time: 7 us for 8192 rows in a trace, of which half are the launch and the ids' latency.  LDS: counts [16][bins], places [bins], item
+// places [bins], 512 ids per wave; bins = adapters + 1 (the last: none).
+constexpr int kPlanWaves = 16, kPlanBins = 1536, kPlanRows = 65536, kPlanFlight = 8;
+constexpr int lora_plan_lds(int bins) { return ((kPlanWaves + 2) * bins + kPlanWaves * kPlanFlight * 64) * 4; }
+static_assert(lora_plan_lds(kPlanBins) <= kSkMaxLds - 1024, "LDS budget");
 constexpr int64_t lora_plan_items(int64_t rows, int64_t adapters) {  // at most
   return rows / kRowsBlock + (rows < adapters + 1 ? rows : adapters + 1);
 }
@@ -541,36 +542,39 @@ __global__ __launch_bounds__(kPlanWaves * 64) void lora_plan_kernel(const int32_
   int* mine = counts + wave * bins;
   for (int b = lane; b < bins; b += 64) mine[b] = 0;
   const int per = (rows + 64 * kPlanWaves - 1) / (64 * kPlanWaves) * 64, end = min(rows, (wave + 1) * per);
-  // f(t0, b, m, first): the rows of mask m among 64 from t0 are bin b's.  The ids of eight
-  // times 64 rows are loaded at once, and once for both passes where a wave has no more.
-  constexpr int kFlight = 8;
-  int bins8[kFlight];
+  // f(t, bin) for 64 rows at a time in order (bin -1 past the wave's last).  The ids of eight
+  // times 64 rows are loaded at once, and once for both passes where a wave has no more; through
+  // LDS, so that the loop over them stays one (unrolled, fetching its code took 3 us).
+  int* bins8 = item_start + bins + wave * kPlanFlight * 64;
   auto load = [&](int t8) __attribute__((always_inline)) {
+    int id[kPlanFlight];
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u) {
-      const int id = ids[min(t8 + 64 * u + lane, rows - 1)];
-      bins8[u] = id < 0 || id >= adapters ? adapters : id;
-    }
+    for (int u = 0; u < kPlanFlight; ++u) id[u] = ids[min(t8 + 64 * u + lane, rows - 1)];
+#pragma unroll
+    for (int u = 0; u < kPlanFlight; ++u)
+      bins8[64 * u + lane] = t8 + 64 * u + lane >= end ? -1 : id[u] < 0 || id[u] >= adapters ? adapters : id[u];
   };
   load(wave * per);
   auto each = [&](auto f) __attribute__((always_inline)) {
-    for (int t8 = wave * per; t8 < end; t8 += 64 * kFlight) {
-      if (per > 64 * kFlight) load(t8);
-#pragma unroll
-      for (int u = 0; u < kFlight; ++u) {
-        uint64_t todo = __ballot(t8 + 64 * u + lane < end);
-        while (todo != 0) {
-          const int first = __builtin_ctzll(todo);
-          const int b = __builtin_amdgcn_readlane(bins8[u], first);
-          const uint64_t m = __ballot(bins8[u] == b) & todo;
-          todo &= ~m;
-          f(t8 + 64 * u, b, m, lane == first);
-        }
-      }
+    for (int t8 = wave * per; t8 < end; t8 += 64 * kPlanFlight) {
+      if (per > 64 * kPlanFlight) load(t8);
+#pragma unroll 1
+      for (int u = 0; u < kPlanFlight && t8 + 64 * u < end; ++u) f(t8 + 64 * u + lane, bins8[64 * u + lane]);
     }
   };
-  each([&](int, int b, uint64_t m, bool first) {
-    if (first) mine[b] += __builtin_popcountll(m);
+  // the lanes with this lane's bin: all of them, or a bit of the bin at a time
+  auto same_bin = [&](int bin) __attribute__((always_inline)) {
+    uint64_t same = __ballot(bin >= 0);
+    if (__ballot(bin == __builtin_amdgcn_readfirstlane(bin)) == ~0ull) return same;
+    for (int k = 0; 1 << k < bins; ++k) {
+      const uint64_t set = __ballot(bin >> k & 1);
+      same &= bin >> k & 1 ? set : ~set;
+    }
+    return same;
+  };
+  each([&](int, int bin) {
+    const uint64_t same = same_bin(bin);
+    if (bin >= 0 && (same & ((1ull << lane) - 1)) == 0) mine[bin] += __builtin_popcountll(same);
   });
   __syncthreads();
   // two bins per thread: the waves' places within a bin, the bins' places and items
@@ -626,10 +630,14 @@ __global__ __launch_bounds__(kPlanWaves * 64) void lora_plan_kernel(const int32_
     const int first = start[b] + (i - item_start[b]) * kRowsBlock;
     items[i] = i32x4{b == adapters ? -1 : b, first, min(kRowsBlock, (b + 1 < bins ? start[b + 1] : rows) - first), 0};
   }
-  each([&](int t0, int b, uint64_t m, bool first) {
-    const int to = start[b] + mine[b];
-    if (m >> lane & 1) perm[to + __builtin_popcountll(m & ((1ull << lane) - 1))] = t0 + lane;
-    if (first) mine[b] += __builtin_popcountll(m);
+  each([&](int t, int bin) {
+    const uint64_t same = same_bin(bin);
+    if (bin >= 0) {
+      const uint64_t before = same & ((1ull << lane) - 1);
+      const int to = start[bin] + mine[bin] + __builtin_popcountll(before);
+      perm[to] = t;
+      if (before == 0) mine[bin] += __builtin_popcountll(same);
+    }
   });
 }
 

@@ -754,13 +754,25 @@ size_t lora_partials(int64_t rows, int64_t hidden, int32_t rank) {
   return align256(static_cast<size_t>(lora_splits(rows, hidden)) * rows * rank * sizeof(float));
 }
 
-// Bytes of A that the row blocks could read, each adapter in each block, from which the rows
-// are sorted first: the plan's launch costs about 4 us.
-constexpr int64_t kLoraPlanBytes = 32ll << 20;
+// Whether each row takes its own workgroup in the second launch (lora_expand_small_kernel): up to
+// these rows x rank, for ranks to 32 and to 64.
+bool lora_small(int64_t rows, int32_t rank) {
+  return rank <= kLoraSmallRank && rows * rank <= (rank <= 32 ? kLoraSmallWork : kLoraSmallWork64);
+}
+
+// Whether the rows are sorted by adapter first (a launch, 4-7 us): from as many bytes of A as the row
+// blocks could read, each adapter in each block, or as many groups of rows for the matrix
+// instruction.  us, unsorted / sorted, as a graph:
+//                                    shuffled    in segments
+//   8192 rows of 8, 7168->64->4096   274 / 94     68 / 75
+//   4096 rows of 8, 4096->16->4096    63 / 45     32 / 36
+//   2048 rows of 16, 4096->32->1024   53 / 28     18 / 19
+//   300 rows of 64, 2048->64->2048    85 / 39     27 / 25
+constexpr int64_t kLoraPlanBytes = 32ll << 20, kLoraPlanGroups = 128;
 bool lora_planned(int64_t rows, int64_t x_stride, int32_t adapters, int64_t hidden, int32_t rank) {
-  const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock;
+  const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock, groups = blocks * std::min<int64_t>(adapters, kRowsBlock);
   return blocks > 1 && rows <= kPlanRows && adapters < kPlanBins && 2 * rows * x_stride < (1ll << 32) - (1 << 22) &&
-         blocks * std::min<int64_t>(adapters, kRowsBlock) * rank * hidden * 2 > kLoraPlanBytes;
+         (groups * rank * hidden * 2 > kLoraPlanBytes || (groups >= kLoraPlanGroups && !lora_small(rows, rank)));
 }
 
 }  // namespace
@@ -1722,7 +1734,7 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
   hipLaunchKernelGGL((rank <= 16 ? lora_shrink_kernel<1> : rank <= 32 ? lora_shrink_kernel<2> : lora_shrink_kernel<4>),
                      dim3(grid_x, parts(p.splits), p.splits), dim3(kLoraWaves * 64), 0, s, p);
   HK_TRY(check_launch("lora_shrink_kernel"));
-  if (rank <= kLoraSmallRank && rows * rank <= (rank <= 32 ? kLoraSmallWork : kLoraSmallWork64)) {
+  if (lora_small(rows, rank)) {
     const bool f32 = y_dtype == HKMOE_F32;
     if (rank > 32 || rows * n <= kLoraNarrow) return f32 ? launch_lora_small<true, 1>(p, s) : launch_lora_small<false, 1>(p, s);
     if (rank > 16) return f32 ? launch_lora_small<true, 2>(p, s) : launch_lora_small<false, 2>(p, s);
