@@ -414,10 +414,11 @@ __global__ __launch_bounds__(P::kWaves * 64) void router_panel_kernel(RouterPara
 // adapters
 //
 // Rows come in blocks of kRowsBlock in their own order, and a workgroup takes the
-// rows of one adapter of one block: a segment of a prefill fills whole blocks, and
-// the requests of a decode batch each find their workgroup, with no sorted order
-// to build first.  Two launches: the narrow product v = x A_l^T (its K split over
-// `splits` workgroups, each writing its own fp32 partial sums), then y + c_l v B_l^T.
+// rows of one adapter of one block: the requests of a decode batch each find their
+// workgroup.  Large batches are sorted by adapter first (lora_plan_kernel), so that
+// the blocks are of one adapter each.  Then two launches: the narrow product
+// v = x A_l^T (its K split over `splits` workgroups, each writing its own fp32 partial
+// sums), and y + c_l v B_l^T.
 // 8192 rows, 7168 -> 64 -> 4096, bf16: 32 us (22 at a copy's rate) and 44 (28).
 // ---------------------------------------------------------------------------
 struct LoraParams {
@@ -521,9 +522,10 @@ __device__ __forceinline__ void lora_groups(const LoraParams& p, bool bare, int*
 // The plan: rows sorted by adapter (stable, so that a row's group, and with it the order of its
 // sums, is the same every time), in items of at most 64 rows.  Without it every block of a
 // shuffled batch reads every adapter (1078 rows over 24 adapters, 5672 -> 72 -> 896: 143 us
-// without).  One workgroup; each of its 16 waves counts and places a run of rows, 64 at a
-// time: 7 us for 8192 rows in a trace, of which half are the launch and the ids' latency.  LDS: counts [16][bins], places [bins], item
-// places [bins], 512 ids per wave; bins = adapters + 1 (the last: none).
+// without, 36 with).  One workgroup; each of its 16 waves counts and places a run of rows, 64
+// at a time: in a trace 6.7 us for 2048 rows shuffled over 64 adapters, 8.1 for 8192 in
+// segments of 7, of which half are the launch and the ids' latency.  LDS: counts [16][bins],
+// places [bins], item places [bins], 512 ids per wave; bins = adapters + 1 (the last: none).
 constexpr int kPlanWaves = 16, kPlanBins = 1536, kPlanRows = 65536, kPlanFlight = 8;
 constexpr int lora_plan_lds(int bins) { return ((kPlanWaves + 2) * bins + kPlanWaves * kPlanFlight * 64) * 4; }
 static_assert(lora_plan_lds(kPlanBins) <= kSkMaxLds - 1024, "LDS budget");

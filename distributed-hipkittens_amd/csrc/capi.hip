@@ -707,12 +707,12 @@ int launch_router(const RouterParams& p, hipStream_t s) {
 }
 
 // Rows x rank up to which each row reads its own B (lora_expand_small_kernel), for ranks to 32 and
-// to 64.  Both launches, us, N = 4096, as a graph: rows shuffled over 64 adapters / in
-// segments of 4 or 8, small kernel against matrix instruction
-//   512 x 16    13.7 / 10.3,  62 / 11.3        2048 x 16  36 / 21,  180 / 16
-//   4096 x 16   84 / 34,     284 / 26
-//   128 x 64    21 / 17,      26 / 12          256 x 64   34 / 27,   45 / 14
-// The small kernel's loss on segments is bounded, the other's on shuffled rows is not.
+// to 64.  All launches, us, N = 4096, as a graph: rows shuffled over 64 adapters / in segments
+// of 4 or 8, small kernel against matrix instruction (sorted where lora_planned says so)
+//   H 1024:  128 x 64   21 / 18,  39 / 12      256 x 64   34 / 27,  40 / 15
+//            512 x 16   14 / 10,  34 / 12
+//   H 4096:  512 x 32   43 / 16,  40 / 13     1024 x 16   41 / 17,  42 / 18
+//           2048 x 16   69 / 24,  66 / 23
 constexpr int64_t kLoraSmallWork = 32768, kLoraSmallWork64 = 8192;
 // Rows x columns up to which a thread takes one column (both launches, rank 16, 64x4096: 9.2 us
 // with one, 9.6 with four; 512x4096: 17.1, 13.7).
@@ -760,14 +760,14 @@ bool lora_small(int64_t rows, int32_t rank) {
   return rank <= kLoraSmallRank && rows * rank <= (rank <= 32 ? kLoraSmallWork : kLoraSmallWork64);
 }
 
-// Whether the rows are sorted by adapter first (a launch, 4-7 us): from as many bytes of A as the row
+// Whether the rows are sorted by adapter first (a launch, 4-6 us): from as many bytes of A as the row
 // blocks could read, each adapter in each block, or as many groups of rows for the matrix
 // instruction.  us, unsorted / sorted, as a graph:
 //                                    shuffled    in segments
-//   8192 rows of 8, 7168->64->4096   274 / 94     68 / 75
-//   4096 rows of 8, 4096->16->4096    63 / 45     32 / 36
-//   2048 rows of 16, 4096->32->1024   53 / 28     18 / 19
-//   300 rows of 64, 2048->64->2048    85 / 39     27 / 25
+//   8192 rows of 8, 7168->64->4096   274 / 80     68 / 75
+//   4096 rows of 8, 4096->16->4096    63 / 38     32 / 36
+//   2048 rows of 16, 4096->32->1024   53 / 20     18 / 19
+//   300 rows of 64, 2048->64->2048    85 / 22     27 / 22
 constexpr int64_t kLoraPlanBytes = 32ll << 20, kLoraPlanGroups = 128;
 bool lora_planned(int64_t rows, int64_t x_stride, int32_t adapters, int64_t hidden, int32_t rank) {
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock, groups = blocks * std::min<int64_t>(adapters, kRowsBlock);
