@@ -306,6 +306,33 @@ def test_lora_sorted_first_same_bits(hk):
         assert torch.equal(hk.lora_add(*args), first)
 
 
+def test_lora_sorted_first_from_graphs(hk):
+    """Two graphs of one sorted batch on a stream of their own, replayed in turn with other ids
+    each time and eager calls between."""
+    rng = np.random.default_rng(12)
+    y, x, a, b, c = _lora_data(rng, 1500, 2048, 264, 64, 40, True)
+    ids = torch.zeros(1500, dtype=torch.int32, device="cuda")
+    args = [_dev(y, BF16), _dev(x, BF16), _dev(a, BF16), _dev(b, BF16), ids, torch.from_numpy(c).cuda()]
+    hk.lora_add(*args)
+    side = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = hk.lora_add(*args)
+        graphs.append((g, out))
+    for k, how in enumerate(["mixed", "none", "segments", "one", "out of range", "mixed"]):
+        ids.copy_(torch.from_numpy(_ids(rng, 1500, 40, how)))
+        eager = hk.lora_add(*args)
+        g, out = graphs[k % 2]
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager), how
+        assert torch.equal(hk.lora_add(*args), eager), how
+
+
 def test_lora_far_offsets(hk):
     """An adapter whose weights lie past 2^31 values, and far rows of strided x, y and out."""
     l, r, h, n = 140, 256, 65536, 512
