@@ -14,7 +14,6 @@ on the GPU:
 ``own`` chooses between the framework's calls and the plain forms below (the
 same formulas in elementary fp32 operations).
 """
-import functools
 import math
 import os
 import sys
@@ -221,9 +220,10 @@ def run(state):
     return _plain_lora(state)
 
 
-@functools.lru_cache(maxsize=None)
 def _framework():
-    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "distributed-hipkittens_amd"))
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "distributed-hipkittens_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
     import hkmoe
     return hkmoe
 
