@@ -125,4 +125,7 @@ class MoEBlock:
         """x [T, H] (what the previous sublayer added, or the stream itself) ->
         (bf16 layer output [T, H], the new residual stream)."""
         q, s, r, n = rms_norm_quant(x, self.norm_weight, residual, scales=self.scales, eps=self.eps, with_norm=True)
-        return self.layer(q, s, router_logits(n, self.router_weight), out=out), r
+        # a workspace per call, as in the calls before it: the layer's cached one would be shared by
+        # calls on several streams and by captured graphs
+        ws = q.new_empty((self.layer.workspace_size(q.shape[0]),), dtype=torch.uint8)
+        return self.layer(q, s, router_logits(n, self.router_weight), out=out, workspace=ws), r

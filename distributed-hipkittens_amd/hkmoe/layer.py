@@ -263,18 +263,24 @@ class MoELayer:
         self.block = w13_scale.dim() == 3
         self._ws = None
 
-    def workspace(self, num_tokens, device):
+    def workspace_size(self, num_tokens):
         mode = tk_kernel.SCALE_BLOCK if self.block else tk_kernel.SCALE_TENSOR
-        need = tk_kernel.moe_workspace_size(num_tokens, self.num_experts, self.top_k, self.hidden,
+        return tk_kernel.moe_workspace_size(num_tokens, self.num_experts, self.top_k, self.hidden,
                                             self.inter, mode)
+
+    def workspace(self, num_tokens, device):
+        need = self.workspace_size(num_tokens)
         if self._ws is None or self._ws.numel() < need:
             self._ws = torch.empty(need, dtype=torch.uint8, device=device)
         return self._ws
 
-    def __call__(self, x_q, x_scale, logits, out=None):
-        ws = self.workspace(x_q.shape[0], x_q.device)
+    def __call__(self, x_q, x_scale, logits, out=None, workspace=None):
+        """``workspace``: uint8, at least workspace_size(T) bytes, instead of the
+        cached one (calls that overlap in time need one each)."""
+        if workspace is None:
+            workspace = self.workspace(x_q.shape[0], x_q.device)
         return moe_forward(x_q, x_scale, logits, self.w13_q, self.w13_scale, self.w2_q,
-                           self.w2_scale, self.top_k, out=out, workspace=ws, packed=self.packed)
+                           self.w2_scale, self.top_k, out=out, workspace=workspace, packed=self.packed)
 
 
 # ----------------------------------------------------------------------------
@@ -365,17 +371,23 @@ class MoELayerMX:
         self.inter = two_i // 2
         self._ws = None
 
-    def workspace(self, num_tokens, device):
-        need = tk_kernel.moe_workspace_size(num_tokens, self.num_experts, self.top_k, self.hidden,
+    def workspace_size(self, num_tokens):
+        return tk_kernel.moe_workspace_size(num_tokens, self.num_experts, self.top_k, self.hidden,
                                             self.inter, tk_kernel.SCALE_MX)
+
+    def workspace(self, num_tokens, device):
+        need = self.workspace_size(num_tokens)
         if self._ws is None or self._ws.numel() < need:
             self._ws = torch.empty(need, dtype=torch.uint8, device=device)
         return self._ws
 
-    def __call__(self, x_q, x_e8m0, logits, out=None):
+    def __call__(self, x_q, x_e8m0, logits, out=None, workspace=None):
+        """``workspace`` as in :class:`MoELayer`."""
         t = x_q.shape[0]
         if out is None:
             out = x_q.new_empty((t, self.hidden), dtype=torch.bfloat16)
+        if workspace is None:
+            workspace = self.workspace(t, x_q.device)
         tk_kernel.dispatch_moe_mx(x_q, x_e8m0, logits, self.w13_q, self.w13_words, self.w2_q, self.w2_words,
-                                  self.top_k, out, self.workspace(t, x_q.device), packed=self.packed)
+                                  self.top_k, out, workspace, packed=self.packed)
         return out

@@ -556,3 +556,42 @@ def test_refusals_on_the_device(hk):
         with pytest.raises(RuntimeError):
             hk.lora_add(**args)
     hk.lora_add(**ok)
+
+
+@pytest.mark.parametrize("scales", ["group", "mx", "tensor"])
+def test_one_block_on_two_streams(hk, scales):
+    """Calls of one block that overlap in time, on inputs of their own."""
+    d = _weights(hk, 1, scales)
+    block = hk.MoEBlock(d["norm"], d["router"], d["layer"])
+    sets = [_inputs(s)[:2] for s in (10, 11)]
+    want = [[v.clone() for v in block(*s)] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(10):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(block(*sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for g in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[k]))
+
+
+def test_block_graph_beside_larger_calls(hk):
+    """A graph of the block replayed after eager calls of more tokens, which need a larger workspace."""
+    d = _weights(hk, 1, "group")
+    block = hk.MoEBlock(d["norm"], d["router"], d["layer"])
+    x, res, _ = _inputs(12)
+    want = [v.clone() for v in block(x, res)]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = block(x, res)
+    for k in (2, 5, 9):
+        big = block(x.repeat(k, 1), res.repeat(k, 1))
+        held = torch.zeros(1 << 22, device="cuda")  # takes whatever memory is free now
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        assert not held.any() and all(bool(v.isfinite().all()) for v in big)

@@ -184,3 +184,39 @@ refused(lambda: tk_kernel.dispatch_router_logits(T([4, 64], strides=(128, 1)), T
               "a: tensor must be contiguous", "ids: expected dtype torch.int32", "y: expected a torch.Tensor",
               "x: tensor must be contiguous"]
     assert [s.split(": ", 1)[1] for s in said] == wanted and "taken" not in out
+
+
+# ---------------------------------------------------------------------------
+# workspaces of the layers and of the block in front of them: CPU tensors, and
+# dispatches that only note what they were given
+# ---------------------------------------------------------------------------
+def _bare_layer(hkmoe, torch, mx):
+    f8, e, h, i = torch.float8_e4m3fn, 8, 256, 256
+    layer = object.__new__(hkmoe.MoELayerMX if mx else hkmoe.MoELayer)
+    layer.packed, layer.top_k, layer.num_experts, layer.hidden, layer.inter = True, 2, e, h, i
+    layer.block, layer._ws = True, None
+    layer.w13_q, layer.w2_q = torch.empty((e, 2 * i, h), dtype=f8), torch.empty((e, h, i), dtype=f8)
+    layer.w13_scale = layer.w2_scale = layer.w13_words = layer.w2_words = torch.empty(0)
+    return layer
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_block_calls_share_no_workspace(monkeypatch, mx):
+    """Two calls of one block may overlap in time, on two streams or in two graphs: each has a
+    workspace of its own, large enough, and neither is the layer's."""
+    import torch
+    hkmoe = pytest.importorskip("hkmoe")
+    tk, given = hkmoe.tk_kernel, []
+    monkeypatch.setattr("hkmoe.layer._check_dev", lambda *ts: None)
+    monkeypatch.setattr(tk, "dispatch_rms_norm_quant", lambda *a, **k: None)
+    monkeypatch.setattr(tk, "dispatch_router_logits", lambda *a, **k: None)
+    monkeypatch.setattr(tk, "dispatch_moe_mx" if mx else "dispatch_moe", lambda *a, **k: given.append(a[9]))
+    layer = _bare_layer(hkmoe, torch, mx)
+    block = hkmoe.MoEBlock(torch.ones(256), torch.zeros((8, 256), dtype=torch.bfloat16), layer)
+    x = torch.zeros((5, 256), dtype=torch.bfloat16)
+    for _ in range(2):
+        out, r = block(x)
+        assert out.shape == (5, 256) and r is x
+    need = tk.moe_workspace_size(5, 8, 2, 256, 256, tk.SCALE_MX if mx else tk.SCALE_BLOCK)
+    assert len(given) == 2 and all(w.dtype == torch.uint8 and w.numel() >= need for w in given)
+    assert given[0].data_ptr() != given[1].data_ptr() and all(w is not layer._ws for w in given)
