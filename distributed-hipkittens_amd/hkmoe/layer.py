@@ -241,7 +241,25 @@ def _steps_narrow(r, x_q, x_scale, logits, w13_q, w13_scale, w2_q, w2_scale, top
     return r
 
 
-class MoELayer:
+class _Workspace:
+    """The layers' cached workspace: grows with the largest call so far.  A captured graph keeps
+    writing to the one it saw, so that one is held for good when a larger one takes its place."""
+
+    _ws = None
+    _captured = False
+    _held = ()
+
+    def workspace(self, num_tokens, device):
+        need = self.workspace_size(num_tokens)
+        if self._ws is None or self._ws.numel() < need:
+            if self._captured:
+                self._held += (self._ws,)
+            self._ws, self._captured = torch.empty(need, dtype=torch.uint8, device=device), False
+        self._captured = self._captured or torch.cuda.is_current_stream_capturing()
+        return self._ws
+
+
+class MoELayer(_Workspace):
     """FP8 MoE FFN layer: e4m3 expert weights with per-tensor ([E]) or
     128x128 block scales; runs hkmoe_moe_forward with a cached workspace.
     With ``pack`` (default) the weights are repacked once, here, into the
@@ -261,18 +279,11 @@ class MoELayer:
         self.num_experts, two_i, self.hidden = w13_q.shape
         self.inter = two_i // 2
         self.block = w13_scale.dim() == 3
-        self._ws = None
 
     def workspace_size(self, num_tokens):
         mode = tk_kernel.SCALE_BLOCK if self.block else tk_kernel.SCALE_TENSOR
         return tk_kernel.moe_workspace_size(num_tokens, self.num_experts, self.top_k, self.hidden,
                                             self.inter, mode)
-
-    def workspace(self, num_tokens, device):
-        need = self.workspace_size(num_tokens)
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = torch.empty(need, dtype=torch.uint8, device=device)
-        return self._ws
 
     def __call__(self, x_q, x_scale, logits, out=None, workspace=None):
         """``workspace``: uint8, at least workspace_size(T) bytes, instead of the
@@ -347,7 +358,7 @@ def moe_forward_mx_steps(x_q, x_e8m0, logits, w13_q, w13_words, w2_q, w2_words, 
     return r
 
 
-class MoELayerMX:
+class MoELayerMX(_Workspace):
     """MX FP8 MoE FFN layer: e4m3 expert weights with 1x32 e8m0 exponents
     (uint8 [E, 2I, H/32] and [E, H, I/32]); activations come with their e8m0
     exponents [T, H/32] (see :func:`quant_mx`).  Weights and their exponents
@@ -369,17 +380,10 @@ class MoELayerMX:
         self.top_k = int(top_k)
         self.num_experts, two_i, self.hidden = w13_q.shape
         self.inter = two_i // 2
-        self._ws = None
 
     def workspace_size(self, num_tokens):
         return tk_kernel.moe_workspace_size(num_tokens, self.num_experts, self.top_k, self.hidden,
                                             self.inter, tk_kernel.SCALE_MX)
-
-    def workspace(self, num_tokens, device):
-        need = self.workspace_size(num_tokens)
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = torch.empty(need, dtype=torch.uint8, device=device)
-        return self._ws
 
     def __call__(self, x_q, x_e8m0, logits, out=None, workspace=None):
         """``workspace`` as in :class:`MoELayer`."""

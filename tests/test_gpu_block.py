@@ -595,3 +595,29 @@ def test_block_graph_beside_larger_calls(hk):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
         assert not held.any() and all(bool(v.isfinite().all()) for v in big)
+
+
+@pytest.mark.parametrize("scales", ["group", "mx"])
+def test_layer_graph_beside_larger_calls(hk, scales):
+    """The same for a layer called by itself, whose workspace is cached."""
+    layer = _weights(hk, 1, scales)["layer"]
+    quant = hk.quant_mx if scales == "mx" else hk.quant_group
+    g = torch.Generator(device="cuda").manual_seed(13)
+    x_q, x_s = quant(torch.randn((T, H), generator=g, device="cuda"))
+    logits = torch.randn((T, E), generator=g, device="cuda")
+    want = layer(x_q, x_s, logits).clone()
+    out = torch.empty_like(want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(x_q, x_s, logits, out=out)
+    seen = layer._ws
+    size = seen.numel()
+    del seen
+    for k in (2, 5, 9):
+        big = layer(*(v.view(torch.uint8).repeat(k, 1).view(v.dtype) for v in (x_q, x_s, logits)))
+        held = torch.zeros(size, dtype=torch.uint8, device="cuda")  # would take the first workspace's place
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(big[:T], big[-T:]) and not held.any(), k

@@ -220,3 +220,27 @@ def test_block_calls_share_no_workspace(monkeypatch, mx):
     need = tk.moe_workspace_size(5, 8, 2, 256, 256, tk.SCALE_MX if mx else tk.SCALE_BLOCK)
     assert len(given) == 2 and all(w.dtype == torch.uint8 and w.numel() >= need for w in given)
     assert given[0].data_ptr() != given[1].data_ptr() and all(w is not layer._ws for w in given)
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_layer_keeps_the_workspace_of_a_captured_graph(monkeypatch, mx):
+    """A layer's workspace that a capture has used outlives a larger one: the graph writes to it
+    whenever it is replayed.  One that only eager calls used does not."""
+    import weakref
+
+    import torch
+    hkmoe = pytest.importorskip("hkmoe")
+    layer, capturing = _bare_layer(hkmoe, torch, mx), []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(capturing))
+    eager = weakref.ref(layer.workspace(4, "cpu"))
+    layer.workspace(40, "cpu")
+    assert eager() is None
+    capturing.append(1)
+    held = weakref.ref(layer.workspace(4, "cpu"))  # a graph over fewer tokens: the same workspace
+    assert held() is layer._ws
+    capturing.clear()
+    layer.workspace(400, "cpu")
+    assert held() is not None and held() is not layer._ws
+    later = weakref.ref(layer._ws)
+    layer.workspace(4000, "cpu")
+    assert later() is None and held() is not None
