@@ -33,7 +33,7 @@ struct NormParams {
   void* residual_out;    // null without a residual
   uint16_t* norm_out;    // bf16, may be null
   uint8_t* q;
-  void* s;            // group: fp32, mx: e8m0, static: fp32 [1] (written if s != scale), amax: unused
+  void* s;            // group: fp32, mx: e8m0; static: unused; amax: fp32 [1], the second launch's
   const float* scale;  // static
   float* rstd;         // amax: [rows]
   float* amax;         // amax: one per workgroup
@@ -202,7 +202,11 @@ __global__ __launch_bounds__(kNormMaxThreads) void rms_norm_quant_kernel(NormPar
           if ((threadIdx.x & 3) == 0) static_cast<uint8_t*>(p.s)[(base + j) / 32] = static_cast<uint8_t>(e);
         }
       } else if constexpr (SC == NormScale::kStatic) {
-        const float sc = *p.scale;
+        // 448 sc may be past fp32: there n and sc are taken 2^-24 as large (what that loses of n is far
+        // below the smallest e4m3 value), so that an infinite n is cut as any other
+        const float by = *p.scale > 0x1p100f ? 0x1p-24f : 1.0f, sc = *p.scale * by;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n.v[i] *= by;
         if (live) *reinterpret_cast<uint2*>(p.q + base + j) = quant8<true>(n, sc, quot_scale(sc));
       } else {
         amax = fmaxf(amax, m);

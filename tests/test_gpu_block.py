@@ -621,3 +621,26 @@ def test_layer_graph_beside_larger_calls(hk, scales):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(big[:T], big[-T:]) and not held.any(), k
+
+
+# ---------------------------------------------------------------------------
+# norm: scales and epsilons at the ends of their range
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("given", [1e-44, 2e-38, 1e30, 1e36, 3e38])
+def test_norm_given_scale_at_the_ends(hk, given):
+    """Subnormal scales, and scales of which 448 is past fp32: values past 448 scale saturate, an
+    infinite one too."""
+    rng = np.random.default_rng(17)
+    x = rng.standard_normal((6, 520)).astype(np.float32)
+    x[2:4] = 0
+    x[2, 3], x[3, 3] = -5, 5  # n = -sqrt(520) w and sqrt(520) w there
+    w = (rng.standard_normal(520).astype(np.float32) * np.float32(30 * min(given, 1e36))).astype(np.float32)
+    w[3] = np.float32(min(3e37, 100 * given))
+    with np.errstate(all="ignore"):
+        _, n = block_ref.rms_norm(x, None, w, 1e-6, False)
+        q_ref, _ = block_ref.quantise(n, "tensor", given)
+    assert given < 1e36 or np.isinf(n[2, 3])
+    assert q_ref[2, 3] == 0xFE and q_ref[3, 3] == 0x7E
+    q = hk.rms_norm_quant(_dev(x, F32), _dev(w, F32), scales="tensor", scale=torch.tensor([given], device="cuda"))[0]
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(f8_np(q), q_ref)
