@@ -1,7 +1,7 @@
 // Residual addition, root-mean-square norm and e4m3 quantisation in one pass.
 //
 //   r = rnd(x + residual)                (kept in x's type: the new residual stream)
-//   m = mean_j r_j^2,  rstd = fl32(1 / sqrt(m + eps))
+//   m = mean_j r_j^2,  rstd = fl32(1 / sqrt(m + eps)), at most the largest fp32 value
 //   n_j = fl32(fl32(r_j rstd) w_j)       (q, and rnd(n) as bf16 where asked for)
 //
 // and n quantised as quant_group_kernel, quant_mx_kernel and quant_tensor_kernel
@@ -165,7 +165,9 @@ __global__ __launch_bounds__(kNormMaxThreads) void rms_norm_quant_kernel(NormPar
       }
     }
     sum = group_sum(sum, red[turn]);
-    const float rstd = static_cast<float>(1.0 / sqrt(sum / static_cast<double>(cols) + p.eps));
+    // past fp32 (rows of zeros with eps below 2^-256) the largest one, so that zeros stay zeros
+    const float inv = static_cast<float>(1.0 / sqrt(sum / static_cast<double>(cols) + p.eps)), most = 0x1.fffffep127f;
+    const float rstd = inv > most ? most : inv;
     if constexpr (SC == NormScale::kAmax) {
       if (threadIdx.x == 0) p.rstd[row] = rstd;
     }

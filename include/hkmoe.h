@@ -411,7 +411,8 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
  *
  * hkmoe_rms_norm_quant: the residual's addition, the norm and the e4m3 operand.
  *     r = x + residual, rounded to x's type (written to residual_out)
- *     rstd = fl32(1 / sqrt(mean_j r_j^2 + eps)), mean and root in 64 bits
+ *     rstd = fl32(1 / sqrt(mean_j r_j^2 + eps)), mean and root in 64 bits; finite:
+ *            at most the largest fp32 value
  *     n_j = fl32(fl32(r_j * rstd) * weight_j)
  *   x, residual, residual_out [R, C] bf16 or fp32 (x_dtype; residual and
  *   residual_out both NULL: r = x; residual_out may be x or residual itself),

@@ -644,3 +644,22 @@ def test_norm_given_scale_at_the_ends(hk, given):
     q = hk.rms_norm_quant(_dev(x, F32), _dev(w, F32), scales="tensor", scale=torch.tensor([given], device="cuda"))[0]
     torch.cuda.synchronize()
     np.testing.assert_array_equal(f8_np(q), q_ref)
+
+
+@pytest.mark.parametrize("scales", ["group", "mx", "tensor", "given"])
+@pytest.mark.parametrize("eps", [1e-80, 1e-300])
+def test_norm_rows_of_zeros_tiny_eps(hk, scales, eps):
+    """1 / sqrt(eps) past fp32: rows of zeros stay zeros, the others do not notice."""
+    rng = np.random.default_rng(18)
+    x = rng.standard_normal((5, 256)).astype(np.float32)
+    x[1] = x[4] = 0
+    w = np.ones(256, np.float32)
+    _, n_ref = block_ref.rms_norm(x, None, w, 1e-30, False)  # far below the other rows' last bit
+    given = 0.01 if scales == "given" else None
+    q_ref, s_ref = block_ref.quantise(n_ref, "tensor" if given else scales, given)
+    q, s, _, n = hk.rms_norm_quant(_dev(x, F32), _dev(w, F32), scales="tensor" if given else scales, eps=eps, with_norm=True,
+                                   scale=torch.tensor([given], device="cuda") if given else None)
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(bf16_np(n), _bf16(n_ref))
+    np.testing.assert_array_equal(f8_np(q), q_ref)
+    np.testing.assert_array_equal(s.cpu().numpy(), s_ref)
