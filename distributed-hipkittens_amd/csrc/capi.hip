@@ -707,13 +707,24 @@ int launch_router(const RouterParams& p, hipStream_t s) {
 }
 
 // Rows x rank up to which each row reads its own B (lora_expand_small_kernel), for ranks to 32 and
-// to 64.  All launches, us, N = 4096, as a graph: rows shuffled over 64 adapters / in segments
-// of 4 or 8, small kernel against matrix instruction (sorted where lora_planned says so)
-//   H 1024:  128 x 64   21 / 18,  39 / 12      256 x 64   34 / 27,  40 / 15
-//            512 x 16   14 / 10,  34 / 12
-//   H 4096:  512 x 32   43 / 16,  40 / 13     1024 x 16   41 / 17,  42 / 18
-//           2048 x 16   69 / 24,  66 / 23
-constexpr int64_t kLoraSmallWork = 32768, kLoraSmallWork64 = 8192;
+// to 64, and rows x rank^2 x N below which it does: a column costs its thread the more the fewer of
+// them it has for a rank.  All launches as a graph, us, rows shuffled over 64 adapters / over 8 /
+// in segments of 8: small kernel against matrix instruction (sorted where lora_planned says
+// so), with * the one that is taken
+//   H 4096, N 4096:  512 x 16  *20.9 / 13.0 / 11.3    22.8 / 20.9 / 14.6
+//                   1024 x 16  *25.6 / 20.7 / 16.6    25.4 / 20.8 / 19.7
+//                   2048 x 16   34.9 / 32.4 / 23.3   *31.1 / 26.3 / 23.7
+//                   256 x 32   *24.0 / 15.1 / 13.1    24.0 / 15.8 / 12.7
+//                   512 x 32    30.5 / 21.9 / 18.3   *25.9 / 23.3 / 15.1
+//                   64 x 64    *18.5 / 15.2 / 16.1    21.7 / 14.2 / 13.9
+//                   128 x 64    31.1 / 21.6 / 20.9   *30.3 / 15.4 / 13.7
+//   H 4096, N 1024: 2048 x 16  *22.7 / 22.5 / 13.7    23.2 / 21.5 / 19.6
+//                   4096 x 16   31.0 / 27.7 / 25.4   *30.3 / 27.3 / 24.6
+//                   128 x 64   *22.0 / 11.7 / 11.2    23.7 / 14.2 / 13.0
+//                   256 x 64    25.3 / 16.3 / 14.1   *24.2 / 16.5 / 13.5
+//   H 2048, N 8192:  700 x 16  *30.5 / 18.8 / 17.5    28.6 / 36.2 / 19.9
+//                   2048 x 16   48.4 / 39.4 / 35.1   *38.9 / 32.5 / 27.2
+constexpr int64_t kLoraSmallWork = 32768, kLoraSmallWork64 = 8192, kLoraSmallColumns = 1ll << 31;
 // Rows x columns up to which a thread takes one column (both launches, rank 16, 64x4096: 9.2 us
 // with one, 9.6 with four; 512x4096: 17.1, 13.7).
 constexpr int64_t kLoraNarrow = 1 << 18;
@@ -754,10 +765,10 @@ size_t lora_partials(int64_t rows, int64_t hidden, int32_t rank) {
   return align256(static_cast<size_t>(lora_splits(rows, hidden)) * rows * rank * sizeof(float));
 }
 
-// Whether each row takes its own workgroup in the second launch (lora_expand_small_kernel): up to
-// these rows x rank, for ranks to 32 and to 64.
-bool lora_small(int64_t rows, int32_t rank) {
-  return rank <= kLoraSmallRank && rows * rank <= (rank <= 32 ? kLoraSmallWork : kLoraSmallWork64);
+// Whether each row takes its own workgroup in the second launch (lora_expand_small_kernel).
+bool lora_small(int64_t rows, int32_t rank, int64_t n) {
+  return rank <= kLoraSmallRank && rows * rank <= (rank <= 32 ? kLoraSmallWork : kLoraSmallWork64) &&
+         rows * rank * rank * n < kLoraSmallColumns;
 }
 
 // Whether the rows are sorted by adapter first (a launch, 4-6 us): from as many bytes of A as the row
@@ -769,10 +780,10 @@ bool lora_small(int64_t rows, int32_t rank) {
 //   2048 rows of 16, 4096->32->1024   53 / 20     18 / 19
 //   300 rows of 64, 2048->64->2048    85 / 22     27 / 22
 constexpr int64_t kLoraPlanBytes = 32ll << 20, kLoraPlanGroups = 128;
-bool lora_planned(int64_t rows, int64_t x_stride, int32_t adapters, int64_t hidden, int32_t rank) {
+bool lora_planned(int64_t rows, int64_t x_stride, int32_t adapters, int64_t hidden, int64_t n, int32_t rank) {
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock, groups = blocks * std::min<int64_t>(adapters, kRowsBlock);
   return blocks > 1 && rows <= kPlanRows && adapters < kPlanBins && 2 * rows * x_stride < (1ll << 32) - (1 << 22) &&
-         (groups * rank * hidden * 2 > kLoraPlanBytes || (groups >= kLoraPlanGroups && !lora_small(rows, rank)));
+         (groups * rank * hidden * 2 > kLoraPlanBytes || (groups >= kLoraPlanGroups && !lora_small(rows, rank, n)));
 }
 
 }  // namespace
@@ -1712,7 +1723,7 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
   p.splits = lora_splits(rows, hidden);
   auto s = static_cast<hipStream_t>(stream);
   const int64_t blocks = (rows + kRowsBlock - 1) / kRowsBlock;
-  const bool planned = lora_planned(rows, x_stride, adapters, hidden, rank);
+  const bool planned = lora_planned(rows, x_stride, adapters, hidden, n, rank);
   const int64_t places = planned ? lora_plan_items(rows, adapters) : blocks;
   const unsigned grid_x = static_cast<unsigned>(!planned && blocks <= 8 ? blocks : (places + 7) / 8 * 8);
   if (planned) {
@@ -1734,7 +1745,7 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
   hipLaunchKernelGGL((rank <= 16 ? lora_shrink_kernel<1> : rank <= 32 ? lora_shrink_kernel<2> : lora_shrink_kernel<4>),
                      dim3(grid_x, parts(p.splits), p.splits), dim3(kLoraWaves * 64), 0, s, p);
   HK_TRY(check_launch("lora_shrink_kernel"));
-  if (lora_small(rows, rank)) {
+  if (lora_small(rows, rank, n)) {
     const bool f32 = y_dtype == HKMOE_F32;
     if (rank > 32 || rows * n <= kLoraNarrow) return f32 ? launch_lora_small<true, 1>(p, s) : launch_lora_small<false, 1>(p, s);
     if (rank > 16) return f32 ? launch_lora_small<true, 2>(p, s) : launch_lora_small<false, 2>(p, s);

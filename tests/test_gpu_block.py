@@ -663,3 +663,11 @@ def test_norm_rows_of_zeros_tiny_eps(hk, scales, eps):
     np.testing.assert_array_equal(bf16_np(n), _bf16(n_ref))
     np.testing.assert_array_equal(f8_np(q), q_ref)
     np.testing.assert_array_equal(s.cpu().numpy(), s_ref)
+
+
+@pytest.mark.parametrize("t,r,n", [(1023, 16, 8192), (1024, 16, 8192), (127, 64, 4096), (128, 64, 4096), (511, 32, 4096), (512, 32, 4096)])
+@pytest.mark.parametrize("how", ["mixed", "segments"])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_lora_rows_at_the_small_kernels_end(hk, t, r, n, how, bf16):
+    """The last shapes in which a row reads its own B, and the first after them."""
+    _lora_case(hk, t, 72, n, r, 9, how, bf16=bf16, in_place=bf16)

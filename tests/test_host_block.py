@@ -244,3 +244,17 @@ def test_layer_keeps_the_workspace_of_a_captured_graph(monkeypatch, mx):
     later = weakref.ref(layer._ws)
     layer.workspace(4000, "cpu")
     assert later() is None and held() is not None
+
+
+def test_adapters_of_many_columns_take_the_matrix_instruction(fake):
+    """The shapes on which a row's own workgroup was measured slower in each order of the rows."""
+    out = hip_host.run(fake, """
+        lib.hkmoe_lora_workspace_size.restype = ctypes.c_size_t
+        for rows, h, r, n in ((2048, 4096, 16, 4096), (512, 4096, 32, 4096), (2048, 2048, 16, 8192), (1024, 4096, 24, 4096),
+                              (1024, 4096, 16, 4096), (256, 4096, 32, 4096), (2048, 4096, 16, 1024), (200, 4096, 40, 4096)):
+            assert lib.hkmoe_lora_add(P, i64(n), P, i64(h), P, P, P, None, i64(rows), i32(64), i64(h), i64(n), i32(r), 0, P, i64(n),
+                                      P, ctypes.c_size_t(1 << 40), None) == 0
+        for line in log(): print(line)
+    """)
+    second = [l for l in out if l.startswith("launch") and "lora_expand" in l]
+    assert len(second) == 8 and ["small" in l for l in second] == [False] * 4 + [True] * 4, second
