@@ -51,3 +51,38 @@ def lora_bound(out, mag, hidden, rank, bf16):
     half = 2.0 ** -8 if bf16 else 2.0 ** -24
     inner = (hidden + rank + 32) * 2.0 ** -24 + (2.0 ** -17 if bf16 else 2.0 ** -25)
     return half * np.abs(out) + (1 + half) * inner * mag + 32 * 2.0 ** -24 * np.abs(out)
+
+
+def lora_exact_inputs(rng, t, h, n, r, adapters, bf16):
+    """(x, a, b, c, v) of whole numbers and powers of two such that every product and every partial
+    sum, in whatever order, is exact in fp32, and v = x A^T (the same for every adapter up to
+    its signs) needs 24 bits: three bytes, each a value of x, at three places of K far from each other.
+    fp32 output: a column is c v_r alone, with c B a power of two.  bf16 output (v of 16
+    bits): a column is v_r - v_r', small, so that only v's first term would leave nothing or too much."""
+    places = np.array([h // 9, h // 2, h - 1])
+    x, a, b = np.zeros((t, h), np.float32), np.zeros((adapters, r, h), np.float32), np.zeros((adapters, n, r), np.float32)
+    top = rng.integers(64, 128, t) if not bf16 else np.zeros(t, np.int64)
+    x[:, places] = np.stack([top, rng.integers(128, 256, t), 2 * rng.integers(0, 128, t) + 1], 1)
+    x *= rng.choice([-1.0, 1.0], (t, 1)).astype(np.float32)
+    a[:, :, places] = [65536.0, 256.0, 1.0]
+    c = (2.0 ** rng.integers(-3, 4, adapters)).astype(np.float32)
+    col = np.arange(n)
+    if bf16:
+        # ranks differ by small multiples of x's last byte: v_r = 256 x1 + (1 + r % 2) x0
+        a[:, 1::2, places[2]] = 2.0
+        b[:, col, 2 * (col % (r // 2))] = -1.0
+        b[:, col, 2 * (col % (r // 2)) + 1] = 1.0  # their difference: x0, at most 255
+    else:
+        a *= rng.choice([-1.0, 1.0], (adapters, r, 1)).astype(np.float32)
+        b[:, col, col % r] = 2.0 ** rng.integers(-4, 5, (adapters, n))
+    v = np.einsum("th,arh->atr", x.astype(np.float64), a.astype(np.float64))
+    return x, a, b, c, v
+
+
+def split_terms(v, terms):
+    """v as a sum of `terms` bf16 values, each the rounding of what those before it leave."""
+    left, out = np.asarray(v, np.float32).copy(), np.zeros(np.shape(v))
+    for _ in range(terms):
+        t = fp8.bf16_round(left)
+        out, left = out + t, left - t
+    return out

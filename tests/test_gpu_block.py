@@ -671,3 +671,30 @@ def test_norm_rows_of_zeros_tiny_eps(hk, scales, eps):
 def test_lora_rows_at_the_small_kernels_end(hk, t, r, n, how, bf16):
     """The last shapes in which a row reads its own B, and the first after them."""
     _lora_case(hk, t, 72, n, r, 9, how, bf16=bf16, in_place=bf16)
+
+
+# ---------------------------------------------------------------------------
+# adapters: v's terms, held to equality
+# ---------------------------------------------------------------------------
+def _exact_lora(hk, t, h, n, r, adapters, how, bf16):
+    rng = np.random.default_rng(t + h + r)
+    x, a, b, c, v = block_ref.lora_exact_inputs(rng, t, h, n, r, adapters, bf16)
+    ids = _ids(rng, t, adapters, how)
+    y = np.zeros((t, n), np.float32)
+    ref = block_ref.lora(y, x, a, b, ids, c)[0]
+    out = hk.lora_add(_dev(y, BF16 if bf16 else F32), _dev(x, BF16), _dev(a, BF16), _dev(b, BF16), torch.from_numpy(ids).cuda(),
+                      torch.from_numpy(c).cuda())
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(bf16_np(out).astype(np.float64), ref)
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("how", ["one", "mixed", "segments"])
+@pytest.mark.parametrize("t,adapters,r,h", [(40, 2, 72, 4096), (40, 12, 72, 4096), (20, 3, 256, 264), (300, 4, 64, 1024),
+                                            (1100, 6, 32, 2048), (1000, 20, 72, 1032), (2500, 40, 16, 1048), (150, 3, 200, 8200),
+                                            (33, 5, 16, 4096)])
+def test_lora_exact_terms(hk, t, adapters, r, h, how, bf16):
+    """Whole numbers whose every product and sum is exact, with a v that needs all of its terms: the
+    matrix instruction's two (three for an fp32 output), split and unsplit sums, few and many rows
+    of an adapter, sorted or not, and the small kernel's plain products."""
+    _exact_lora(hk, t, h, 136, r, adapters, how, bf16)

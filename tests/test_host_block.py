@@ -258,3 +258,29 @@ def test_adapters_of_many_columns_take_the_matrix_instruction(fake):
     """)
     second = [l for l in out if l.startswith("launch") and "lora_expand" in l]
     assert len(second) == 8 and ["small" in l for l in second] == [False] * 4 + [True] * 4, second
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+def test_exact_adapter_inputs_need_every_term(bf16):
+    """The inputs of the adapters' equality test: every sum exact in fp32, and one bf16 term of v less
+    (the mistake planted here) moves most outputs."""
+    import numpy as np
+
+    import block_ref
+    rng = np.random.default_rng(0)
+    x, a, b, c, v = block_ref.lora_exact_inputs(rng, 50, 264, 136, 40, 3, bf16)
+    for part in (x, a, b):
+        assert (block_ref.fp8.bf16_round(part) == part).all()
+    assert np.abs(v).max() < 1 << 24  # so is every partial sum: x's terms of a row have one sign, A's of a rank too
+    terms = 2 if bf16 else 3
+    ids = np.arange(50) % 3
+    mine = v[ids, np.arange(50)]
+    assert (block_ref.split_terms(mine, terms) == mine).all()
+    ref, _ = block_ref.lora(np.zeros((50, 136), np.float32), x, a, b, ids, c)
+    if bf16:
+        assert (block_ref.fp8.bf16_round(ref.astype(np.float32)) == ref).all()
+    else:
+        assert (ref.astype(np.float32) == ref).all()
+    for k in range(1, terms + 1):
+        lost = c[ids][:, None] * np.einsum("tr,tnr->tn", block_ref.split_terms(mine, k), b.astype(np.float64)[ids])
+        assert (lost == ref).all() if k == terms else (lost != ref).mean() > 0.8
