@@ -1751,7 +1751,7 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
     if (rank > 16) return f32 ? launch_lora_small<true, 2>(p, s) : launch_lora_small<false, 2>(p, s);
     return f32 ? launch_lora_small<true, 4>(p, s) : launch_lora_small<false, 4>(p, s);
   }
-  const int64_t strips = (n + 255) / 256, cols = std::min<int64_t>({strips, 65535, std::max<int64_t>(1, 512 / blocks)});
+  const int64_t strips = (n + 255) / 256, cols = std::min(strips, std::max<int64_t>(1, 512 / blocks));
   p.cols_per_wg = static_cast<int32_t>((strips + cols - 1) / cols * 256);
   const dim3 grid(grid_x, parts(cols), static_cast<unsigned>((n + p.cols_per_wg - 1) / p.cols_per_wg));
   const bool nt = rows * n * (y_dtype == HKMOE_F32 ? 4 : 2) > kLoraCached;

@@ -2,8 +2,8 @@
 // GPU: built as libamdhip64.so.7 and found before the real one through
 // LD_LIBRARY_PATH, it defines every runtime function that libhkmoe.so imports.
 // Nothing runs; each call that matters for ordering is appended to a log that
-// the test reads (fake_hip_log): kernel launches with their demangled name, grid
-// and stream, events, streams.
+// the test reads (fake_hip_log): kernel launches with their demangled name, grid,
+// threads and stream, events, streams.
 #include <cxxabi.h>
 
 #include <chrono>
@@ -46,10 +46,12 @@ bool fails(const char* fn) {
   return true;
 }
 std::string id(const void* p) { return std::to_string(reinterpret_cast<intptr_t>(p)); }
-int launch(const void* f, Dim3 grid, void** args, void* stream) {
+int launch(const void* f, Dim3 grid, Dim3 block, void** args, void* stream) {
+  const uint32_t threads = block.x * block.y * block.z;
   std::lock_guard<std::mutex> g(mu);
   const std::string& name = kernels[f];
-  say("launch " + name + " grid=" + std::to_string(grid.x) + " stream=" + id(stream));
+  say("launch " + name + " grid=" + std::to_string(grid.x) + " y=" + std::to_string(grid.y) + " z=" + std::to_string(grid.z) +
+      " threads=" + std::to_string(threads) + " stream=" + id(stream));
   if (watch_arg >= 0 && name.find(watch_name) != std::string::npos)
     say("arg " + std::to_string(*static_cast<int32_t*>(args[watch_arg])));
   return 0;
@@ -132,11 +134,11 @@ int __hipPopCallConfiguration(Dim3* grid, Dim3* block, size_t* lds, void** strea
   *stream = c.stream;
   return 0;
 }
-int hipLaunchKernel(const void* f, Dim3 grid, Dim3, void** args, size_t, void* stream) {
-  return launch(f, grid, args, stream);
+int hipLaunchKernel(const void* f, Dim3 grid, Dim3 block, void** args, size_t, void* stream) {
+  return launch(f, grid, block, args, stream);
 }
-int hipExtLaunchKernel(const void* f, Dim3 grid, Dim3, void** args, size_t, void* stream, void*, void*, int) {
-  return launch(f, grid, args, stream);
+int hipExtLaunchKernel(const void* f, Dim3 grid, Dim3 block, void** args, size_t, void* stream, void*, void*, int) {
+  return launch(f, grid, block, args, stream);
 }
 int hipGetDevice(int* d) { return *d = 0; }
 int hipDeviceGetAttribute(int* v, int, int) {  // only asked for the CU count

@@ -284,3 +284,31 @@ def test_exact_adapter_inputs_need_every_term(bf16):
     for k in range(1, terms + 1):
         lost = c[ids][:, None] * np.einsum("tr,tnr->tn", block_ref.split_terms(mine, k), b.astype(np.float64)[ids])
         assert (lost == ref).all() if k == terms else (lost != ref).mean() > 0.8
+
+
+def test_every_grid_dimension_in_range(fake):
+    """The largest sizes that are taken: x below 2^32 work-items, y and z at most 65535."""
+    out = hip_host.run(fake, """
+        size, dbl = ctypes.c_size_t, ctypes.c_double
+        for rows in (1, 63, 64, 65, 2048, 4096, 65536, 65537, 1 << 24):
+            for cols in (8, 65536):
+                for mode in (0, 1, 2):
+                    if mode and cols == 8: continue
+                    assert lib.hkmoe_rms_norm_quant(P, None, P, i64(rows), i64(cols), 0, 0, dbl(1e-6), mode, None, P, P, None,
+                                                    None, P, size(1 << 50), None) == 0
+            for e in (1, 1024):
+                for h in (8, 1 << 20):
+                    assert lib.hkmoe_router_logits(P, P, i64(rows), i32(e), i64(h), P, None) == 0
+            for n in (8, 1 << 23):
+                for h, r, adapters in ((8, 8, 1), (1 << 20, 8, 1535), (4096, 16, 1 << 20), (4096, 40, 64), (1 << 20, 256, 64)):
+                    for yt in (0, 1):
+                        assert lib.hkmoe_lora_add(P, i64(n), P, i64(h), P, P, P, None, i64(rows), i32(adapters), i64(h), i64(n),
+                                                  i32(r), yt, P, i64(n), P, size(1 << 50), None) == 0
+        for line in log(): print(line)
+    """)
+    launches = [l for l in out if l.startswith("launch")]
+    assert len({l.split()[1] for l in launches}) > 15
+    for l in launches:
+        v = {k: int(n) for k, n in (f.split("=") for f in l.split()[2:])}
+        assert 1 <= v["grid"] and v["grid"] * v["threads"] < 1 << 32 and 1 <= v["y"] <= 65535 and 1 <= v["z"] <= 65535, l
+        assert v["threads"] <= 1024, l
