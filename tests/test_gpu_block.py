@@ -698,3 +698,33 @@ def test_lora_exact_terms(hk, t, adapters, r, h, how, bf16):
     matrix instruction's two (three for an fp32 output), split and unsplit sums, few and many rows
     of an adapter, sorted or not, and the small kernel's plain products."""
     _exact_lora(hk, t, h, 136, r, adapters, how, bf16)
+
+
+# ---------------------------------------------------------------------------
+# more rows than one pass of the grid, or than are sorted
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("scales", ["group", "mx", "tensor"])
+def test_norm_more_rows_than_workgroups(hk, scales):
+    rows, cols = (1 << 20) + 70, 128
+    g = torch.Generator(device="cuda").manual_seed(19)
+    x, res = (torch.randn((rows, cols), generator=g, device="cuda").to(BF16) for _ in range(2))
+    w = torch.rand(cols, generator=g, device="cuda")
+    scale = torch.full((1,), 0.01, device="cuda") if scales == "tensor" else None  # given: independent of the other rows
+    q, s, r, n = hk.rms_norm_quant(x, w, res, scales=scales, scale=scale, with_norm=True)
+    for part in (slice(0, 200), slice((1 << 20) - 60, rows)):
+        q1, s1, r1, n1 = hk.rms_norm_quant(x[part], w, res[part], scales=scales, scale=scale, with_norm=True)
+        assert torch.equal(q[part].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(n[part], n1)
+        assert torch.equal(r[part], r1) and (scale is not None or torch.equal(s[part], s1))
+
+
+@pytest.mark.parametrize("t,e,h", [(70001, 8, 64), (100003, 60, 72)])
+def test_router_many_rows(hk, t, e, h):
+    rng = np.random.default_rng(t)
+    x, w = rng.integers(-3, 4, (t, h)).astype(np.float32), rng.integers(-3, 4, (e, h)).astype(np.float32)
+    np.testing.assert_array_equal(hk.router_logits(_dev(x, BF16), _dev(w, BF16)).cpu().numpy(), x @ w.T)
+
+
+@pytest.mark.parametrize("how", ["mixed", "segments"])
+@pytest.mark.parametrize("r,bf16", [(8, True), (72, False)])
+def test_lora_more_rows_than_are_sorted(hk, r, bf16, how):
+    _lora_case(hk, 65536 + 70, 72, 72, r, 5, how, bf16=bf16, in_place=bf16)
