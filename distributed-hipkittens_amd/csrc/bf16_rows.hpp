@@ -24,25 +24,24 @@ __device__ __forceinline__ f32x4 mfma_bf16_16x16x32(const bf16x8& a, const bf16x
 
 __device__ __forceinline__ bf16x8 zero_bf16x8() { return __builtin_bit_cast(bf16x8, i32x4{0, 0, 0, 0}); }
 
-constexpr int kRowsBlock = 64;  // rows per workgroup at most (4 MFMA row tiles)
+constexpr int kRowsBlock = 64;  // adapters' rows per workgroup at most (4 MFMA row tiles)
 constexpr int kRowsStep = 64;   // K per step: whole 128-byte lines
 
-// acc[mt][nt] += rows of x (MT tiles of 16; xr: this lane's row in each) times rows of
-// w (wr, likewise), over K steps st, st + stride, ... < steps of 64.  Rows past the
+// acc[nt] += 16 rows of x (xr: this lane's) times NT tiles of 16 rows of w (wr: this lane's
+// row in each), over K steps st, st + stride, ... < steps of 64.  Rows past the
 // last may repeat a valid one: a result row depends on its own operand rows alone.
 // The loads of up to DEPTH steps are issued before the first product, so that
-// 2 DEPTH (MT + NT) of them are in flight per wave.
-template <int MT, int NT, int DEPTH>
-__device__ __forceinline__ void rows_product(const uint16_t* const (&xr)[MT], const uint16_t* const (&wr)[NT], int K,
-                                             int st, int stride, int steps, f32x4 (&acc)[MT][NT]) {
+// 2 DEPTH (1 + NT) of them are in flight per wave.
+template <int NT, int DEPTH>
+__device__ __forceinline__ void rows_product(const uint16_t* xr, const uint16_t* const (&wr)[NT], int K, int st, int stride,
+                                             int steps, f32x4 (&acc)[NT]) {
   const int k_lane = 8 * (lane_id() >> 4);
-  bf16x8 a[DEPTH][2][MT], b[DEPTH][2][NT];
+  bf16x8 a[DEPTH][2], b[DEPTH][2][NT];
   auto load = [&](int d, int k0) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = k0 + 32 * h + k_lane;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[d][h][i] = *reinterpret_cast<const bf16x8*>(xr[i] + k);
+      a[d][h] = *reinterpret_cast<const bf16x8*>(xr + k);
 #pragma unroll
       for (int i = 0; i < NT; ++i) b[d][h][i] = *reinterpret_cast<const bf16x8*>(wr[i] + k);
     }
@@ -51,9 +50,7 @@ __device__ __forceinline__ void rows_product(const uint16_t* const (&xr)[MT], co
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mfma_bf16_16x16x32(a[d][h][i], b[d][h][j], acc[i][j]);
+      for (int j = 0; j < NT; ++j) acc[j] = mfma_bf16_16x16x32(a[d][h], b[d][h][j], acc[j]);
   };
   const int full = min(steps, K / kRowsStep);  // steps without a ragged end
   for (; st + (DEPTH - 1) * stride < full; st += DEPTH * stride) {
@@ -70,8 +67,7 @@ __device__ __forceinline__ void rows_product(const uint16_t* const (&xr)[MT], co
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = st * kRowsStep + 32 * h + k_lane;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[0][h][i] = k < K ? *reinterpret_cast<const bf16x8*>(xr[i] + k) : zero_bf16x8();
+      a[0][h] = k < K ? *reinterpret_cast<const bf16x8*>(xr + k) : zero_bf16x8();
 #pragma unroll
       for (int i = 0; i < NT; ++i) b[0][h][i] = k < K ? *reinterpret_cast<const bf16x8*>(wr[i] + k) : zero_bf16x8();
     }
@@ -80,19 +76,16 @@ __device__ __forceinline__ void rows_product(const uint16_t* const (&xr)[MT], co
 }
 
 // Sums the waves' tiles in wave order and hands (row, column, value) of the
-// [16 MT, 16 NT] result to `put`.  red: WAVES * MT * NT * 256 floats of LDS.
-template <int MT, int NT, int WAVES, typename Put>
-__device__ __forceinline__ void rows_reduce(const f32x4 (&acc)[MT][NT], float* red, Put put) {
+// [16, 16 NT] result to `put`.  red: WAVES * NT * 256 floats of LDS.
+template <int NT, int WAVES, typename Put>
+__device__ __forceinline__ void rows_reduce(const f32x4 (&acc)[NT], float* red, Put put) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr int kTile = MT * NT * 256;
+  constexpr int kTile = NT * 256;
   __syncthreads();  // red is free: the last user's reads are done
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        red[wave * kTile + ((i * 16 + 4 * (lane >> 4) + r) * NT + j) * 16 + (lane & 15)] = acc[i][j][r];
+    for (int r = 0; r < 4; ++r) red[wave * kTile + ((4 * (lane >> 4) + r) * NT + j) * 16 + (lane & 15)] = acc[j][r];
   __syncthreads();
   for (int e = threadIdx.x; e < kTile; e += WAVES * 64) {
     float v = red[e];
@@ -282,7 +275,7 @@ struct Strip {
   static constexpr int kStep = (MT + NT) * 2048, kRing = NW * DEPTH * kStep, kLd = 16 * NT + 4;
   static constexpr int kPart = NW * 16 * MT * kLd * 4, kLds = kRing > kPart ? kRing : kPart;
   static constexpr int kLoads = 2 * (MT + NT);  // DMA instructions per step
-  static_assert((MT == 1 || MT == 2) && (NT == 1 || NT == 2), "tile");
+  static_assert(1 <= MT && MT <= NT && NT <= 2, "tile");
   static_assert(DEPTH >= 2 && kLoads * (DEPTH - 1) <= 63 && kLds <= kSkMaxLds, "ring depth, vmcnt range");
 };
 
@@ -643,15 +636,13 @@ __global__ __launch_bounds__(kPlanWaves * 64) void lora_plan_kernel(const int32_
   });
 }
 
-// v[split] of up to 16 MT rows of adapter `id` and 16 NT ranks from r0.
-template <int MT, int NT, int DEPTH>
+// v[split] of up to 16 rows of adapter `id` and 16 NT ranks from r0.
+template <int NT, int DEPTH>
 __device__ __forceinline__ void lora_shrink_tile(const LoraParams& p, int64_t t0, int id, int n, const int* list, int r0,
                                                  float* red) {
   const int lane = lane_id(), wave = threadIdx.x >> 6, split = blockIdx.z;
-  const uint16_t* xr[MT];
+  const uint16_t* xr = p.x + (t0 + list[min(lane & 15, n - 1)]) * p.x_stride;
   const uint16_t* wr[NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) xr[i] = p.x + (t0 + list[min(16 * i + (lane & 15), n - 1)]) * p.x_stride;
 #pragma unroll
   for (int j = 0; j < NT; ++j)
     wr[j] = p.a + (static_cast<int64_t>(id) * p.rank + min(r0 + 16 * j + (lane & 15), p.rank - 1)) * p.hidden;
@@ -659,10 +650,10 @@ __device__ __forceinline__ void lora_shrink_tile(const LoraParams& p, int64_t t0
   const int steps = (p.hidden + kRowsStep - 1) / kRowsStep;
   const int s0 = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
   const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
-  f32x4 acc[MT][NT] = {};
-  rows_product<MT, NT, DEPTH>(xr, wr, p.hidden, s0 + wave, kLoraWaves, s1, acc);
+  f32x4 acc[NT] = {};
+  rows_product<NT, DEPTH>(xr, wr, p.hidden, s0 + wave, kLoraWaves, s1, acc);
   float* v = p.v + (split * p.rows + t0) * p.rank;
-  rows_reduce<MT, NT, kLoraWaves>(acc, red, [&](int i, int c, float val) {
+  rows_reduce<NT, kLoraWaves>(acc, red, [&](int i, int c, float val) {
     if (i < n && r0 + c < p.rank) v[static_cast<int64_t>(list[i]) * p.rank + r0 + c] = val;
   });
 }
@@ -709,7 +700,7 @@ __global__ __launch_bounds__(kLoraWaves * 64) void lora_shrink_kernel(LoraParams
       if (n > 16)
         lora_shrink_panel<P>(p, t0, gid, n, list, r0, smem);
       else
-        lora_shrink_tile<1, NT, 4>(p, t0, gid, n, list, r0, red);
+        lora_shrink_tile<NT, 4>(p, t0, gid, n, list, r0, red);
     }
   });
 }
