@@ -707,10 +707,10 @@ __global__ __launch_bounds__(kLoraWaves * 64) void lora_shrink_kernel(LoraParams
 
 // The narrow product's terms in bf16: v = t0 + t1 (+ t2), each the rounding of what
 // the terms before it leave, 2^-17 (2^-25) of |v| at most: a single bf16 term would
-// be off by 2^-9, more than an fp32 output may lose and as much as a bf16 one rounds.
+// be off by 2^-8, more than an fp32 output may lose and as much as a bf16 one rounds.
 // B is bf16 already and every product is exact, so two terms give a bf16 output,
 // three an fp32 one, the result of an fp32 v.  An infinite or NaN v keeps its value
-// in t0 and leaves 0 in the others.
+// in t0 and leaves 0 in the others, and one past bf16's largest value becomes infinite.
 template <int TERMS>
 __device__ __forceinline__ void split_bf16(float v, uint16_t (&t)[TERMS]) {
 #pragma unroll

@@ -440,12 +440,13 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
  *   scaling [adapters] fp32 or NULL (1).  out may be y itself (with its stride; rows
  *   without an adapter are then not touched) and overlaps nothing else.
  *   H % 8 == 0, N % 8 == 0, rank % 8 == 0, rank <= 256, H <= 2^20, N <= 2^23; pad
- *   smaller ranks with zeros.  v = x A_l^T is kept to 2^-17 (fp32 y: 2^-25) of its
- *   value; an infinite value of A or B gives an infinity or a NaN.
+ *   smaller ranks with zeros.  v = scaling[l] x A_l^T is kept to 2^-17 (fp32 y: 2^-25) of its
+ *   value, for 2^-100 < |v| < 2^127; an infinite value of A or B gives an infinity or a NaN.
  *   workspace: hkmoe_lora_workspace_size(T, H, rank) bytes, not shared by calls that
  *   overlap in time.
- * Results are deterministic, but the sums' order follows from the shapes: a row's last
- * bits may differ with the number of rows beside it.
+ * The same call gives the same bits, but the order of the sums follows from the shapes, and
+ * in lora_add also from how many of the rows around a row have its adapter: a row's last
+ * bits may differ with the rows beside it.  (The norm's do not.)
  */
 size_t hkmoe_rms_norm_quant_workspace_size(int64_t rows, int scale_mode, int given_scale);
 int hkmoe_rms_norm_quant(const void* x, const void* residual, const void* weight, int64_t rows, int64_t cols,
