@@ -609,6 +609,7 @@ int launch_expert_offsets(const int32_t* block_counts, int64_t num_tokens, int32
 // residual + norm + quantisation, router, adapters
 // ---------------------------------------------------------------------------
 constexpr int64_t kMaxRows = 1 << 24;  // a launch's work-items stay below 2^32 in each dimension
+constexpr int64_t kLoraMaxHidden = 1 << 20;  // 64 rows, and an adapter's ranks, below 2^32 bytes
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -1675,7 +1676,7 @@ int hkmoe_router_logits(const void* x, const void* w, int64_t num_tokens, int32_
 }
 
 size_t hkmoe_lora_workspace_size(int64_t rows, int64_t hidden, int32_t rank) {
-  if (rows <= 0 || hidden <= 0 || rank <= 0) return 0;
+  if (rows <= 0 || rows > kMaxRows || hidden <= 0 || hidden > kLoraMaxHidden || rank <= 0 || rank > kLoraMaxRank) return 0;
   return lora_partials(rows, hidden, rank) + lora_plan_bytes(rows);
 }
 
@@ -1685,7 +1686,7 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
                    hkmoe_stream_t stream) {
   HK_REQUIRE(rows >= 0 && rows <= kMaxRows && adapters >= 1, "lora_add: bad shape rows=%lld adapters=%d",
              (long long)rows, adapters);
-  HK_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= (1 << 20) && n > 0 && n % 8 == 0 && n <= (1 << 23),
+  HK_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= kLoraMaxHidden && n > 0 && n % 8 == 0 && n <= (1 << 23),
              "lora_add: H=%lld and N=%lld must be multiples of 8, at most 2^20 and 2^23", (long long)hidden, (long long)n);
   HK_REQUIRE(rank > 0 && rank % 8 == 0 && rank <= kLoraMaxRank, "lora_add: rank=%d must be a multiple of 8, at most %d",
              rank, kLoraMaxRank);

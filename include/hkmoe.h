@@ -442,8 +442,8 @@ int hkmoe_quant_tensor(const float* x, int64_t rows, int64_t cols, void* q, floa
  *   H % 8 == 0, N % 8 == 0, rank % 8 == 0, rank <= 256, H <= 2^20, N <= 2^23; pad
  *   smaller ranks with zeros.  v = scaling[l] x A_l^T is kept to 2^-17 (fp32 y: 2^-25) of its
  *   value, for 2^-100 < |v| < 2^127; an infinite value of A or B gives an infinity or a NaN.
- *   workspace: hkmoe_lora_workspace_size(T, H, rank) bytes, not shared by calls that
- *   overlap in time.
+ *   workspace: hkmoe_lora_workspace_size(T, H, rank) bytes (0 for T, H or rank out of range),
+ *   not shared by calls that overlap in time.
  * The same call gives the same bits, but the order of the sums follows from the shapes, and
  * in lora_add also from how many of the rows around a row have its adapter: a row's last
  * bits may differ with the rows beside it.  (The norm's do not.)

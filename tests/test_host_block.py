@@ -312,3 +312,12 @@ def test_every_grid_dimension_in_range(fake):
         v = {k: int(n) for k, n in (f.split("=") for f in l.split()[2:])}
         assert 1 <= v["grid"] and v["grid"] * v["threads"] < 1 << 32 and 1 <= v["y"] <= 65535 and 1 <= v["z"] <= 65535, l
         assert v["threads"] <= 1024, l
+
+
+def test_lora_workspace_of_refused_sizes(lib):
+    """Sizes that lora_add refuses have no workspace: no sum of theirs leaves 64 bits."""
+    top = 2 ** 63 - 1
+    for rows, hidden, rank in ((top, 256, 8), (4, top, 8), (top, top, 2 ** 31 - 1), (4, 256, 2 ** 31 - 1), ((1 << 24) + 1, 256, 8),
+                               (4, (1 << 20) + 8, 8), (4, 256, 264)):
+        assert lib.hkmoe_lora_workspace_size(i64(rows), i64(hidden), i32(rank)) == 0, (rows, hidden, rank)
+    assert lib.hkmoe_lora_workspace_size(i64(1 << 24), i64(1 << 20), i32(256)) >= (1 << 24) * 256 * 4
