@@ -412,7 +412,7 @@ __global__ __launch_bounds__(P::kWaves * 64) void router_panel_kernel(RouterPara
 // the blocks are of one adapter each.  Then two launches: the narrow product
 // v = x A_l^T (its K split over `splits` workgroups, each writing its own fp32 partial
 // sums), and y + c_l v B_l^T.
-// 8192 rows, 7168 -> 64 -> 4096, bf16: 32 us (22 at a copy's rate) and 44 (28).
+// 8192 rows, 7168 -> 64 -> 4096, bf16: 31 us (22 at a copy's rate) and 43 (28).
 // ---------------------------------------------------------------------------
 struct LoraParams {
   const void* y;

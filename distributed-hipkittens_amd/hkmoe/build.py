@@ -26,7 +26,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared",
-    # packed fp32 VALU ops are kept out of every kernel on this hardware pool
+    # packed fp32 VALU ops are kept out of every kernel: some forms gave wrong results
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # fp32 '/' must be IEEE-correctly rounded (quantisation is bit-exact)
     "-fhip-fp32-correctly-rounded-divide-sqrt",
