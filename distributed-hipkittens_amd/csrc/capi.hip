@@ -12,6 +12,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <limits>
 #include <string>
 
 #include "../../include/hkmoe.h"
@@ -20,8 +21,10 @@
 #include "gemm_narrow.hpp"
 #include "gemm_skinny.hpp"
 #include "gemm_small.hpp"
+#include "layer_norm.hpp"
 #include "moe_kernels.hpp"
 #include "norm_quant.hpp"
+#include "permute.hpp"
 
 #include <atomic>
 #include <cstdlib>
@@ -186,12 +189,10 @@ std::atomic<int> g_dense_mfma{32};
 
 // The dense GEMM on 128x128 tiles (gemm_small.hpp): one workgroup per tile,
 // the grid a whole number of 4x8 tile blocks.
-template <bool F32OUT, bool M32, bool MX>
-int launch_gemm_small(const SmallGemmParams& p, hipStream_t stream) {
-  static bool attr_set[kMaxDevices] = {false};
+template <bool MX, typename K>
+int launch_gemm_small(K kern, bool (&attr_set)[kMaxDevices], const SmallGemmParams& p, hipStream_t stream) {
   int dev = 0;
   (void)hipGetDevice(&dev);
-  auto kern = gemm_fp8_small<F32OUT, M32, MX>;
   constexpr int lds = sm_lds_bytes(MX);
   if (dev >= 0 && dev < kMaxDevices && !attr_set[dev]) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
@@ -203,13 +204,19 @@ int launch_gemm_small(const SmallGemmParams& p, hipStream_t stream) {
   hipLaunchKernelGGL(kern, dim3(grid), dim3(kSmThreads), lds, stream, p);
   return check_launch("gemm_fp8_small");
 }
+template <bool F32OUT, bool M32, bool MX, bool EPI>
+int launch_gemm_small(const SmallGemmParams& p, hipStream_t stream) {
+  static bool attr_set[kMaxDevices] = {false};
+  if constexpr (EPI) return launch_gemm_small<MX>(gemm_fp8_small_act<F32OUT, MX>, attr_set, p, stream);
+  else return launch_gemm_small<MX>(gemm_fp8_small<F32OUT, M32, MX>, attr_set, p, stream);
+}
 
-template <int MF, int NF, int NW, bool MX, bool F32OUT>
+template <int MF, int NF, int NW, bool MX, bool F32OUT, bool EPI>
 int launch_gemm_skinny(const SkinnyParams& p, hipStream_t stream) {
   static bool attr_set[kMaxDevices] = {false};
   int dev = 0;
   (void)hipGetDevice(&dev);
-  auto kern = gemm_fp8_skinny<MF, NF, NW, MX, F32OUT>;
+  auto kern = gemm_fp8_skinny<MF, NF, NW, MX, F32OUT, EPI>;
   constexpr int lds = sk_lds_bytes(MF, NF, NW, MX);
   if (dev >= 0 && dev < kMaxDevices && !attr_set[dev]) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
@@ -221,11 +228,12 @@ int launch_gemm_skinny(const SkinnyParams& p, hipStream_t stream) {
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(grid)), dim3(NW * 64), lds, stream, p);
   return check_launch("gemm_fp8_skinny");
 }
-template <int MF, int NF, int NW, bool MX>
+template <int MF, int NF, int NW, bool MX, bool EPI>
 int launch_gemm_skinny(SkinnyParams p, bool f32out, hipStream_t stream) {
   p.strips = p.n / (16 * NF);
   p.m_blocks = (p.m + 16 * MF - 1) / (16 * MF);
-  return f32out ? launch_gemm_skinny<MF, NF, NW, MX, true>(p, stream) : launch_gemm_skinny<MF, NF, NW, MX, false>(p, stream);
+  return f32out ? launch_gemm_skinny<MF, NF, NW, MX, true, EPI>(p, stream)
+                : launch_gemm_skinny<MF, NF, NW, MX, false, EPI>(p, stream);
 }
 
 // Estimated times (us) of the dense kernels, from which the dense GEMM picks one:
@@ -259,16 +267,17 @@ int dense_block_log2(int64_t m, int64_t n, int64_t* rounds) {
   return best;
 }
 
-DenseKernel pick_dense(int64_t m, int64_t n, int64_t k, bool f32out, bool mx) {
+// wide: fp32 C with an epilogue, whose products run in bf16 and not in the 256x256 kernel.
+DenseKernel pick_dense(int64_t m, int64_t n, int64_t k, bool f32out, bool mx, bool wide = false) {
   const double ks = static_cast<double>(k / kBK), cus = device_cus(), nk = static_cast<double>(n) * k;
   const uint64_t um = m, un = n, ncu = device_cus();
-  DenseKernel best = DenseKernel::kTile256;
-  double best_t = 0;
+  DenseKernel best = DenseKernel::kTile128;
+  double best_t = std::numeric_limits<double>::infinity();
   auto offer = [&](DenseKernel kern, double compute, double hbm) {
     const double t = std::max(compute, hbm) + 0.1 * compute;
-    if (kern == DenseKernel::kTile256 || t < best_t) best = kern, best_t = t;
+    if (t < best_t) best = kern, best_t = t;
   };
-  {
+  if (!wide) {
     const double tiles = static_cast<double>((m + kBM - 1) / kBM) * (n / kBN);
     auto step = [&](double t) {  // per step, t tiles in the round
       return t <= cus / 4 ? (mx ? 1.12 : 0.95) : t <= cus / 2 ? (mx ? 1.27 : 1.13) : (mx ? 1.45 : 1.3);
@@ -308,13 +317,13 @@ DenseKernel pick_dense(int64_t m, int64_t n, int64_t k, bool f32out, bool mx) {
 }
 
 // The dense GEMM (a, b, c and shapes checked by the caller).  MX: scale_a and
-// scale_b are the packed exponent words.
-template <bool MX>
+// scale_b are the packed exponent words.  EPI: with epi's epilogue.
+template <bool MX, bool EPI = false>
 int launch_dense(const void* a, const void* b, void* c, int64_t m, int64_t n, int64_t k, const float* scale_a,
-                 const float* scale_b, int out_dtype, hipStream_t s) {
+                 const float* scale_b, int out_dtype, hipStream_t s, const EpilogueArgs& epi = {}) {
   const bool f32out = out_dtype == HKMOE_F32;
   const int32_t m64 = static_cast<int32_t>((m + 63) / 64 * 64);
-  const DenseKernel kern = pick_dense(m, n, k, f32out, MX);
+  const DenseKernel kern = pick_dense(m, n, k, f32out, MX, EPI && f32out);
   if (kern < DenseKernel::kTile128) {
     SkinnyParams q{};
     q.a = static_cast<const uint8_t*>(a);
@@ -326,13 +335,14 @@ int launch_dense(const void* a, const void* b, void* c, int64_t m, int64_t n, in
     q.n = static_cast<int32_t>(n);
     q.k = static_cast<int32_t>(k);
     q.m64 = m64;
+    q.epi = epi;
     switch (kern) {
-      case DenseKernel::kStrip11: return launch_gemm_skinny<1, 1, 8, MX>(q, f32out, s);
-      case DenseKernel::kStrip21: return launch_gemm_skinny<2, 1, 8, MX>(q, f32out, s);
-      case DenseKernel::kStrip12: return launch_gemm_skinny<1, 2, 8, MX>(q, f32out, s);
-      case DenseKernel::kStrip22: return launch_gemm_skinny<2, 2, 8, MX>(q, f32out, s);
-      case DenseKernel::kStrip24: return launch_gemm_skinny<2, 4, 4, MX>(q, f32out, s);
-      default: return launch_gemm_skinny<4, 4, 4, MX>(q, f32out, s);
+      case DenseKernel::kStrip11: return launch_gemm_skinny<1, 1, 8, MX, EPI>(q, f32out, s);
+      case DenseKernel::kStrip21: return launch_gemm_skinny<2, 1, 8, MX, EPI>(q, f32out, s);
+      case DenseKernel::kStrip12: return launch_gemm_skinny<1, 2, 8, MX, EPI>(q, f32out, s);
+      case DenseKernel::kStrip22: return launch_gemm_skinny<2, 2, 8, MX, EPI>(q, f32out, s);
+      case DenseKernel::kStrip24: return launch_gemm_skinny<2, 4, 4, MX, EPI>(q, f32out, s);
+      default: return launch_gemm_skinny<4, 4, 4, MX, EPI>(q, f32out, s);
     }
   }
   if (kern == DenseKernel::kTile128) {
@@ -351,13 +361,12 @@ int launch_dense(const void* a, const void* b, void* c, int64_t m, int64_t n, in
     q.m_tiles = static_cast<int32_t>((m + kSmTile - 1) / kSmTile);
     q.n_tiles = static_cast<int32_t>(n / kSmTile);
     q.nbn = (q.n_tiles + 7) / 8;
-    if constexpr (MX) {
-      return f32out ? launch_gemm_small<true, false, true>(q, s) : launch_gemm_small<false, false, true>(q, s);
-    } else {
+    q.epi = epi;
+    if constexpr (!MX && !EPI) {
       if (g_dense_mfma.load() == 32)
-        return f32out ? launch_gemm_small<true, true, false>(q, s) : launch_gemm_small<false, true, false>(q, s);
-      return f32out ? launch_gemm_small<true, false, false>(q, s) : launch_gemm_small<false, false, false>(q, s);
+        return f32out ? launch_gemm_small<true, true, false, false>(q, s) : launch_gemm_small<false, true, false, false>(q, s);
     }
+    return f32out ? launch_gemm_small<true, false, MX, EPI>(q, s) : launch_gemm_small<false, false, MX, EPI>(q, s);
   }
   GemmParams p{};
   p.a = static_cast<const uint8_t*>(a);
@@ -375,8 +384,12 @@ int launch_dense(const void* a, const void* b, void* c, int64_t m, int64_t n, in
   p.n_tiles = static_cast<int32_t>(n / kBN);
   int64_t rounds;
   p.blk_m_log2 = dense_block_log2(m, n, &rounds);
+  p.epi = epi;
   constexpr Scale kSc = MX ? Scale::kMX : Scale::kTensor;
-  return f32out ? launch_gemm<Epi::kStoreF32, kSc>(p, s) : launch_gemm<Epi::kStoreBf16, kSc>(p, s);
+  if constexpr (!EPI) {
+    if (f32out) return launch_gemm<Epi::kStoreF32, kSc>(p, s);
+  }
+  return launch_gemm<EPI ? Epi::kActBf16 : Epi::kStoreBf16, kSc>(p, s);
 }
 
 template <Epi EPI, Scale SC, int P, int NW, int ROWS, bool PAD>
@@ -648,6 +661,77 @@ int launch_norm(const NormParams& p, int mode, hipStream_t s) {
   return check_launch("norm_quant_tensor_kernel");
 }
 
+// ---------------------------------------------------------------------------
+// layer norm
+// ---------------------------------------------------------------------------
+// A row's threads.  To 512 columns a part of a wave, to 1024 a wave with two chunks a lane: no
+// barrier, several rows a workgroup.  Wider rows take a workgroup.
+template <typename F>
+int with_layer_norm_shape(int64_t cols, F&& f) {
+  using std::integral_constant;
+  if (cols <= 128) return f(integral_constant<int, 1>{}, integral_constant<int, 16>{});
+  if (cols <= 256) return f(integral_constant<int, 1>{}, integral_constant<int, 32>{});
+  if (cols <= 512) return f(integral_constant<int, 1>{}, integral_constant<int, 64>{});
+  if (cols <= 1024) return f(integral_constant<int, 2>{}, integral_constant<int, 64>{});
+  if (cols <= kNormMaxThreads * kNormChunk) return f(integral_constant<int, 1>{}, integral_constant<int, 0>{});
+  return f(integral_constant<int, 4>{}, integral_constant<int, 0>{});
+}
+
+// Threads of a workgroup that has a whole row of `ch` chunks a thread.
+int row_threads(int64_t cols, int ch) { return static_cast<int>((cols / kNormChunk + ch * kWave - 1) / (ch * kWave) * kWave); }
+
+template <bool F32>
+int launch_layer_norm(const LayerNormParams& p, hipStream_t s) {
+  return with_layer_norm_shape(p.cols, [&](auto ch, auto lanes) {
+    constexpr int CH = decltype(ch)::value, LANES = decltype(lanes)::value;
+    constexpr int rows = kLnRowThreads / (LANES ? LANES : kLnRowThreads);  // of a workgroup
+    const int threads = LANES ? kLnRowThreads : row_threads(p.cols, CH);
+    const int64_t grid = LANES ? (p.rows + rows - 1) / rows : std::min<int64_t>(p.rows, 1 << 20);
+    hipLaunchKernelGGL((layer_norm_kernel<F32, CH, LANES>), dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, p);
+    return check_launch("layer_norm_kernel");
+  });
+}
+
+// Workgroups of the gradient, each of which leaves one partial of dw and db.
+int layer_norm_parts(int64_t rows, int64_t cols) {
+  int per = 1;  // rows at a time
+  (void)with_layer_norm_shape(cols, [&](auto, auto lanes) {
+    constexpr int LANES = decltype(lanes)::value;
+    per = kLnRowThreads / (LANES ? LANES : kLnRowThreads);
+    return HKMOE_OK;
+  });
+  return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, kLnParts));
+}
+
+template <bool F32>
+int launch_layer_norm_grad(const LayerNormGradParams& p, hipStream_t s) {
+  return with_layer_norm_shape(p.cols, [&](auto ch, auto lanes) {
+    constexpr int CH = decltype(ch)::value, LANES = decltype(lanes)::value;
+    const int threads = LANES ? kLnRowThreads : row_threads(p.cols, CH);
+    hipLaunchKernelGGL((layer_norm_grad_kernel<F32, CH, LANES>), dim3(layer_norm_parts(p.rows, p.cols)), dim3(threads), 0, s, p);
+    return check_launch("layer_norm_grad_kernel");
+  });
+}
+
+// ---------------------------------------------------------------------------
+// tokens by expert
+// ---------------------------------------------------------------------------
+int64_t sort_span(int64_t slots) {  // slots of a sorting workgroup
+  const int64_t chunks = (slots + kSortSlots - 1) / kSortSlots;
+  return (chunks + kSortBlocks - 1) / kSortBlocks * kSortSlots;
+}
+int sort_blocks(int64_t slots) { return static_cast<int>((slots + sort_span(slots) - 1) / sort_span(slots)); }
+
+// A workgroup per token, to 2^20 of them; more tokens take turns.
+unsigned move_grid(int64_t tokens) { return static_cast<unsigned>(std::min<int64_t>(tokens, 1 << 20)); }
+
+// Threads for a row of `chunks` 16-byte chunks (or 8 values): the fewest turns of up to
+// kMoveThreads, then the fewest threads.
+int move_threads(int64_t chunks) {
+  const int64_t turns = (chunks + kMoveThreads - 1) / kMoveThreads;
+  return static_cast<int>(((chunks + turns - 1) / turns + kWave - 1) / kWave * kWave);
+}
+
 template <typename K>
 int raise_lds(K kern, int bytes, bool (&done)[kMaxDevices]) {
   int dev = 0;
@@ -825,18 +909,44 @@ int hkmoe_set_dense_mfma(int32_t shape) {
 
 int hkmoe_get_dense_mfma(void) { return g_dense_mfma.load(); }
 
+static int gemm_fp8_check(const char* name, const void* a, const void* b, void* c, int64_t m, int64_t n, int64_t k,
+                          int out_dtype) {
+  HK_REQUIRE(b && (m == 0 || (a && c)), "%s: null tensor pointer", name);
+  HK_REQUIRE(m >= 0 && n > 0 && k > 0, "%s: bad shape M=%lld N=%lld K=%lld", name, (long long)m, (long long)n, (long long)k);
+  HK_REQUIRE(k % 128 == 0, "%s: K=%lld must be a multiple of 128", name, (long long)k);
+  HK_REQUIRE(n % kBN == 0, "%s: N=%lld must be a multiple of 256", name, (long long)n);
+  HK_REQUIRE(k <= (1 << 20) && n * k < (1ll << 32) && m * k < (1ll << 32) && m < (1ll << 31),
+             "%s: operand too large for 32-bit buffer offsets (M*K and N*K must be < 2^32)", name);
+  HK_REQUIRE(out_dtype == HKMOE_BF16 || out_dtype == HKMOE_F32, "%s: bad out_dtype %d", name, out_dtype);
+  return HKMOE_OK;
+}
+
 int hkmoe_gemm_fp8(const void* a, const void* b, void* c, int64_t m, int64_t n, int64_t k,
                    const float* scale_a, const float* scale_b, int out_dtype, hkmoe_stream_t stream) {
-  HK_REQUIRE(b && (m == 0 || (a && c)), "gemm_fp8: null tensor pointer");
-  HK_REQUIRE(m >= 0 && n > 0 && k > 0, "gemm_fp8: bad shape M=%lld N=%lld K=%lld", (long long)m,
-             (long long)n, (long long)k);
-  HK_REQUIRE(k % 128 == 0, "gemm_fp8: K=%lld must be a multiple of 128", (long long)k);
-  HK_REQUIRE(n % kBN == 0, "gemm_fp8: N=%lld must be a multiple of 256", (long long)n);
-  HK_REQUIRE(k <= (1 << 20) && n * k < (1ll << 32) && m * k < (1ll << 32) && m < (1ll << 31),
-             "gemm_fp8: operand too large for 32-bit buffer offsets (M*K and N*K must be < 2^32)");
-  HK_REQUIRE(out_dtype == HKMOE_BF16 || out_dtype == HKMOE_F32, "gemm_fp8: bad out_dtype %d", out_dtype);
+  HK_TRY(gemm_fp8_check("gemm_fp8", a, b, c, m, n, k, out_dtype));
   if (m == 0) return HKMOE_OK;
   return launch_dense<false>(a, b, c, m, n, k, scale_a, scale_b, out_dtype, static_cast<hipStream_t>(stream));
+}
+
+// The epilogue's arguments (C's shape and type checked before).
+static int epilogue_check(const char* name, const void* c, int64_t m, int64_t n, const void* bias, int bias_dtype,
+                          int activation, const void* residual, EpilogueArgs* e) {
+  HK_REQUIRE(activation >= HKMOE_ACT_NONE && activation <= HKMOE_ACT_GELU_TANH, "%s: bad activation %d", name, activation);
+  HK_REQUIRE(!bias || bias_dtype == HKMOE_BF16 || bias_dtype == HKMOE_F32, "%s: bad bias_dtype %d", name, bias_dtype);
+  HK_REQUIRE(n <= (1 << 22), "%s: N=%lld must be at most 2^22", name, (long long)n);
+  HK_REQUIRE(aligned16(bias) && aligned16(residual) && aligned16(c), "%s: bias, residual and C must be 16-byte aligned", name);
+  *e = EpilogueArgs{bias, m > 0 ? residual : nullptr, static_cast<Act>(activation), bias_dtype == HKMOE_F32};
+  return HKMOE_OK;
+}
+
+int hkmoe_gemm_fp8_epilogue(const void* a, const void* b, void* c, int64_t m, int64_t n, int64_t k, const float* scale_a,
+                            const float* scale_b, int out_dtype, const void* bias, int bias_dtype, int activation,
+                            const void* residual, hkmoe_stream_t stream) {
+  EpilogueArgs e{};
+  HK_TRY(gemm_fp8_check("gemm_fp8_epilogue", a, b, c, m, n, k, out_dtype));
+  HK_TRY(epilogue_check("gemm_fp8_epilogue", c, m, n, bias, bias_dtype, activation, residual, &e));
+  if (m == 0) return HKMOE_OK;
+  return launch_dense<false, true>(a, b, c, m, n, k, scale_a, scale_b, out_dtype, static_cast<hipStream_t>(stream), e);
 }
 
 int hkmoe_route_blocks(int64_t num_tokens) { return route_blocks(num_tokens); }
@@ -1660,6 +1770,181 @@ int hkmoe_rms_norm_quant(const void* x, const void* residual, const void* weight
   return x_dtype == HKMOE_F32 ? launch_norm<true>(p, scale_mode, st) : launch_norm<false>(p, scale_mode, st);
 }
 
+size_t hkmoe_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
+  if (rows <= 0 || rows > kMaxRows || cols <= 0 || cols > kLnMaxCols) return 0;
+  return align256(static_cast<size_t>(layer_norm_parts(rows, cols)) * 2 * cols * sizeof(float));
+}
+
+// What both directions ask of the sizes and types.
+static int layer_norm_check(const char* name, int64_t rows, int64_t cols, int x_dtype, int weight_dtype) {
+  HK_REQUIRE(rows >= 0 && rows <= kMaxRows, "%s: bad shape rows=%lld", name, (long long)rows);
+  HK_REQUIRE(cols > 0 && cols % kNormChunk == 0 && cols <= kLnMaxCols, "%s: cols=%lld must be a multiple of 8, at most %d",
+             name, (long long)cols, kLnMaxCols);
+  HK_REQUIRE((x_dtype == HKMOE_BF16 || x_dtype == HKMOE_F32) && (weight_dtype == HKMOE_BF16 || weight_dtype == HKMOE_F32),
+             "%s: bad dtype %d / %d", name, x_dtype, weight_dtype);
+  return HKMOE_OK;
+}
+
+int hkmoe_layer_norm(const void* x, const void* residual, const void* weight, const void* bias, int64_t rows, int64_t cols,
+                     int x_dtype, int weight_dtype, double eps, void* y, void* residual_out, float* stats,
+                     hkmoe_stream_t stream) {
+  HK_TRY(layer_norm_check("layer_norm", rows, cols, x_dtype, weight_dtype));
+  HK_REQUIRE(eps > 0 && eps < 1e30, "layer_norm: eps=%g must be positive and finite", eps);
+  HK_REQUIRE(weight && (rows == 0 || (x && y && stats)), "layer_norm: null pointer");
+  HK_REQUIRE(rows == 0 || !residual == !residual_out, "layer_norm: residual and residual_out come together");
+  HK_REQUIRE(aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(bias) && aligned16(y) &&
+                 aligned16(residual_out) && aligned16(stats),
+             "layer_norm: tensors must be 16-byte aligned");
+  if (rows == 0) return HKMOE_OK;
+  LayerNormParams p{};
+  p.x = x;
+  p.residual = residual;
+  p.weight = weight;
+  p.bias = bias;
+  p.y = y;
+  p.residual_out = residual_out;
+  p.stats = reinterpret_cast<f32x4*>(stats);
+  p.rows = rows;
+  p.cols = static_cast<int32_t>(cols);
+  p.w_f32 = weight_dtype == HKMOE_F32;
+  p.eps = eps;
+  auto s = static_cast<hipStream_t>(stream);
+  return x_dtype == HKMOE_F32 ? launch_layer_norm<true>(p, s) : launch_layer_norm<false>(p, s);
+}
+
+int hkmoe_layer_norm_backward(const void* dy, const void* r, const void* weight, const void* dr, const float* stats,
+                              int64_t rows, int64_t cols, int x_dtype, int weight_dtype, void* dx, void* dweight,
+                              void* dbias, void* workspace, size_t workspace_bytes, hkmoe_stream_t stream) {
+  HK_TRY(layer_norm_check("layer_norm_backward", rows, cols, x_dtype, weight_dtype));
+  HK_REQUIRE(weight && dweight && (rows == 0 || (dy && r && stats && dx)), "layer_norm_backward: null pointer");
+  HK_REQUIRE(aligned16(dy) && aligned16(r) && aligned16(weight) && aligned16(dr) && aligned16(stats) && aligned16(dx) &&
+                 aligned16(dweight) && aligned16(dbias),
+             "layer_norm_backward: tensors must be 16-byte aligned");
+  const size_t need = hkmoe_layer_norm_backward_workspace_size(rows, cols);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    return fail(HKMOE_ERR_WORKSPACE, "layer_norm_backward: workspace needs %zu bytes, 16-byte aligned", need);
+  LayerNormGradParams p{};
+  p.dy = dy;
+  p.r = r;
+  p.weight = weight;
+  p.dr = dr;
+  p.stats = reinterpret_cast<const f32x4*>(stats);
+  p.dx = dx;
+  p.part = static_cast<float*>(workspace);
+  p.rows = rows;
+  p.cols = static_cast<int32_t>(cols);
+  p.w_f32 = weight_dtype == HKMOE_F32;
+  auto s = static_cast<hipStream_t>(stream);
+  if (rows > 0) HK_TRY(x_dtype == HKMOE_F32 ? launch_layer_norm_grad<true>(p, s) : launch_layer_norm_grad<false>(p, s));
+  // without rows the sums are empty: zeros
+  hipLaunchKernelGGL(layer_norm_sum_kernel, dim3(static_cast<unsigned>((2 * cols + 63) / 64)), dim3(256), 0, s, p.part,
+                     rows > 0 ? layer_norm_parts(rows, cols) : 0, p.cols, dweight, dbias, p.w_f32);
+  return check_launch("layer_norm_sum_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// tokens by expert and back, and their gradients
+// ---------------------------------------------------------------------------
+static int slots_check(const char* name, int64_t num_tokens, int32_t top_k) {
+  HK_REQUIRE(num_tokens >= 0 && num_tokens <= kMaxRows && top_k >= 1 && top_k <= kMaxTopK,
+             "%s: bad shape T=%lld k=%d (1 <= k <= %d)", name, (long long)num_tokens, top_k, kMaxTopK);
+  return HKMOE_OK;
+}
+static int hidden_check(const char* name, int64_t hidden, int dtype) {
+  HK_REQUIRE(hidden > 0 && hidden <= (1 << 24) && hidden % 8 == 0, "%s: H=%lld must be a multiple of 8, at most 2^24", name,
+             (long long)hidden);
+  HK_REQUIRE(dtype == HKMOE_BF16 || dtype == HKMOE_F32, "%s: bad dtype %d", name, dtype);
+  return HKMOE_OK;
+}
+
+size_t hkmoe_permute_workspace_size(int64_t num_tokens, int32_t num_experts, int32_t top_k) {
+  if (num_tokens <= 0 || num_tokens > kMaxRows || top_k < 1 || top_k > kMaxTopK || num_experts < 1 || num_experts > kMaxExperts)
+    return 0;
+  const int64_t slots = num_tokens * top_k;
+  return slots <= kSortSmall ? 0 : align256(static_cast<size_t>(sort_blocks(slots)) * (num_experts + 1) * sizeof(int32_t));
+}
+
+int hkmoe_permute(const void* x, const int32_t* ids, int64_t num_tokens, int32_t num_experts, int32_t top_k, int64_t hidden,
+                  int dtype, void* xp, int32_t* offsets, int32_t* perm, int32_t* inv_perm, void* workspace,
+                  size_t workspace_bytes, hkmoe_stream_t stream) {
+  HK_TRY(slots_check("permute", num_tokens, top_k));
+  HK_REQUIRE(num_experts >= 1 && num_experts <= kMaxExperts, "permute: E=%d outside [1, %d]", num_experts, kMaxExperts);
+  if (dtype == HKMOE_E4M3) {
+    HK_REQUIRE(hidden > 0 && hidden <= (1 << 24) && hidden % 16 == 0, "permute: H=%lld must be a multiple of 16, at most 2^24",
+               (long long)hidden);
+  } else {
+    HK_TRY(hidden_check("permute", hidden, dtype));
+  }
+  HK_REQUIRE(offsets && (num_tokens == 0 || (x && ids && xp && perm && inv_perm)), "permute: null pointer");
+  HK_REQUIRE(aligned16(x) && aligned16(xp), "permute: x and xp must be 16-byte aligned");
+  const size_t need = hkmoe_permute_workspace_size(num_tokens, num_experts, top_k);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    return fail(HKMOE_ERR_WORKSPACE, "permute: workspace needs %zu bytes, 16-byte aligned", need);
+  const int64_t slots = num_tokens * top_k, row_bytes = hidden * (dtype == HKMOE_E4M3 ? 1 : dtype == HKMOE_BF16 ? 2 : 4);
+  auto s = static_cast<hipStream_t>(stream);
+  if (slots <= kSortSmall) {
+    hipLaunchKernelGGL(permute_small_kernel, dim3(static_cast<unsigned>(slots + 1)), dim3(kSortThreads), 0, s, ids,
+                       static_cast<int>(slots), num_experts, top_k, static_cast<const uint8_t*>(x), row_bytes,
+                       static_cast<uint8_t*>(xp), offsets, perm, inv_perm);
+    return check_launch("permute_small_kernel");
+  }
+  const int blocks = sort_blocks(slots);
+  auto* counts = static_cast<int32_t*>(workspace);
+  hipLaunchKernelGGL(sort_count_kernel, dim3(blocks), dim3(kSortThreads), 0, s, ids, slots, sort_span(slots), num_experts, counts);
+  HK_TRY(check_launch("sort_count_kernel"));
+  hipLaunchKernelGGL(sort_place_kernel, dim3(blocks), dim3(kSortThreads), 0, s, ids, slots, sort_span(slots), num_experts,
+                     counts, blocks, offsets, perm, inv_perm);
+  HK_TRY(check_launch("sort_place_kernel"));
+  hipLaunchKernelGGL(permute_rows_kernel, dim3(move_grid(num_tokens)), dim3(move_threads(row_bytes / 16)), 0, s,
+                     static_cast<const uint8_t*>(x), num_tokens, row_bytes, inv_perm, top_k, offsets + num_experts,
+                     static_cast<uint8_t*>(xp));
+  return check_launch("permute_rows_kernel");
+}
+
+int hkmoe_combine_rows(const void* y, const float* topk_w, const int32_t* offsets, const int32_t* inv_perm, int64_t num_tokens,
+                       int32_t num_experts, int32_t top_k, int64_t hidden, int dtype, void* out, hkmoe_stream_t stream) {
+  HK_TRY(slots_check("combine_rows", num_tokens, top_k));
+  HK_TRY(hidden_check("combine_rows", hidden, dtype));
+  HK_REQUIRE(num_experts >= 1 && num_experts <= kMaxExperts, "combine_rows: E=%d outside [1, %d]", num_experts, kMaxExperts);
+  HK_REQUIRE(num_tokens == 0 || (y && offsets && inv_perm && out), "combine_rows: null pointer");
+  HK_REQUIRE(aligned16(y) && aligned16(out), "combine_rows: y and out must be 16-byte aligned");
+  if (num_tokens == 0) return HKMOE_OK;
+  auto kern = dtype == HKMOE_F32 ? combine_rows_kernel<true> : combine_rows_kernel<false>;
+  hipLaunchKernelGGL(kern, dim3(move_grid(num_tokens)), dim3(move_threads(hidden / 8)), 0,
+                     static_cast<hipStream_t>(stream), y, topk_w, num_tokens, inv_perm, top_k, offsets + num_experts,
+                     static_cast<int>(hidden), out);
+  return check_launch("combine_rows_kernel");
+}
+
+int hkmoe_combine_rows_backward(const void* dout, const void* y, const float* topk_w, const int32_t* offsets,
+                                const int32_t* inv_perm, int64_t num_tokens, int32_t num_experts, int32_t top_k,
+                                int64_t hidden, int dtype, void* dy, float* dw, hkmoe_stream_t stream) {
+  HK_TRY(slots_check("combine_rows_backward", num_tokens, top_k));
+  HK_TRY(hidden_check("combine_rows_backward", hidden, dtype));
+  HK_REQUIRE(num_experts >= 1 && num_experts <= kMaxExperts, "combine_rows_backward: E=%d outside [1, %d]", num_experts,
+             kMaxExperts);
+  HK_REQUIRE(num_tokens == 0 || (dout && y && topk_w && offsets && inv_perm && dy && dw), "combine_rows_backward: null pointer");
+  HK_REQUIRE(aligned16(dout) && aligned16(y) && aligned16(dy), "combine_rows_backward: dout, y and dy must be 16-byte aligned");
+  if (num_tokens == 0) return HKMOE_OK;
+  auto kern = dtype == HKMOE_F32 ? combine_grad_kernel<true> : combine_grad_kernel<false>;
+  hipLaunchKernelGGL(kern, dim3(move_grid(num_tokens)), dim3(move_threads(hidden / 8)), 0,
+                     static_cast<hipStream_t>(stream), dout, y, topk_w, num_tokens, inv_perm, top_k, offsets + num_experts,
+                     static_cast<int>(hidden), dy, dw);
+  return check_launch("combine_grad_kernel");
+}
+
+int hkmoe_route_topk_backward(const float* dw, const float* topk_w, const int32_t* topk_idx, int64_t num_tokens,
+                              int32_t num_experts, int32_t top_k, float* dlogits, hkmoe_stream_t stream) {
+  HK_TRY(slots_check("route_topk_backward", num_tokens, top_k));
+  HK_REQUIRE(num_experts >= 1 && num_experts <= kMaxExperts && top_k <= num_experts,
+             "route_topk_backward: E=%d outside [k, %d]", num_experts, kMaxExperts);
+  HK_REQUIRE(num_tokens == 0 || (dw && topk_w && topk_idx && dlogits), "route_topk_backward: null pointer");
+  if (num_tokens == 0) return HKMOE_OK;
+  hipLaunchKernelGGL(route_grad_kernel, dim3(static_cast<unsigned>((num_tokens + 3) / 4)), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), dw, topk_w, topk_idx, num_tokens, num_experts, top_k, dlogits);
+  return check_launch("route_grad_kernel");
+}
+
 int hkmoe_router_logits(const void* x, const void* w, int64_t num_tokens, int32_t num_experts, int64_t hidden,
                         float* logits, hkmoe_stream_t stream) {
   HK_REQUIRE(num_tokens >= 0 && num_tokens <= kMaxRows && num_experts >= 1 && num_experts <= kMaxExperts,
@@ -1792,21 +2077,37 @@ int hkmoe_mx_pack_scales(const void* s, int64_t rows, int64_t cols, void* packed
   return check_launch("mx_pack_scales_kernel");
 }
 
-int hkmoe_gemm_mx(const void* a, const void* a_scale, const void* b, const void* b_scale, void* c, int64_t m,
-                  int64_t n, int64_t k, int out_dtype, hkmoe_stream_t stream) {
-  HK_REQUIRE(b && b_scale && (m == 0 || (a && a_scale && c)), "gemm_mx: null pointer");
-  HK_REQUIRE(m >= 0 && n > 0 && k > 0, "gemm_mx: bad shape M=%lld N=%lld K=%lld", (long long)m, (long long)n,
-             (long long)k);
-  HK_REQUIRE(k % kBK == 0, "gemm_mx: K=%lld must be a multiple of 128", (long long)k);
-  HK_REQUIRE(n % kBN == 0, "gemm_mx: N=%lld must be a multiple of 256", (long long)n);
+static int gemm_mx_check(const char* name, const void* a, const void* a_scale, const void* b, const void* b_scale, void* c,
+                         int64_t m, int64_t n, int64_t k, int out_dtype) {
+  HK_REQUIRE(b && b_scale && (m == 0 || (a && a_scale && c)), "%s: null pointer", name);
+  HK_REQUIRE(m >= 0 && n > 0 && k > 0, "%s: bad shape M=%lld N=%lld K=%lld", name, (long long)m, (long long)n, (long long)k);
+  HK_REQUIRE(k % kBK == 0, "%s: K=%lld must be a multiple of 128", name, (long long)k);
+  HK_REQUIRE(n % kBN == 0, "%s: N=%lld must be a multiple of 256", name, (long long)n);
   const int64_t m64 = (m + 63) / 64 * 64;
   HK_REQUIRE(k <= (1 << 20) && n * k < (1ll << 32) && m * k < (1ll << 32) && m < (1ll << 31) &&
                  m64 * (k / 32) < (1ll << 32) && n * (k / 32) < (1ll << 32),
-             "gemm_mx: operand too large for 32-bit buffer offsets (M*K and N*K must be < 2^32)");
-  HK_REQUIRE(out_dtype == HKMOE_BF16 || out_dtype == HKMOE_F32, "gemm_mx: bad out_dtype %d", out_dtype);
+             "%s: operand too large for 32-bit buffer offsets (M*K and N*K must be < 2^32)", name);
+  HK_REQUIRE(out_dtype == HKMOE_BF16 || out_dtype == HKMOE_F32, "%s: bad out_dtype %d", name, out_dtype);
+  return HKMOE_OK;
+}
+
+int hkmoe_gemm_mx(const void* a, const void* a_scale, const void* b, const void* b_scale, void* c, int64_t m,
+                  int64_t n, int64_t k, int out_dtype, hkmoe_stream_t stream) {
+  HK_TRY(gemm_mx_check("gemm_mx", a, a_scale, b, b_scale, c, m, n, k, out_dtype));
   if (m == 0) return HKMOE_OK;
   return launch_dense<true>(a, b, c, m, n, k, static_cast<const float*>(a_scale),
                             static_cast<const float*>(b_scale), out_dtype, static_cast<hipStream_t>(stream));
+}
+
+int hkmoe_gemm_mx_epilogue(const void* a, const void* a_scale, const void* b, const void* b_scale, void* c, int64_t m,
+                           int64_t n, int64_t k, int out_dtype, const void* bias, int bias_dtype, int activation,
+                           const void* residual, hkmoe_stream_t stream) {
+  EpilogueArgs e{};
+  HK_TRY(gemm_mx_check("gemm_mx_epilogue", a, a_scale, b, b_scale, c, m, n, k, out_dtype));
+  HK_TRY(epilogue_check("gemm_mx_epilogue", c, m, n, bias, bias_dtype, activation, residual, &e));
+  if (m == 0) return HKMOE_OK;
+  return launch_dense<true, true>(a, b, c, m, n, k, static_cast<const float*>(a_scale), static_cast<const float*>(b_scale),
+                                  out_dtype, static_cast<hipStream_t>(stream), e);
 }
 
 int64_t hkmoe_mx_words_per_step(int64_t rows, int32_t num_experts) {

@@ -74,10 +74,11 @@
 #include <type_traits>
 
 #include "common.hpp"
+#include "epilogue.hpp"
 
 namespace hkmoe {
 
-enum class Epi : int { kStoreBf16 = 0, kStoreF32 = 1, kSiluBf16 = 2, kSiluQuant = 3, kSiluMx = 4 };
+enum class Epi : int { kStoreBf16 = 0, kStoreF32 = 1, kSiluBf16 = 2, kSiluQuant = 3, kSiluMx = 4, kActBf16 = 5 };
 enum class Scale : int { kTensor = 0, kBlock = 1, kMX = 2 };
 
 struct GemmParams {
@@ -121,6 +122,7 @@ struct GemmParams {
   int32_t b_packed;            // 1: b is in the packed tile layout of pack_weights_kernel
   int32_t blk_m_log2;          // tile blocks are 2^blk_m_log2 M tiles x 32 / 2^blk_m_log2 N tiles
   int64_t cs_rs;               // kSiluMx: words per K step of the packed h exponents
+  EpilogueArgs epi;            // kActBf16
 };
 
 constexpr int kBM = 256, kBN = 256, kBK = 128;
@@ -909,7 +911,8 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_fp8_persistent(GemmParams p)
     const int row0 = cur.row0, valid = cur.valid, nt = cur.nt;
     // output rows row0 .. row0 + valid - 1 as one buffer: stores to rows past
     // `valid` (the next expert's rows) fall outside it and are dropped
-    constexpr int kOutBytes = (EPI == Epi::kStoreBf16) ? 2 : (EPI == Epi::kSiluQuant || EPI == Epi::kSiluMx) ? 1 : 4;
+    constexpr bool kAct = EPI == Epi::kActBf16;
+    constexpr int kOutBytes = (EPI == Epi::kStoreBf16 || EPI == Epi::kActBf16) ? 2 : (EPI == Epi::kSiluQuant || EPI == Epi::kSiluMx) ? 1 : 4;
     const i32x4 out_srd =
         make_srd(static_cast<uint8_t*>(p.c) + static_cast<int64_t>(row0) * p.n_out * kOutBytes,
                  static_cast<uint32_t>(valid) * static_cast<uint32_t>(p.n_out) * kOutBytes);
@@ -922,21 +925,51 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_fp8_persistent(GemmParams p)
     if constexpr (SC == Scale::kTensor)
       tens = (p.a_scale ? p.a_scale[0] : 1.0f) * (p.b_scale ? p.b_scale[cur.e] : 1.0f);
 
-    if constexpr (EPI == Epi::kStoreBf16) {
+    // kAct: bias of the lane's columns, and the residual of two sub-tiles as it is stored, loaded
+    // together ahead of the activation (rows past `valid` repeat the last one, and are not stored)
+    const int ecol = nt * kBN + wg * 64 + elg * 4;
+    f32x4 bias[4];
+    if constexpr (kAct) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bias[j] = epilogue_bias(p.epi, ecol + 16 * j);
+    }
+    uint2 res[2][4];
+    auto load_res = [&, HK_CAP](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t at = static_cast<int64_t>(row0 + min(wave_row0 + (i + h) * 16 + el16, valid - 1)) * p.n_out + ecol;
+        const uint16_t* from = static_cast<const uint16_t*>(p.epi.residual) + at;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) res[h][j] = *reinterpret_cast<const uint2*>(from + 16 * j);
+      }
+    };
+    // sub-tile i, fragment j
+    auto out4 = [&, HK_CAP](int i, int j) __attribute__((always_inline)) -> f32x4 {
+      f32x4 v{acc[i][j][0] * tens, acc[i][j][1] * tens, acc[i][j][2] * tens, acc[i][j][3] * tens};
+      if constexpr (kAct) {
+        v = activate(v + bias[j], p.epi.act);
+        if (p.epi.residual != nullptr) v = v + as_f32x4(res[i & 1][j]);
+      }
+      return v;
+    };
+
+    if constexpr (EPI == Epi::kStoreBf16 || EPI == Epi::kActBf16) {
       // four rounds of 64 rows: sub-tiles 2q, 2q+1 of both halves (LDS row
       // rr = 32*grp + 16*(i - 2q) + l16, 512 bytes = 32 chunks)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (32 * q >= valid) break;  // uniform: no row of this round or later is stored
+        if constexpr (kAct) {
+          if (p.epi.residual != nullptr) load_res(2 * q);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int i = 2 * q + h, rr = grp * 32 + h * 16 + el16;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int c = wg * 8 + 2 * j + (elg >> 1);
-            uint2 v;
-            v.x = pack_bf16x2(acc[i][j][0] * tens, acc[i][j][1] * tens);
-            v.y = pack_bf16x2(acc[i][j][2] * tens, acc[i][j][3] * tens);
+            const f32x4 o = out4(i, j);
+            const uint2 v{pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w)};
             *reinterpret_cast<uint2*>(ct + rr * 512 + ((c ^ (rr & 31)) << 4) + (elg & 1) * 8) = v;
           }
         }
@@ -967,12 +1000,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_fp8_persistent(GemmParams p)
         if (i < live_sub && r < valid) {
           const int64_t off = static_cast<int64_t>(row0 + r) * p.n_out + nt * kBN + wg * 64 + lg * 4;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float4 v;
-            v.x = acc[i][j][0] * tens; v.y = acc[i][j][1] * tens;
-            v.z = acc[i][j][2] * tens; v.w = acc[i][j][3] * tens;
-            *reinterpret_cast<float4*>(static_cast<float*>(p.c) + off + j * 16) = v;
-          }
+          for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + off + j * 16) = out4(i, j);
         }
       }
     } else {

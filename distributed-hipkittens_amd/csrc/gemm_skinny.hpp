@@ -18,6 +18,7 @@
 // same loads give on whole lines.
 #pragma once
 
+#include "epilogue.hpp"
 #include "gemm_fp8.hpp"
 
 namespace hkmoe {
@@ -31,6 +32,7 @@ struct SkinnyParams {
   int32_t m, n, k, m64;
   int32_t strips;    // N / (16 NF)
   int32_t m_blocks;  // ceil(M / (16 MF))
+  EpilogueArgs epi;  // kernels with an epilogue
 };
 
 constexpr int kSkMaxLds = 160 * 1024;
@@ -95,7 +97,18 @@ __device__ __forceinline__ void skinny_mma(f32x4 (&acc)[NF], const i32x8& a, con
   }
 }
 
-template <int MF, int NF, int NW, bool MX, bool F32OUT>
+// The same with the operands widened to bf16.
+template <int NF, bool MX, int U>
+__device__ __forceinline__ void skinny_mma_wide(f32x4 (&acc)[NF], const i32x8& a, const WideFrag (&b)[NF], int sa) {
+  const WideFrag w = widen(a, MX ? e8m0_scale<U>(sa) : 1.0f);
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].v[s], w.v[s], acc[j], 0, 0, 0);
+}
+
+// EPI: act(C + bias) + residual, and with fp32 C products in bf16 (epilogue.hpp).
+template <int MF, int NF, int NW, bool MX, bool F32OUT, bool EPI = false>
 __global__ __launch_bounds__(NW * 64, 1) void gemm_fp8_skinny(SkinnyParams p) {
   static_assert((MF == 1 || MF == 2 || MF == 4) && (NF == 1 || NF == 2 || NF == 4), "tile");
   constexpr int kRows = 16 * MF, kCols = 16 * NF;
@@ -179,9 +192,12 @@ __global__ __launch_bounds__(NW * 64, 1) void gemm_fp8_skinny(SkinnyParams p) {
   };
   const int x = swz(l16);
   const uint32_t ring_a = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring));
-  const uint32_t lo_off = l16 * kBK + ((lg ^ x) << 4), hi_off = l16 * kBK + (((lg + 4) ^ x) << 4);
   // The scaled MFMA's K order (chunks lg and lg + 4 of a row); any order common
-  // to both operands serves the unscaled one.
+  // to both operands serves the unscaled one.  kWide: the chunks of MX block lg, whose
+  // exponents are in the lane's own words.
+  constexpr bool kWide = EPI && F32OUT;
+  const int c_lo = kWide ? 2 * lg : lg, c_hi = kWide ? 2 * lg + 1 : lg + 4;
+  const uint32_t lo_off = l16 * kBK + ((c_lo ^ x) << 4), hi_off = l16 * kBK + ((c_hi ^ x) << 4);
   auto step = [&](int i, int slot) __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads * (D - 1)) : "memory");
@@ -207,11 +223,27 @@ __global__ __launch_bounds__(NW * 64, 1) void gemm_fp8_skinny(SkinnyParams p) {
     }
     issue(i + D, slot);  // this wave has read the slot
     __builtin_amdgcn_sched_barrier(0);
-    skinny_mma<NF, MX, 0>(acc[0], a[0], b, sa, sb);
-    if constexpr (MF > 1) skinny_mma<NF, MX, 1>(acc[1], a[1], b, sa, sb);
-    if constexpr (MF > 2) {
-      skinny_mma<NF, MX, 2>(acc[2], a[2], b, sa, sb);
-      skinny_mma<NF, MX, 3>(acc[3], a[3], b, sa, sb);
+    if constexpr (kWide) {
+      WideFrag wb[NF];
+      wb[0] = widen(b[0], MX ? e8m0_scale<0>(sb) : 1.0f);
+      if constexpr (NF > 1) wb[1] = widen(b[1], MX ? e8m0_scale<1>(sb) : 1.0f);
+      if constexpr (NF > 2) {
+        wb[2] = widen(b[2], MX ? e8m0_scale<2>(sb) : 1.0f);
+        wb[3] = widen(b[3], MX ? e8m0_scale<3>(sb) : 1.0f);
+      }
+      skinny_mma_wide<NF, MX, 0>(acc[0], a[0], wb, sa);
+      if constexpr (MF > 1) skinny_mma_wide<NF, MX, 1>(acc[1], a[1], wb, sa);
+      if constexpr (MF > 2) {
+        skinny_mma_wide<NF, MX, 2>(acc[2], a[2], wb, sa);
+        skinny_mma_wide<NF, MX, 3>(acc[3], a[3], wb, sa);
+      }
+    } else {
+      skinny_mma<NF, MX, 0>(acc[0], a[0], b, sa, sb);
+      if constexpr (MF > 1) skinny_mma<NF, MX, 1>(acc[1], a[1], b, sa, sb);
+      if constexpr (MF > 2) {
+        skinny_mma<NF, MX, 2>(acc[2], a[2], b, sa, sb);
+        skinny_mma<NF, MX, 3>(acc[3], a[3], b, sa, sb);
+      }
     }
   };
 #pragma unroll
@@ -239,11 +271,12 @@ __global__ __launch_bounds__(NW * 64, 1) void gemm_fp8_skinny(SkinnyParams p) {
 #pragma unroll
     for (int w = 1; w < NW; ++w) s += *reinterpret_cast<const f32x4*>(part + (w * kRows + r) * kLd + cc);
     const int64_t at = static_cast<int64_t>(m0 + r) * p.n + n0 + cc;
+    s = f32x4{s.x * tens, s.y * tens, s.z * tens, s.w * tens};
+    if constexpr (EPI) s = epilogue4<F32OUT>(p.epi, s, epilogue_bias(p.epi, n0 + cc), at);
     if constexpr (F32OUT) {
-      *reinterpret_cast<float4*>(static_cast<float*>(p.c) + at) = float4{s.x * tens, s.y * tens, s.z * tens, s.w * tens};
+      *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at) = s;
     } else {
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.c) + at) =
-          uint2{pack_bf16x2(s.x * tens, s.y * tens), pack_bf16x2(s.z * tens, s.w * tens)};
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.c) + at) = uint2{pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w)};
     }
   }
 }

@@ -18,6 +18,7 @@
 // 64.
 #pragma once
 
+#include "epilogue.hpp"
 #include "gemm_fp8.hpp"
 
 namespace hkmoe {
@@ -44,6 +45,7 @@ struct SmallGemmParams {
   uint32_t a_bytes, b_bytes;  // buffer bounds (min(rows * K, 2^32 - 1))
   int32_t m_tiles, n_tiles;   // 128-row / 128-column tiles
   int32_t nbn;                // tile blocks per block row: ceil(n_tiles / 8)
+  EpilogueArgs epi;           // kernels with an epilogue
 };
 
 // vmcnt wait leaving the newest n_newer stages (L loads each) of this wave in
@@ -60,9 +62,11 @@ static_assert(kSmAhead <= 4, "small_wait_stage covers at most 3 newer stages");
 // MX: e8m0 exponents applied by the scaled 16x16x128 MFMA (read_operand's K
 // order); a K step's words of the tile (64 per 64-row group of A and of B)
 // ride in the stage, one 4-byte-per-lane DMA per wave.
-template <bool F32OUT, bool M32, bool MX = false>
-__global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small(SmallGemmParams p) {
-  static_assert(!(M32 && MX), "MX runs on the 16x16x128 MFMA");
+// EPI: act(C + bias) + residual, and with fp32 C products in bf16 (epilogue.hpp).
+template <bool F32OUT, bool M32, bool MX, bool EPI>
+__device__ __forceinline__ void gemm_small_tile(const SmallGemmParams& p) {
+  static_assert(!(M32 && (MX || EPI)), "MX and the epilogue run on 16x16 outputs");
+  constexpr bool kWide = EPI && F32OUT;  // operands widened to bf16
   constexpr int kStg = sm_stage_bytes(MX);
   constexpr int kLoads = MX ? 5 : 4;  // vector-memory instructions per wave and step
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -141,9 +145,9 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small(SmallGemmParams 
       for (int f = 0; f < 2; ++f) bf[f] = read_frag(st + kSmOperandBytes, 32 * wn + l32, 2 * f + g32, f32);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) af[i] = read_operand<MX>(st, 64 * wm + 16 * i + l16, lg, fx);
+      for (int i = 0; i < 4; ++i) af[i] = read_operand<MX && !kWide>(st, 64 * wm + 16 * i + l16, lg, fx);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) bf[j] = read_operand<MX>(st + kSmOperandBytes, 32 * wn + 16 * j + l16, lg, fx);
+      for (int j = 0; j < 2; ++j) bf[j] = read_operand<MX && !kWide>(st + kSmOperandBytes, 32 * wn + 16 * j + l16, lg, fx);
     }
   };
 
@@ -162,7 +166,24 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small(SmallGemmParams 
       for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   auto mma = [&](const i32x8 (&af)[4], const i32x8 (&bf)[2], const Words& w) __attribute__((always_inline)) {
-    if constexpr (MX) {
+    if constexpr (kWide) {
+      // lane group lg holds K bytes 32lg .. +31 of its rows: MX block lg, whose exponents are in the
+      // lane's own words
+      const WideFrag b0 = widen(bf[0], MX ? e8m0_scale<0>(w.b) : 1.0f), b1 = widen(bf[1], MX ? e8m0_scale<1>(w.b) : 1.0f);
+      auto sub = [&](auto u) __attribute__((always_inline)) {
+        constexpr int U = decltype(u)::value;
+        const WideFrag a = widen(af[U], MX ? e8m0_scale<U>(w.a) : 1.0f);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          acc[U][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b0.v[s], a.v[s], acc[U][0], 0, 0, 0);
+          acc[U][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b1.v[s], a.v[s], acc[U][1], 0, 0, 0);
+        }
+      };
+      sub(std::integral_constant<int, 0>{});
+      sub(std::integral_constant<int, 1>{});
+      sub(std::integral_constant<int, 2>{});
+      sub(std::integral_constant<int, 3>{});
+    } else if constexpr (MX) {
       auto sub = [&](auto u) __attribute__((always_inline)) {
         constexpr int U = decltype(u)::value;
         acc[U][0] = mfma_mx<0, U>(bf[0], af[U], acc[U][0], w.b, w.a);
@@ -247,18 +268,28 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small(SmallGemmParams 
     else
       return acc[i][j];
   };
+  constexpr int kColStep = 32 / kColSteps;
+  const int ecol = n0 + 32 * wn + 4 * (M32 ? g32 : lg);  // the lane's first column
+  f32x4 bias[kColSteps];
+  if constexpr (EPI) {
+#pragma unroll
+    for (int j = 0; j < kColSteps; ++j) bias[j] = epilogue_bias(p.epi, ecol + kColStep * j);
+  }
+  // the finished values of row step i (row r < M of C), columns j
+  auto finish = [&](int i, int j, int r) __attribute__((always_inline)) -> f32x4 {
+    f32x4 v = value(i, j);
+    v = f32x4{v.x * tens, v.y * tens, v.z * tens, v.w * tens};
+    if constexpr (EPI) v = epilogue4<F32OUT>(p.epi, v, bias[j], static_cast<int64_t>(r) * p.n + ecol + kColStep * j);
+    return v;
+  };
   if constexpr (F32OUT) {
 #pragma unroll
     for (int i = 0; i < kRowSteps; ++i) {
       const int r = m0 + 64 * wm + (64 / kRowSteps) * i + er;
       if (r < p.m) {
-        float* dst = static_cast<float*>(p.c) + static_cast<int64_t>(r) * p.n + n0 + 32 * wn + 4 * (M32 ? g32 : lg);
+        float* dst = static_cast<float*>(p.c) + static_cast<int64_t>(r) * p.n + ecol;
 #pragma unroll
-        for (int j = 0; j < kColSteps; ++j) {
-          const f32x4 v = value(i, j);
-          *reinterpret_cast<float4*>(dst + (32 / kColSteps) * j) =
-              float4{v.x * tens, v.y * tens, v.z * tens, v.w * tens};
-        }
+        for (int j = 0; j < kColSteps; ++j) *reinterpret_cast<f32x4*>(dst + kColStep * j) = finish(i, j, r);
       }
     }
   } else {
@@ -271,10 +302,10 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small(SmallGemmParams 
 #pragma unroll
       for (int j = 0; j < kColSteps; ++j) {
         const int c = 4 * wn + (M32 ? j : 2 * j + (lg >> 1)), half = M32 ? g32 : (lg & 1);
-        const f32x4 a = value(i, j);
+        const f32x4 a = finish(i, j, min(m0 + r, p.m - 1));  // rows past M repeat the last one, and are not stored
         uint2 v;
-        v.x = pack_bf16x2(a.x * tens, a.y * tens);
-        v.y = pack_bf16x2(a.z * tens, a.w * tens);
+        v.x = pack_bf16x2(a.x, a.y);
+        v.y = pack_bf16x2(a.z, a.w);
         *reinterpret_cast<uint2*>(smem + r * 256 + ((c ^ (r & 15)) << 4) + half * 8) = v;
       }
     }
@@ -288,6 +319,16 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small(SmallGemmParams 
       }
     }
   }
+}
+
+template <bool F32OUT, bool M32, bool MX = false>
+__global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small(SmallGemmParams p) {
+  gemm_small_tile<F32OUT, M32, MX, false>(p);
+}
+// With an epilogue, on the 16x16x128 MFMA.
+template <bool F32OUT, bool MX>
+__global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small_act(SmallGemmParams p) {
+  gemm_small_tile<F32OUT, false, MX, true>(p);
 }
 
 }  // namespace hkmoe

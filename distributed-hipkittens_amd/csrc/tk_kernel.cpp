@@ -987,6 +987,220 @@ void dispatch_lora_add(py::object y_, py::object x_, py::object a_, py::object b
                        static_cast<int32_t>(rank), yt, o.ptr, os, ws.ptr, byte_size(ws, "workspace"), cur.stream));
 }
 
+// ---------------------------------------------------------------------------
+// dense products with an epilogue
+// ---------------------------------------------------------------------------
+struct EpilogueTensors {
+  TensorArg bias, residual;
+  int out, bias_type;
+};
+// Checks A, B, C and the epilogue's tensors against each other.
+EpilogueTensors epilogue_tensors(const TensorArg& a, const TensorArg& b, const TensorArg& c, const py::object& bias_,
+                                 const py::object& residual_, const Current& cur) {
+  want_dtype(a, "A", kF8);
+  want_dtype(b, "B", kF8);
+  want_dim(a, "A", 2);
+  want_dim(b, "B", 2);
+  want_dim(c, "C", 2);
+  if (b.shape[1] != a.shape[1]) throw std::runtime_error("A and B must have the same K");
+  if (c.shape[0] != a.shape[0] || c.shape[1] != b.shape[0]) throw std::runtime_error("C must be [M, N]");
+  EpilogueTensors e{as_current_opt(bias_, "bias", cur), as_current_opt(residual_, "residual", cur), float_type(c, "C"), HKMOE_F32};
+  if (!bias_.is_none()) {
+    e.bias_type = float_type(e.bias, "bias");
+    if (e.bias.shape.size() != 1 || e.bias.shape[0] != c.shape[1]) throw std::runtime_error("bias must be [N]");
+  }
+  if (!residual_.is_none()) {
+    if (e.residual.dtype != c.dtype.name) throw std::runtime_error("residual must have C's dtype");
+    if (e.residual.shape != c.shape) throw std::runtime_error("residual must be [M, N]");
+  }
+  return e;
+}
+
+void dispatch_gemm_fp8_epilogue(py::object A, py::object B, py::object C, py::object sa, py::object sb, py::object bias,
+                                int activation, py::object residual) {
+  const Current cur = current();
+  auto a = as_current(A, "A", cur), b = as_current(B, "B", cur), c = as_current(C, "C", cur),
+       as = as_current_opt(sa, "scale_a", cur), bs = as_current_opt(sb, "scale_b", cur);
+  const EpilogueTensors e = epilogue_tensors(a, b, c, bias, residual, cur);
+  want_dtype(as, "scale_a", kF32);
+  want_dtype(bs, "scale_b", kF32);
+  if (!sa.is_none() && as.numel() != 1) throw std::runtime_error("scale_a must hold one value");
+  if (!sb.is_none() && bs.numel() != 1) throw std::runtime_error("scale_b must hold one value");
+  check(hkmoe_gemm_fp8_epilogue(a.ptr, b.ptr, c.ptr, a.shape[0], b.shape[0], a.shape[1], static_cast<const float*>(as.ptr),
+                                static_cast<const float*>(bs.ptr), e.out, e.bias.ptr, e.bias_type, activation,
+                                e.residual.ptr, cur.stream));
+}
+
+void dispatch_gemm_mx_epilogue(py::object A, py::object sa, py::object B, py::object sb, py::object C, py::object bias,
+                               int activation, py::object residual) {
+  const Current cur = current();
+  auto a = as_current(A, "A", cur), b = as_current(B, "B", cur), c = as_current(C, "C", cur),
+       as = as_current(sa, "scale_a", cur), bs = as_current(sb, "scale_b", cur);
+  const EpilogueTensors e = epilogue_tensors(a, b, c, bias, residual, cur);
+  want_dtype(as, "scale_a", kI32);
+  want_dtype(bs, "scale_b", kI32);
+  const int64_t m = a.shape[0], k = a.shape[1], n = b.shape[0];
+  if (as.numel() != (k / 128) * round64(m)) throw std::runtime_error("scale_a must be packed [K/128, M64]");
+  if (bs.numel() != (k / 128) * round64(n)) throw std::runtime_error("scale_b must be packed [K/128, N]");
+  check(hkmoe_gemm_mx_epilogue(a.ptr, as.ptr, b.ptr, bs.ptr, c.ptr, m, n, k, e.out, e.bias.ptr, e.bias_type, activation,
+                               e.residual.ptr, cur.stream));
+}
+
+// ---------------------------------------------------------------------------
+// layer norm
+// ---------------------------------------------------------------------------
+// `t` must have `like`'s shape and dtype.
+void want_like(const TensorArg& t, const char* name, const TensorArg& like, const char* what) {
+  if (t.dtype != like.dtype.name || t.shape != like.shape)
+    throw std::runtime_error(std::string(name) + " must have " + what + "'s shape and dtype");
+}
+
+void dispatch_layer_norm(py::object x_, py::object residual_, py::object weight_, py::object bias_, double eps, py::object y_,
+                         py::object residual_out_, py::object stats_) {
+  const Current cur = current();
+  auto x = as_current(x_, "x", cur), w = as_current(weight_, "weight", cur), y = as_current(y_, "y", cur),
+       st = as_current(stats_, "stats", cur), r = as_current_opt(residual_, "residual", cur),
+       b = as_current_opt(bias_, "bias", cur), ro = as_current_opt(residual_out_, "residual_out", cur);
+  want_dim(x, "x", 2);
+  const int xt = float_type(x, "x"), wt = float_type(w, "weight");
+  const int64_t rows = x.shape[0], cols = x.shape[1];
+  if (w.numel() != cols) throw std::runtime_error("weight must be [C]");
+  if (!bias_.is_none()) want_like(b, "bias", w, "weight");
+  want_like(y, "y", x, "x");
+  if (residual_.is_none() != residual_out_.is_none())
+    throw std::runtime_error("residual and residual_out come together");
+  if (!residual_.is_none()) {
+    want_like(r, "residual", x, "x");
+    want_like(ro, "residual_out", x, "x");
+  }
+  if (st.dtype != kF32 || st.numel() != rows * 4) throw std::runtime_error("stats must be [R, 4] float32");
+  check(hkmoe_layer_norm(x.ptr, r.ptr, w.ptr, b.ptr, rows, cols, xt, wt, eps, y.ptr, ro.ptr, static_cast<float*>(st.ptr),
+                         cur.stream));
+}
+
+void dispatch_layer_norm_backward(py::object dy_, py::object r_, py::object weight_, py::object dr_, py::object stats_,
+                                  py::object dx_, py::object dweight_, py::object dbias_, py::object workspace_) {
+  const Current cur = current();
+  auto dy = as_current(dy_, "dy", cur), r = as_current(r_, "r", cur), w = as_current(weight_, "weight", cur),
+       st = as_current(stats_, "stats", cur), dx = as_current(dx_, "dx", cur), dw = as_current(dweight_, "dweight", cur),
+       dr = as_current_opt(dr_, "dr", cur), db = as_current_opt(dbias_, "dbias", cur),
+       ws = as_current_opt(workspace_, "workspace", cur);
+  want_dim(r, "r", 2);
+  const int xt = float_type(r, "r"), wt = float_type(w, "weight");
+  const int64_t rows = r.shape[0], cols = r.shape[1];
+  if (w.numel() != cols) throw std::runtime_error("weight must be [C]");
+  want_like(dy, "dy", r, "r");
+  want_like(dx, "dx", r, "r");
+  if (!dr_.is_none()) want_like(dr, "dr", r, "r");
+  want_like(dw, "dweight", w, "weight");
+  if (!dbias_.is_none()) want_like(db, "dbias", w, "weight");
+  if (st.dtype != kF32 || st.numel() != rows * 4) throw std::runtime_error("stats must be [R, 4] float32");
+  check(hkmoe_layer_norm_backward(dy.ptr, r.ptr, w.ptr, dr.ptr, static_cast<const float*>(st.ptr), rows, cols, xt, wt, dx.ptr,
+                                  dw.ptr, db.ptr, ws.ptr, byte_size(ws, "workspace"), cur.stream));
+}
+
+// ---------------------------------------------------------------------------
+// tokens by expert and back
+// ---------------------------------------------------------------------------
+void want_ints(const TensorArg& t, const char* name, int64_t n) {
+  if (t.dtype != kI32 || t.numel() != n)
+    throw std::runtime_error(std::string(name) + ": expected " + std::to_string(n) + " int32 values");
+}
+
+// The order of T tokens with k slots each: E from offsets, k from inv_perm [T, k].
+struct Order {
+  TensorArg offsets, inv;
+  int64_t tokens;
+  int32_t experts, top_k;
+};
+Order order_of(const py::object& offsets_, const py::object& inv_, const Current& cur) {
+  Order o{as_current(offsets_, "offsets", cur), as_current(inv_, "inv_perm", cur), 0, 0, 0};
+  want_dim(o.offsets, "offsets", 1);
+  want_dim(o.inv, "inv_perm", 2);
+  if (o.offsets.shape[0] < 2 || o.offsets.shape[0] > kMaxInt || o.inv.shape[1] < 1 || o.inv.shape[1] > kMaxInt)
+    throw std::runtime_error("offsets must be [E + 1] and inv_perm [T, k]");
+  o.tokens = o.inv.shape[0];
+  o.experts = static_cast<int32_t>(o.offsets.shape[0] - 1);
+  o.top_k = static_cast<int32_t>(o.inv.shape[1]);
+  want_ints(o.offsets, "offsets", o.experts + 1);
+  want_ints(o.inv, "inv_perm", o.tokens * o.top_k);
+  return o;
+}
+// Rows of H values for the order's slots (a row each) or tokens.
+void want_rows(const TensorArg& t, const char* name, int64_t rows, int64_t hidden, const char* dtype) {
+  if (t.shape.size() != 2 || t.shape[0] != rows || t.shape[1] != hidden || t.dtype != dtype)
+    throw std::runtime_error(std::string(name) + ": expected [" + std::to_string(rows) + ", " + std::to_string(hidden) + "] " + dtype);
+}
+
+void dispatch_permute(py::object x_, py::object ids_, py::object xp_, py::object offsets_, py::object perm_, py::object inv_,
+                      py::object workspace_) {
+  const Current cur = current();
+  auto x = as_current(x_, "x", cur), ids = as_current(ids_, "ids", cur), xp = as_current(xp_, "xp", cur),
+       perm = as_current(perm_, "perm", cur), ws = as_current_opt(workspace_, "workspace", cur);
+  const Order o = order_of(offsets_, inv_, cur);
+  want_dim(x, "x", 2);
+  if (ids.shape != o.inv.shape || ids.dtype != kI32) throw std::runtime_error("ids must be [T, k] int32");
+  const int type = x.dtype == kF8 ? static_cast<int>(HKMOE_E4M3) : float_type(x, "x");
+  const int64_t hidden = x.shape[1];
+  want_rows(x, "x", o.tokens, hidden, x.dtype.name);
+  want_rows(xp, "xp", o.tokens * o.top_k, hidden, x.dtype.name);
+  want_ints(perm, "perm", o.tokens * o.top_k);
+  check(hkmoe_permute(x.ptr, static_cast<const int32_t*>(ids.ptr), o.tokens, o.experts, o.top_k, hidden, type, xp.ptr,
+                      static_cast<int32_t*>(o.offsets.ptr), static_cast<int32_t*>(perm.ptr), static_cast<int32_t*>(o.inv.ptr),
+                      ws.ptr, byte_size(ws, "workspace"), cur.stream));
+}
+
+void dispatch_combine_rows(py::object y_, py::object w_, py::object offsets_, py::object inv_, py::object out_) {
+  const Current cur = current();
+  auto y = as_current(y_, "y", cur), w = as_current_opt(w_, "topk_w", cur), out = as_current(out_, "out", cur);
+  const Order o = order_of(offsets_, inv_, cur);
+  want_dim(y, "y", 2);
+  const int type = float_type(y, "y");
+  const int64_t hidden = y.shape[1];
+  want_rows(y, "y", o.tokens * o.top_k, hidden, y.dtype.name);
+  want_rows(out, "out", o.tokens, hidden, y.dtype.name);
+  if (!w_.is_none()) want_rows(w, "topk_w", o.tokens, o.top_k, kF32);
+  check(hkmoe_combine_rows(y.ptr, static_cast<const float*>(w.ptr), static_cast<const int32_t*>(o.offsets.ptr),
+                           static_cast<const int32_t*>(o.inv.ptr), o.tokens, o.experts, o.top_k, hidden, type, out.ptr,
+                           cur.stream));
+}
+
+void dispatch_combine_rows_backward(py::object dout_, py::object y_, py::object w_, py::object offsets_, py::object inv_,
+                                    py::object dy_, py::object dw_) {
+  const Current cur = current();
+  auto dout = as_current(dout_, "dout", cur), y = as_current(y_, "y", cur), w = as_current(w_, "topk_w", cur),
+       dy = as_current(dy_, "dy", cur), dw = as_current(dw_, "dw", cur);
+  const Order o = order_of(offsets_, inv_, cur);
+  want_dim(y, "y", 2);
+  const int type = float_type(y, "y");
+  const int64_t hidden = y.shape[1];
+  want_rows(y, "y", o.tokens * o.top_k, hidden, y.dtype.name);
+  want_rows(dy, "dy", o.tokens * o.top_k, hidden, y.dtype.name);
+  want_rows(dout, "dout", o.tokens, hidden, y.dtype.name);
+  want_rows(w, "topk_w", o.tokens, o.top_k, kF32);
+  want_rows(dw, "dw", o.tokens, o.top_k, kF32);
+  check(hkmoe_combine_rows_backward(dout.ptr, y.ptr, static_cast<const float*>(w.ptr), static_cast<const int32_t*>(o.offsets.ptr),
+                                    static_cast<const int32_t*>(o.inv.ptr), o.tokens, o.experts, o.top_k, hidden, type, dy.ptr,
+                                    static_cast<float*>(dw.ptr), cur.stream));
+}
+
+void dispatch_route_topk_backward(py::object dw_, py::object w_, py::object idx_, py::object dlogits_) {
+  const Current cur = current();
+  auto dw = as_current(dw_, "dw", cur), w = as_current(w_, "topk_w", cur), idx = as_current(idx_, "topk_idx", cur),
+       dl = as_current(dlogits_, "dlogits", cur);
+  want_dim(idx, "topk_idx", 2);
+  want_dim(dl, "dlogits", 2);
+  const int64_t t = idx.shape[0], k = idx.shape[1], e = dl.shape[1];
+  if (idx.dtype != kI32) throw std::runtime_error("topk_idx: expected dtype torch.int32");
+  if (k > kMaxInt || e > kMaxInt) throw std::runtime_error("topk_idx and dlogits: too many slots or experts");
+  want_rows(dw, "dw", t, k, kF32);
+  want_rows(w, "topk_w", t, k, kF32);
+  want_rows(dl, "dlogits", t, e, kF32);
+  check(hkmoe_route_topk_backward(static_cast<const float*>(dw.ptr), static_cast<const float*>(w.ptr),
+                                  static_cast<const int32_t*>(idx.ptr), t, static_cast<int32_t>(e), static_cast<int32_t>(k),
+                                  static_cast<float*>(dl.ptr), cur.stream));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(tk_kernel, m) {
@@ -1049,6 +1263,29 @@ PYBIND11_MODULE(tk_kernel, m) {
   m.def("dispatch_lora_add", &dispatch_lora_add, "out = y + scaling[ids] (x A[ids]^T) B[ids]^T", py::arg("y"),
         py::arg("x"), py::arg("a"), py::arg("b"), py::arg("ids"), py::arg("scaling"), py::arg("out"),
         py::arg("workspace"));
+  m.def("dispatch_gemm_fp8_epilogue", &dispatch_gemm_fp8_epilogue, "C = act((sa*sb) A . B^T + bias) + residual",
+        py::arg("A"), py::arg("B"), py::arg("C"), py::arg("scale_a") = py::none(), py::arg("scale_b") = py::none(),
+        py::arg("bias") = py::none(), py::arg("activation") = 0, py::arg("residual") = py::none());
+  m.def("dispatch_gemm_mx_epilogue", &dispatch_gemm_mx_epilogue, "C = act(A . B^T + bias) + residual, 1x32 e8m0 scales",
+        py::arg("A"), py::arg("scale_a"), py::arg("B"), py::arg("scale_b"), py::arg("C"), py::arg("bias") = py::none(),
+        py::arg("activation") = 0, py::arg("residual") = py::none());
+  m.attr("ACTIVATIONS") = py::make_tuple("none", "relu", "silu", "gelu", "gelu_tanh");
+  m.def("dispatch_layer_norm", &dispatch_layer_norm, "residual_out = x + residual; y = its layer norm; stats for the gradient",
+        py::arg("x"), py::arg("residual"), py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("y"),
+        py::arg("residual_out"), py::arg("stats"));
+  m.def("dispatch_layer_norm_backward", &dispatch_layer_norm_backward, py::arg("dy"), py::arg("r"), py::arg("weight"),
+        py::arg("dr"), py::arg("stats"), py::arg("dx"), py::arg("dweight"), py::arg("dbias"), py::arg("workspace"));
+  m.def("layer_norm_backward_workspace_size", &hkmoe_layer_norm_backward_workspace_size, py::arg("rows"), py::arg("cols"));
+  m.def("dispatch_permute", &dispatch_permute, "slots sorted by expert, and the tokens' rows in that order", py::arg("x"),
+        py::arg("ids"), py::arg("xp"), py::arg("offsets"), py::arg("perm"), py::arg("inv_perm"), py::arg("workspace"));
+  m.def("permute_workspace_size", &hkmoe_permute_workspace_size, py::arg("num_tokens"), py::arg("num_experts"),
+        py::arg("top_k"));
+  m.def("dispatch_combine_rows", &dispatch_combine_rows, "out[t] = sum_j topk_w[t,j] y[inv_perm[t,j]]", py::arg("y"),
+        py::arg("topk_w"), py::arg("offsets"), py::arg("inv_perm"), py::arg("out"));
+  m.def("dispatch_combine_rows_backward", &dispatch_combine_rows_backward, py::arg("dout"), py::arg("y"), py::arg("topk_w"),
+        py::arg("offsets"), py::arg("inv_perm"), py::arg("dy"), py::arg("dw"));
+  m.def("dispatch_route_topk_backward", &dispatch_route_topk_backward, py::arg("dw"), py::arg("topk_w"), py::arg("topk_idx"),
+        py::arg("dlogits"));
   m.def("rms_norm_quant_workspace_size", &hkmoe_rms_norm_quant_workspace_size, py::arg("rows"), py::arg("scale_mode"),
         py::arg("given_scale"));
   m.def("lora_workspace_size", &hkmoe_lora_workspace_size, py::arg("rows"), py::arg("hidden"), py::arg("rank"));

@@ -18,6 +18,9 @@ Entry points
   hkmoe.lora_add            adapters of many requests beside a projection
   hkmoe.MoEBlock            norm, router and layer; hkmoe.LoraLinear: projection
                             and adapters
+  hkmoe.gemm_fp8 / gemm_mx  dense products, with bias, activation and residual
+  hkmoe.layer_norm, route_topk, moe_permute, moe_combine
+                            what stands around experts in training, with gradients
 """
 import os
 import sys
@@ -38,6 +41,9 @@ from .layer import (MoELayer, moe_forward, moe_forward_steps, pack_weights,  # n
                     quant_block, quant_group, quant_tensor, gemm_fp8, quant_mx, mx_pack_scales, gemm_mx,
                     mx_pack_weight_scales, moe_forward_mx_steps, MoELayerMX)
 from .block import LoraLinear, MoEBlock, lora_add, rms_norm_quant, router_logits  # noqa: E402
+from .train import (MoEOrder, layer_norm, layer_norm_backward, layer_norm_forward, moe_combine,  # noqa: E402
+                    moe_combine_backward, moe_combine_forward, moe_permute, moe_permute_backward,
+                    moe_permute_forward, route_topk, route_topk_backward, route_topk_forward)
 
 LIB_PATH = os.path.join(_PKG_ROOT, "libhkmoe.so")
 SCALE_TENSOR = tk_kernel.SCALE_TENSOR
@@ -46,5 +52,8 @@ SCALE_BLOCK = tk_kernel.SCALE_BLOCK
 __all__ = ["tk_kernel", "MoELayer", "moe_forward", "moe_forward_steps", "pack_weights", "quant_block",
            "quant_group", "quant_tensor", "gemm_fp8", "quant_mx", "mx_pack_scales", "gemm_mx",
            "mx_pack_weight_scales", "moe_forward_mx_steps", "MoELayerMX", "rms_norm_quant", "router_logits",
-           "lora_add", "LoraLinear", "MoEBlock", "LIB_PATH",
+           "lora_add", "LoraLinear", "MoEBlock", "MoEOrder", "layer_norm", "layer_norm_forward",
+           "layer_norm_backward", "route_topk", "route_topk_forward", "route_topk_backward", "moe_permute",
+           "moe_permute_forward", "moe_permute_backward", "moe_combine", "moe_combine_forward",
+           "moe_combine_backward", "LIB_PATH",
            "SCALE_TENSOR", "SCALE_BLOCK"]

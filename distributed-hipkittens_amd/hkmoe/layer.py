@@ -59,11 +59,34 @@ def quant_tensor(x):
     return q, s
 
 
-def gemm_fp8(a_q, b_q, scale_a=None, scale_b=None, out_dtype=torch.bfloat16):
-    """C = (sa*sb) A . B^T for e4m3 A [M,K], B [N,K]."""
+_ACTIVATIONS = {name: i for i, name in enumerate(tk_kernel.ACTIVATIONS)}
+
+
+def _activation(name):
+    """The activation's number; None is "none"."""
+    if name is None:
+        return 0
+    if not isinstance(name, str) or name not in _ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {name!r}")
+    return _ACTIVATIONS[name]
+
+
+def gemm_fp8(a_q, b_q, scale_a=None, scale_b=None, out_dtype=torch.bfloat16, bias=None, activation=None,
+             residual=None, out=None):
+    """C = act((sa*sb) A . B^T + bias) + residual for e4m3 A [M,K], B [N,K], in one launch.
+
+    ``bias`` bf16 or fp32 [N]; ``activation`` "none", "relu", "silu", "gelu" (the erf form) or
+    "gelu_tanh"; ``residual`` [M,N] in C's dtype.  C is rounded once, to ``out_dtype``, or to the dtype of
+    ``out``, which may be the residual.  With any of these three, "none" included, an fp32 C is the
+    product to fp32's own precision, at half the matrix rate; without, it is what the FP8 matrix
+    instruction gives (1.5e-5 of its size)."""
     _check_dev(a_q, b_q)
-    c = a_q.new_empty((a_q.shape[0], b_q.shape[0]), dtype=out_dtype)
-    tk_kernel.dispatch_gemm_fp8(a_q, b_q, c, scale_a, scale_b)
+    act = _activation(activation)
+    c = a_q.new_empty((a_q.shape[0], b_q.shape[0]), dtype=out_dtype) if out is None else out
+    if bias is None and activation is None and residual is None:
+        tk_kernel.dispatch_gemm_fp8(a_q, b_q, c, scale_a, scale_b)
+    else:
+        tk_kernel.dispatch_gemm_fp8_epilogue(a_q, b_q, c, scale_a, scale_b, bias, act, residual)
     return c
 
 
@@ -90,11 +113,17 @@ def mx_pack_scales(s):
     return packed
 
 
-def gemm_mx(a_q, a_packed, b_q, b_packed, out_dtype=torch.float32):
-    """C = A . B^T with 1x32 e8m0 block scales (packed by mx_pack_scales)."""
+def gemm_mx(a_q, a_packed, b_q, b_packed, out_dtype=torch.float32, bias=None, activation=None, residual=None,
+            out=None):
+    """C = act(A . B^T + bias) + residual with 1x32 e8m0 block scales (packed by mx_pack_scales);
+    the other arguments as in :func:`gemm_fp8`."""
     _check_dev(a_q, b_q)
-    c = a_q.new_empty((a_q.shape[0], b_q.shape[0]), dtype=out_dtype)
-    tk_kernel.dispatch_gemm_mx(a_q, a_packed, b_q, b_packed, c)
+    act = _activation(activation)
+    c = a_q.new_empty((a_q.shape[0], b_q.shape[0]), dtype=out_dtype) if out is None else out
+    if bias is None and activation is None and residual is None:
+        tk_kernel.dispatch_gemm_mx(a_q, a_packed, b_q, b_packed, c)
+    else:
+        tk_kernel.dispatch_gemm_mx_epilogue(a_q, a_packed, b_q, b_packed, c, bias, act, residual)
     return c
 
 

@@ -73,6 +73,38 @@ int hkmoe_gemm_fp8(const void* a, const void* b, void* c, int64_t m, int64_t n, 
                    hkmoe_stream_t stream);
 
 /*
+ * The dense products with an epilogue:  C = act(z + bias) + residual, in fp32, rounded once,
+ * where z is the product of hkmoe_gemm_fp8 / hkmoe_gemm_mx (same operands, scales, limits).
+ *   For bf16 C, z comes from the FP8 matrix instructions, whose sums over eight neighbouring K drop
+ *   what is below about 2^-16 of the largest product (1.5e-5 of a random sum, in the plain
+ *   entry points, too).  For fp32 C, z is summed to fp32's own precision at half the matrix rate;
+ *   MX operands, element times its block's power of two, are then exact between 2^-133 and 2^128,
+ *   smaller ones lose bits and larger ones become infinite.
+ *   bias [N] bf16 or fp32 (bias_dtype) or NULL; residual [M, N] in C's type or NULL, may be C.
+ *   activation:
+ *     HKMOE_ACT_RELU       max(z, 0)
+ *     HKMOE_ACT_SILU       z / (1 + e^-z)
+ *     HKMOE_ACT_GELU       z Phi(z), Phi the normal distribution function (the erf form)
+ *     HKMOE_ACT_GELU_TANH  z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2
+ *   to a few ulp of fp32; for large |z| the exponential costs more: (16 + z^2) 2^-23 of
+ *   Phi(-|z|), (4 + |z|) 2^-23 of SiLU.  C, bias and residual 16-byte aligned, N <= 2^22.  hkmoe_set_dense_mfma does not apply.
+ * No reference counterpart (its GEMMs store C as it is).
+ */
+enum hkmoe_activation {
+  HKMOE_ACT_NONE = 0,
+  HKMOE_ACT_RELU = 1,
+  HKMOE_ACT_SILU = 2,
+  HKMOE_ACT_GELU = 3,
+  HKMOE_ACT_GELU_TANH = 4
+};
+int hkmoe_gemm_fp8_epilogue(const void* a, const void* b, void* c, int64_t m, int64_t n, int64_t k, const float* scale_a,
+                            const float* scale_b, int out_dtype, const void* bias, int bias_dtype, int activation,
+                            const void* residual, hkmoe_stream_t stream);
+int hkmoe_gemm_mx_epilogue(const void* a, const void* a_scale, const void* b, const void* b_scale, void* c, int64_t m,
+                           int64_t n, int64_t k, int out_dtype, const void* bias, int bias_dtype, int activation,
+                           const void* residual, hkmoe_stream_t stream);
+
+/*
  * MFMA shape of hkmoe_gemm_fp8's kernel for mid-sized problems (too few 256x256
  * tiles to fill the chip, e.g. 2048^3), which runs 128x128 tiles: 16 for
  * v_mfma_f32_16x16x128_f8f6f4, 32 for v_mfma_f32_32x32x64_f8f6f4 (the default;
@@ -460,6 +492,69 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
                    const int32_t* ids, const float* scaling, int64_t rows, int32_t adapters, int64_t hidden, int64_t n,
                    int32_t rank, int y_dtype, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
                    hkmoe_stream_t stream);
+
+/*
+ * Layer norm of a residual stream and its gradient.  No reference counterpart (it has no norm).
+ *   hkmoe_layer_norm: r = x + residual, rounded to x's type (residual_out);
+ *     m = mean_j r_j, rstd = fl32(1 / sqrt(mean_j (r_j - m)^2 + eps)), sums in 64 bits;
+ *     finite: at most the largest fp32 value
+ *     y_j = (r_j - m) rstd weight_j + bias_j, in fp32, rounded to x's type
+ *     stats [R, 4] fp32: m as the sum of two terms, rstd, 0, for the gradient
+ *   hkmoe_layer_norm_backward: with n = (r - m) rstd and g = dy * weight
+ *     dx_j = rstd (g_j - mean g - n_j mean(g n)) + dr_j, dweight_j = sum_rows dy_j n_j,
+ *     dbias_j = sum_rows dy_j.  dx is the gradient of x and of the residual; dr: NULL, or what
+ *     comes back along the new stream.
+ *   x, residual, residual_out, y, dy, r, dr, dx [R, C] bf16 or fp32 (x_dtype); weight, bias,
+ *   dweight, dbias [C] bf16 or fp32 (weight_dtype); bias and dbias may be NULL.  residual and
+ *   residual_out both NULL: r = x.  residual_out may be x or residual; dx may be dr or dy;
+ *   other outputs overlap nothing.  C % 8 == 0, C <= 16384, R <= 2^24.  R = 0 writes zeros to dweight
+ *   and dbias.  workspace: hkmoe_layer_norm_backward_workspace_size(R, C) bytes (0 for sizes out of
+ *   range), not shared by calls that overlap in time.
+ * The same call gives the same bits; dweight's and dbias' last bits depend on R.
+ */
+int hkmoe_layer_norm(const void* x, const void* residual, const void* weight, const void* bias, int64_t rows, int64_t cols,
+                     int x_dtype, int weight_dtype, double eps, void* y, void* residual_out, float* stats,
+                     hkmoe_stream_t stream);
+size_t hkmoe_layer_norm_backward_workspace_size(int64_t rows, int64_t cols);
+int hkmoe_layer_norm_backward(const void* dy, const void* r, const void* weight, const void* dr, const float* stats,
+                              int64_t rows, int64_t cols, int x_dtype, int weight_dtype, void* dx, void* dweight,
+                              void* dbias, void* workspace, size_t workspace_bytes, hkmoe_stream_t stream);
+
+/*
+ * Tokens by expert and back around any experts' product, and the gradients.  No reference
+ * counterpart.  A slot is f = t k + j; ids [T, k] holds its expert, and a value outside [0, E)
+ * means that it has none here.
+ *   hkmoe_permute: the stable order of the slots by expert, those without one behind the
+ *     last: perm [T k] (perm[p] = f), inv_perm [T, k] (inv_perm[f] = p), offsets [E + 1] (first place
+ *     of each expert; offsets[E]: places in use); and xp[p] = x[perm[p] / k], rows of zeros from
+ *     offsets[E] on.  x [T, H], xp [T k, H] bf16, fp32 (H % 8 == 0) or e4m3 (H % 16 == 0).
+ *   hkmoe_combine_rows: out[t] = sum_j topk_w[t,j] y[inv_perm[t,j]] over the slots in use, j
+ *     ascending, in fp32, rounded to y's type; topk_w NULL: ones, which is the gradient of
+ *     hkmoe_permute's x for y = xp's gradient.  Rows of y from offsets[E] on are not read.
+ *   hkmoe_combine_rows_backward: dy[inv_perm[t,j]] = topk_w[t,j] dout[t], rounded, zeros from
+ *     offsets[E] on, and dw[t,j] = sum_h dout[t,h] y[inv_perm[t,j],h], 0 for slots not in use.
+ *   hkmoe_route_topk_backward: the gradient of hkmoe_route_topk's topk_w: dlogits [T, E] =
+ *     sum_{j: topk_idx[t,j] = e} w_j (dw_j - sum_i w_i dw_i), zeros elsewhere; indexes outside
+ *     [0, E) are skipped.
+ *   Rows 16-byte aligned and contiguous; dw, topk_w, dlogits fp32; k <= 32 (E may be smaller,
+ *   but in hkmoe_route_topk_backward), E <= 1024, T <= 2^24, H <= 2^24.  Outputs overlap nothing.
+ *   inv_perm and offsets are those that hkmoe_permute wrote (or equal ones); other values give
+ *   other results, but nothing outside the buffers is touched.  T = 0 writes zeros to offsets.
+ *   workspace: hkmoe_permute_workspace_size(T, E, k) bytes (0 for sizes out of range, and where
+ *   none is needed), not shared by calls that overlap in time.
+ * The same call gives the same bits.
+ */
+size_t hkmoe_permute_workspace_size(int64_t num_tokens, int32_t num_experts, int32_t top_k);
+int hkmoe_permute(const void* x, const int32_t* ids, int64_t num_tokens, int32_t num_experts, int32_t top_k, int64_t hidden,
+                  int dtype, void* xp, int32_t* offsets, int32_t* perm, int32_t* inv_perm, void* workspace,
+                  size_t workspace_bytes, hkmoe_stream_t stream);
+int hkmoe_combine_rows(const void* y, const float* topk_w, const int32_t* offsets, const int32_t* inv_perm, int64_t num_tokens,
+                       int32_t num_experts, int32_t top_k, int64_t hidden, int dtype, void* out, hkmoe_stream_t stream);
+int hkmoe_combine_rows_backward(const void* dout, const void* y, const float* topk_w, const int32_t* offsets,
+                                const int32_t* inv_perm, int64_t num_tokens, int32_t num_experts, int32_t top_k,
+                                int64_t hidden, int dtype, void* dy, float* dw, hkmoe_stream_t stream);
+int hkmoe_route_topk_backward(const float* dw, const float* topk_w, const int32_t* topk_idx, int64_t num_tokens,
+                              int32_t num_experts, int32_t top_k, float* dlogits, hkmoe_stream_t stream);
 
 /*
  * MX (microscaling) FP8: e4m3 elements with one e8m0 exponent per row and
