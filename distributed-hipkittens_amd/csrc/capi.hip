@@ -21,6 +21,7 @@
 #include "gemm_narrow.hpp"
 #include "gemm_skinny.hpp"
 #include "gemm_small.hpp"
+#include "gemm_wide.hpp"
 #include "layer_norm.hpp"
 #include "moe_kernels.hpp"
 #include "norm_quant.hpp"
@@ -190,7 +191,7 @@ std::atomic<int> g_dense_mfma{32};
 // The dense GEMM on 128x128 tiles (gemm_small.hpp): one workgroup per tile,
 // the grid a whole number of 4x8 tile blocks.
 template <bool MX, typename K>
-int launch_gemm_small(K kern, bool (&attr_set)[kMaxDevices], const SmallGemmParams& p, hipStream_t stream) {
+int launch_tile128(K kern, bool (&attr_set)[kMaxDevices], const SmallGemmParams& p, hipStream_t stream) {
   int dev = 0;
   (void)hipGetDevice(&dev);
   constexpr int lds = sm_lds_bytes(MX);
@@ -202,13 +203,23 @@ int launch_gemm_small(K kern, bool (&attr_set)[kMaxDevices], const SmallGemmPara
   }
   const int grid = ((p.m_tiles + 3) / 4) * p.nbn * 32;
   hipLaunchKernelGGL(kern, dim3(grid), dim3(kSmThreads), lds, stream, p);
-  return check_launch("gemm_fp8_small");
+  return check_launch("128x128 dense kernel");
 }
-template <bool F32OUT, bool M32, bool MX, bool EPI>
+template <bool F32OUT, bool M32, bool MX>
 int launch_gemm_small(const SmallGemmParams& p, hipStream_t stream) {
   static bool attr_set[kMaxDevices] = {false};
-  if constexpr (EPI) return launch_gemm_small<MX>(gemm_fp8_small_act<F32OUT, MX>, attr_set, p, stream);
-  else return launch_gemm_small<MX>(gemm_fp8_small<F32OUT, M32, MX>, attr_set, p, stream);
+  return launch_tile128<MX>(gemm_fp8_small<F32OUT, M32, MX>, attr_set, p, stream);
+}
+// With an epilogue: bf16 C on the FP8 instructions, fp32 C on the bf16 ones.
+template <bool MX>
+int launch_gemm_small_act(const SmallGemmParams& p, hipStream_t stream) {
+  static bool attr_set[kMaxDevices] = {false};
+  return launch_tile128<MX>(gemm_fp8_small_act<MX>, attr_set, p, stream);
+}
+template <bool MX>
+int launch_gemm_wide(const SmallGemmParams& p, hipStream_t stream) {
+  static bool attr_set[kMaxDevices] = {false};
+  return launch_tile128<MX>(gemm_fp8_wide<MX>, attr_set, p, stream);
 }
 
 template <int MF, int NF, int NW, bool MX, bool F32OUT, bool EPI>
@@ -247,7 +258,10 @@ int launch_gemm_skinny(SkinnyParams p, bool f32out, hipStream_t stream) {
 //     6.4 / 7.0, 512x2048x2048 8.2 / 10.4 (and losing: 512x4096x4096 20.8 / 17.3)
 //   128x128 against 256x256 tiles: 2048^3 13.9 / 25.6 us, 2048x4096x4096 40.8 / 48.1
 //     (MX 44.8 / 52.5), 4096^3 79 / 51, 2048x8192x1024 28.3 / 21.2
-// MX: the scaled MFMA's steps take longer in every kernel.
+// MX: the scaled MFMA's steps take longer in every kernel.  Wide (fp32 C with an epilogue: bf16 products,
+// strips or gemm_fp8_wide): the same on 60 shapes (M = 1 .. 2048, N x K = 1024 x 2048 .. 14336 x 4096, both
+// modes, a residual, launches as a graph): the pick costs 2% over the best
+// strip or tile on average, 11% at most.
 enum class DenseKernel { kStrip11, kStrip21, kStrip12, kStrip22, kStrip24, kStrip44, kTile128, kTile256 };
 
 // Tile blocks of the dense 256x256 kernel: 2^b M tiles x 32 / 2^b N tiles, one
@@ -267,7 +281,6 @@ int dense_block_log2(int64_t m, int64_t n, int64_t* rounds) {
   return best;
 }
 
-// wide: fp32 C with an epilogue, whose products run in bf16 and not in the 256x256 kernel.
 DenseKernel pick_dense(int64_t m, int64_t n, int64_t k, bool f32out, bool mx, bool wide = false) {
   const double ks = static_cast<double>(k / kBK), cus = device_cus(), nk = static_cast<double>(n) * k;
   const uint64_t um = m, un = n, ncu = device_cus();
@@ -295,23 +308,25 @@ DenseKernel pick_dense(int64_t m, int64_t n, int64_t k, bool f32out, bool mx, bo
     const uint64_t mt = (um + kSmTile - 1) / kSmTile, nt = un / kSmTile, tiles = (mt + 3) / 4 * 4 * nt;
     const double full = static_cast<double>(tiles / ncu), part = static_cast<double>(tiles % ncu);
     const double live = std::min(part, static_cast<double>(mt * nt));  // of the last round
-    const double busy = mx ? 0.58 : 0.52, idle = mx ? 0.51 : 0.40;  // per step, chip full / half full
-    const double ramp = f32out ? 4.0 : 2.6;
+    // per step, chip full / half full
+    const double busy = wide ? (mx ? 1.07 : 0.95) : mx ? 0.58 : 0.52, idle = wide ? (mx ? 0.77 : 0.69) : mx ? 0.51 : 0.40;
+    const double ramp = wide ? 5.0 : f32out ? 4.0 : 2.6;
     offer(DenseKernel::kTile128,
           1.75 + full * (ramp + ks * busy) + (part > 0 ? ramp + ks * (live <= cus / 2 ? idle : busy) : 0), 3 + nk / 2.0e6);
   }
   const struct {
     DenseKernel kern;
     int rows_log2, cols_log2, waves_log2;
-    double ramp, step;
-  } strips[] = {{DenseKernel::kStrip11, 4, 4, 3, 1.6, 0.055}, {DenseKernel::kStrip21, 5, 4, 3, 1.7, 0.075},
-                {DenseKernel::kStrip12, 4, 5, 3, 1.7, 0.075}, {DenseKernel::kStrip22, 5, 5, 3, 1.85, 0.085},
-                {DenseKernel::kStrip24, 5, 6, 2, 2.4, 0.13},  {DenseKernel::kStrip44, 6, 6, 2, 3.1, 0.215}};
+    double ramp, step, wide_ramp, wide_step;
+  } strips[] = {{DenseKernel::kStrip11, 4, 4, 3, 1.6, 0.055, 2.4, 0.060}, {DenseKernel::kStrip21, 5, 4, 3, 1.7, 0.075, 2.3, 0.088},
+                {DenseKernel::kStrip12, 4, 5, 3, 1.7, 0.075, 2.5, 0.085}, {DenseKernel::kStrip22, 5, 5, 3, 1.85, 0.085, 2.6, 0.105},
+                {DenseKernel::kStrip24, 5, 6, 2, 2.4, 0.13, 4.0, 0.18},   {DenseKernel::kStrip44, 6, 6, 2, 3.1, 0.215, 4.1, 0.32}};
   for (const auto& c : strips) {
     const uint64_t wgs = ((um + (1u << c.rows_log2) - 1) >> c.rows_log2) * (un >> c.cols_log2);
     const double rounds = static_cast<double>((wgs + ncu - 1) / ncu);
     const double steps = static_cast<double>(((k / kBK + (1 << c.waves_log2) - 1) >> c.waves_log2) << c.waves_log2);
-    offer(c.kern, (mx ? 1.6 : 1.3) + rounds * (c.ramp + steps * c.step * (mx ? 1.1 : 1.0)), 3 + nk / 5.5e6);
+    const double ramp = wide ? c.wide_ramp : c.ramp, step = wide ? c.wide_step * (mx ? 1.2 : 1.0) : c.step * (mx ? 1.1 : 1.0);
+    offer(c.kern, (mx ? 1.6 : 1.3) + rounds * (ramp + steps * step), 3 + nk / 5.5e6);
   }
   return best;
 }
@@ -362,11 +377,12 @@ int launch_dense(const void* a, const void* b, void* c, int64_t m, int64_t n, in
     q.n_tiles = static_cast<int32_t>(n / kSmTile);
     q.nbn = (q.n_tiles + 7) / 8;
     q.epi = epi;
-    if constexpr (!MX && !EPI) {
+    if constexpr (EPI) return f32out ? launch_gemm_wide<MX>(q, s) : launch_gemm_small_act<MX>(q, s);
+    if constexpr (!MX) {
       if (g_dense_mfma.load() == 32)
-        return f32out ? launch_gemm_small<true, true, false, false>(q, s) : launch_gemm_small<false, true, false, false>(q, s);
+        return f32out ? launch_gemm_small<true, true, false>(q, s) : launch_gemm_small<false, true, false>(q, s);
     }
-    return f32out ? launch_gemm_small<true, false, MX, EPI>(q, s) : launch_gemm_small<false, false, MX, EPI>(q, s);
+    return f32out ? launch_gemm_small<true, false, MX>(q, s) : launch_gemm_small<false, false, MX>(q, s);
   }
   GemmParams p{};
   p.a = static_cast<const uint8_t*>(a);
@@ -686,21 +702,30 @@ int launch_layer_norm(const LayerNormParams& p, hipStream_t s) {
     constexpr int CH = decltype(ch)::value, LANES = decltype(lanes)::value;
     constexpr int rows = kLnRowThreads / (LANES ? LANES : kLnRowThreads);  // of a workgroup
     const int threads = LANES ? kLnRowThreads : row_threads(p.cols, CH);
-    const int64_t grid = LANES ? (p.rows + rows - 1) / rows : std::min<int64_t>(p.rows, 1 << 20);
+    // whole rows: as many workgroups as the chip holds, each with its next row ahead (8192x7168 bf16 with a
+    // residual: 98 us on 512, 115 on 256, 116 on 1024)
+    const int64_t grid = std::min<int64_t>((p.rows + rows - 1) / rows, LANES ? kMaxRows : device_cus() * (2048 / threads));
     hipLaunchKernelGGL((layer_norm_kernel<F32, CH, LANES>), dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, p);
     return check_launch("layer_norm_kernel");
   });
 }
 
-// Workgroups of the gradient, each of which leaves one partial of dw and db.
+// Workgroups of the gradient, each of which leaves one partial of dw and db: as many as fill the
+// chip with some 16 waves a CU, but rows enough for each that the partials (written and read
+// again) stay a small part, and at least 256 where there are rows for them.  us for 256 / 512 / 768 / 1024:
+//   8192x7168 bf16    94 /  99 / 104 / 111     16384x1024 bf16  45 / 34 / 31 / 38
+//   4096x4096 bf16    35 /  32 /  34 /  38     1999x2560 fp32   16 / 18 / 19 / 22
 int layer_norm_parts(int64_t rows, int64_t cols) {
-  int per = 1;  // rows at a time
-  (void)with_layer_norm_shape(cols, [&](auto, auto lanes) {
+  int per = 1, each = 8, threads = 0;  // rows at a time, turns for each slot
+  (void)with_layer_norm_shape(cols, [&](auto ch, auto lanes) {
     constexpr int LANES = decltype(lanes)::value;
     per = kLnRowThreads / (LANES ? LANES : kLnRowThreads);
+    each = LANES ? 5 : 8;
+    threads = LANES ? kLnRowThreads : row_threads(cols, decltype(ch)::value);
     return HKMOE_OK;
   });
-  return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, kLnParts));
+  const int64_t fill = kLnParts * std::clamp(1024 / threads, 1, 3);
+  return static_cast<int>(std::min((rows + per - 1) / per, std::max<int64_t>(kLnParts, std::min(fill, rows / (per * each)))));
 }
 
 template <bool F32>
@@ -1837,7 +1862,7 @@ int hkmoe_layer_norm_backward(const void* dy, const void* r, const void* weight,
   auto s = static_cast<hipStream_t>(stream);
   if (rows > 0) HK_TRY(x_dtype == HKMOE_F32 ? launch_layer_norm_grad<true>(p, s) : launch_layer_norm_grad<false>(p, s));
   // without rows the sums are empty: zeros
-  hipLaunchKernelGGL(layer_norm_sum_kernel, dim3(static_cast<unsigned>((2 * cols + 63) / 64)), dim3(256), 0, s, p.part,
+  hipLaunchKernelGGL(layer_norm_sum_kernel, dim3(static_cast<unsigned>((2 * cols + 63) / 64)), dim3(kLnSumThreads), 0, s, p.part,
                      rows > 0 ? layer_norm_parts(rows, cols) : 0, p.cols, dweight, dbias, p.w_f32);
   return check_launch("layer_norm_sum_kernel");
 }

@@ -106,24 +106,27 @@ __device__ __forceinline__ float e8m0_scale(int word) {
   return __uint_as_float(e == 0 ? 0x00400000u : e << 23);
 }
 
-// Bytes 8s .. 8s + 7 of a lane's 32 K bytes of an operand row, times scale.
+// Eight e4m3 values (w0's bytes, then w1's) times scale.
+__device__ __forceinline__ bf16x8_t widen8(int w0, int w1, float scale) {
+  union {
+    bf16x2_t p[4];
+    bf16x8_t v;
+  } u;
+  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
+  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
+  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
+  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
+  return u.v;
+}
+
+// A lane's 32 K bytes of an operand row, times scale: bytes 8s .. 8s + 7 in v[s].
 struct WideFrag {
   bf16x8_t v[4];
 };
 __device__ __forceinline__ WideFrag widen(const i32x8& f, float scale) {
   WideFrag w;
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    union {
-      bf16x2_t p[4];
-      bf16x8_t v;
-    } u;
-    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * s], scale, false);
-    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * s], scale, true);
-    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * s + 1], scale, false);
-    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * s + 1], scale, true);
-    w.v[s] = u.v;
-  }
+  for (int s = 0; s < 4; ++s) w.v[s] = widen8(f[2 * s], f[2 * s + 1], scale);
   return w;
 }
 

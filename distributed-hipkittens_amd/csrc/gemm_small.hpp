@@ -62,11 +62,10 @@ static_assert(kSmAhead <= 4, "small_wait_stage covers at most 3 newer stages");
 // MX: e8m0 exponents applied by the scaled 16x16x128 MFMA (read_operand's K
 // order); a K step's words of the tile (64 per 64-row group of A and of B)
 // ride in the stage, one 4-byte-per-lane DMA per wave.
-// EPI: act(C + bias) + residual, and with fp32 C products in bf16 (epilogue.hpp).
+// EPI: act(C + bias) + residual (epilogue.hpp), bf16 C (fp32 C: gemm_wide.hpp).
 template <bool F32OUT, bool M32, bool MX, bool EPI>
 __device__ __forceinline__ void gemm_small_tile(const SmallGemmParams& p) {
-  static_assert(!(M32 && (MX || EPI)), "MX and the epilogue run on 16x16 outputs");
-  constexpr bool kWide = EPI && F32OUT;  // operands widened to bf16
+  static_assert(!(M32 && (MX || EPI)), "MX and the epilogue run on the 16x16x128 MFMA");
   constexpr int kStg = sm_stage_bytes(MX);
   constexpr int kLoads = MX ? 5 : 4;  // vector-memory instructions per wave and step
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -145,9 +144,9 @@ __device__ __forceinline__ void gemm_small_tile(const SmallGemmParams& p) {
       for (int f = 0; f < 2; ++f) bf[f] = read_frag(st + kSmOperandBytes, 32 * wn + l32, 2 * f + g32, f32);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) af[i] = read_operand<MX && !kWide>(st, 64 * wm + 16 * i + l16, lg, fx);
+      for (int i = 0; i < 4; ++i) af[i] = read_operand<MX>(st, 64 * wm + 16 * i + l16, lg, fx);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) bf[j] = read_operand<MX && !kWide>(st + kSmOperandBytes, 32 * wn + 16 * j + l16, lg, fx);
+      for (int j = 0; j < 2; ++j) bf[j] = read_operand<MX>(st + kSmOperandBytes, 32 * wn + 16 * j + l16, lg, fx);
     }
   };
 
@@ -166,24 +165,7 @@ __device__ __forceinline__ void gemm_small_tile(const SmallGemmParams& p) {
       for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   auto mma = [&](const i32x8 (&af)[4], const i32x8 (&bf)[2], const Words& w) __attribute__((always_inline)) {
-    if constexpr (kWide) {
-      // lane group lg holds K bytes 32lg .. +31 of its rows: MX block lg, whose exponents are in the
-      // lane's own words
-      const WideFrag b0 = widen(bf[0], MX ? e8m0_scale<0>(w.b) : 1.0f), b1 = widen(bf[1], MX ? e8m0_scale<1>(w.b) : 1.0f);
-      auto sub = [&](auto u) __attribute__((always_inline)) {
-        constexpr int U = decltype(u)::value;
-        const WideFrag a = widen(af[U], MX ? e8m0_scale<U>(w.a) : 1.0f);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          acc[U][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b0.v[s], a.v[s], acc[U][0], 0, 0, 0);
-          acc[U][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b1.v[s], a.v[s], acc[U][1], 0, 0, 0);
-        }
-      };
-      sub(std::integral_constant<int, 0>{});
-      sub(std::integral_constant<int, 1>{});
-      sub(std::integral_constant<int, 2>{});
-      sub(std::integral_constant<int, 3>{});
-    } else if constexpr (MX) {
+    if constexpr (MX) {
       auto sub = [&](auto u) __attribute__((always_inline)) {
         constexpr int U = decltype(u)::value;
         acc[U][0] = mfma_mx<0, U>(bf[0], af[U], acc[U][0], w.b, w.a);
@@ -325,10 +307,10 @@ template <bool F32OUT, bool M32, bool MX = false>
 __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small(SmallGemmParams p) {
   gemm_small_tile<F32OUT, M32, MX, false>(p);
 }
-// With an epilogue, on the 16x16x128 MFMA.
-template <bool F32OUT, bool MX>
+// bf16 C with an epilogue, on the 16x16x128 MFMA.
+template <bool MX>
 __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_small_act(SmallGemmParams p) {
-  gemm_small_tile<F32OUT, false, MX, true>(p);
+  gemm_small_tile<false, false, MX, true>(p);
 }
 
 }  // namespace hkmoe

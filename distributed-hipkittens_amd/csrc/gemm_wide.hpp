@@ -1,0 +1,197 @@
+// Dense product of e4m3 operands to fp32's own precision, with an epilogue: C[M,N] =
+// act((sa*sb) A[M,K] . B[N,K]^T + bias) + residual, fp32 C, per-tensor scales or MX exponents
+// (epilogue.hpp says why the products run in bf16).  For more rows than the strips of
+// gemm_skinny.hpp take.
+//
+// 128x128 output tiles and the LDS ring of gemm_small.hpp: e4m3 in LDS, widened in registers,
+// so LDS carries half the bytes of a bf16 product.  8 waves of 64x32 outputs, two per SIMD:
+// two 32x32 blocks, each eight v_mfma_f32_32x32x16_bf16 a K step, with six conversions per MFMA.
+// Those fit behind 32x32x16 (7.9 ns per 16x16x32 of work, two waves per SIMD, against 6.9 without
+// any) and not behind 16x16x32 (9.3 against 7.3).  The conversions of the next 16 K run beside
+// the MFMAs of this one, the LDS reads of step kt+1 beside step kt.  8192x4096x7168: 443 us, 1.09
+// PFLOP/s (a bf16 library product 1.4); with operands of ones 350 us, so the chip's power takes a
+// fifth.  4 waves of 64x64 outputs (fewer conversions per MFMA) and 16x16x32 MFMAs came to 1.05.
+#pragma once
+
+#include "gemm_small.hpp"
+
+namespace hkmoe {
+
+template <bool MX>
+__global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p) {
+  constexpr int kStg = sm_stage_bytes(MX);
+  constexpr int kLoads = MX ? 5 : 4;  // vector-memory instructions per wave and step
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, l32 = lane & 31, g32 = lane >> 5;
+  const int wm = wave >> 2, wn = wave & 3;  // the wave's 64 rows and 32 columns
+  const int fx = swz(l32);
+
+  // tile of this workgroup, as in gemm_small.hpp
+  const int g = gridDim.x;
+  const int vid = (g & 7) == 0 ? (blockIdx.x & 7) * (g >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  const int blk = vid >> 5, sl = vid & 31;
+  const int mt = (blk / p.nbn) * 4 + (sl & 3), nt = (blk % p.nbn) * 8 + (sl >> 2);
+  if (mt >= p.m_tiles || nt >= p.n_tiles) return;
+  const int m0 = mt * kSmTile, n0 = nt * kSmTile;
+  const int k_steps = p.k / kBK;
+
+  // DMA as in gemm_small.hpp: instruction i of wave w fills LDS rows 64i + 8w + lane/8 of an
+  // operand tile, swizzled; A rows past M repeat row M-1 (never stored).  MX: waves 0, 1 fetch the
+  // words of A's 64-row groups (one past the padded rows repeats the last), 2, 3 B's, 4-7 repeat them.
+  const int ld_row = 8 * wave + (lane >> 3);
+  const int ld_chunk = (lane & 7) ^ swz(ld_row);
+  const i32x4 a_srd = make_srd(p.a, p.a_bytes);
+  const i32x4 b_srd = make_srd(p.b, p.b_bytes);
+  int a_voff[2], b_voff[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    a_voff[i] = buf_off(min(m0 + 64 * i + ld_row, p.m - 1), p.k, ld_chunk * 16);
+    b_voff[i] = buf_off(n0 + 64 * i + ld_row, p.k, ld_chunk * 16);
+  }
+  const int ww = wave & 3;
+  const i32x4 w_srd = make_srd(ww < 2 ? p.a_scale : p.b_scale, 0xffffffffu);
+  const int w_voff = ((ww < 2 ? min(m0 + 64 * ww, p.m64 - 64) : n0 + 64 * (ww - 2)) + lane) * 4;
+  const int w_step = (ww < 2 ? p.m64 : p.n) * 4;
+  auto issue = [&](int kt) __attribute__((always_inline)) {
+    uint8_t* st = smem + (kt % kSmStages) * kStg;
+    if constexpr (MX) load_lds_4B(w_srd, st + kSmStageBytes + ww * 256, w_voff, buf_off(kt, w_step, 0));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) load_lds_16B(a_srd, st + (64 * i + 8 * wave) * kBK, a_voff[i], kt * kBK);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      load_lds_16B(b_srd, st + kSmOperandBytes + (64 * i + 8 * wave) * kBK, b_voff[i], kt * kBK);
+  };
+
+  // Fragments of a step: a[2i + h] bytes 64h + 32g32 .. +31 of row 64wm + 32i + l32, b[h] of column
+  // 32wn + l32; MX: block 2h + g32, whose exponents are bytes 2i + l32/16 (columns: 2(wn % 2) + l32/16)
+  // of word 16(2h + g32) + l32 % 16 of the 64-row group, here shifted so that i = 0 is byte 0.
+  struct Step {
+    i32x8 a[4], b[2];
+    int wa[2], wb[2];
+  };
+  const int sh_a = 8 * (l32 >> 4), sh_b = sh_a + 16 * (wn & 1);
+  auto read = [&](int kt, Step& s) __attribute__((always_inline)) {
+    const uint8_t* st = smem + (kt % kSmStages) * kStg;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (MX) {
+        const int32_t* words = reinterpret_cast<const int32_t*>(st + kSmStageBytes) + 16 * (2 * h + g32) + (l32 & 15);
+        s.wa[h] = words[wm * 64] >> sh_a;
+        s.wb[h] = words[kSmTile + (wn >> 1) * 64] >> sh_b;
+      }
+      s.b[h] = read_frag(st + kSmOperandBytes, 32 * wn + l32, 2 * h + g32, fx);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s.a[2 * i + h] = read_frag(st, 64 * wm + 32 * i + l32, 2 * h + g32, fx);
+    }
+  };
+  // A step's fragments have landed by the wait in front of the next step's reads; without this the
+  // compiler, which does not see that wait, waits for those reads as well.
+  auto landed = [&](Step& s) __attribute__((always_inline)) {
+    asm volatile("" : "+v"(s.a[0]), "+v"(s.a[1]), "+v"(s.a[2]), "+v"(s.a[3]), "+v"(s.b[0]), "+v"(s.b[1]));
+  };
+
+  f32x16 acc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  struct Ops {
+    bf16x8_t b, a0, a1;
+  };
+  auto conv = [&](const Step& s, int t) __attribute__((always_inline)) -> Ops {
+    const int h = t >> 2, q = t & 3;  // K bytes 8q .. 8q + 7 of half h's 32
+    const float sb = MX ? e8m0_scale<0>(s.wb[h]) : 1.0f, s0 = MX ? e8m0_scale<0>(s.wa[h]) : 1.0f,
+                s1 = MX ? e8m0_scale<2>(s.wa[h]) : 1.0f;
+    return Ops{widen8(s.b[h][2 * q], s.b[h][2 * q + 1], sb), widen8(s.a[h][2 * q], s.a[h][2 * q + 1], s0),
+               widen8(s.a[2 + h][2 * q], s.a[2 + h][2 * q + 1], s1)};
+  };
+  auto mma = [&](const Step& s) __attribute__((always_inline)) {
+    Ops o = conv(s, 0);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const Ops n = t < 7 ? conv(s, t + 1) : o;
+      acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.b, o.a0, acc[0], 0, 0, 0);
+      acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.b, o.a1, acc[1], 0, 0, 0);
+      o = n;
+    }
+  };
+
+  // The schedule of gemm_small.hpp: step kt's MFMAs beside the reads of kt+1 and the DMA of kt+3.
+  const int pre = min(kSmAhead, k_steps);
+  for (int kt = 0; kt < pre; ++kt) issue(kt);
+  small_wait_stage<kLoads>(pre - 1);
+  Step s0, s1;
+  read(0, s0);
+  auto step = [&](int kt, Step& cur, Step& next) __attribute__((always_inline)) {
+    if (kt + kSmAhead < k_steps) issue(kt + kSmAhead);
+    small_wait_stage<kLoads>(min(kSmAhead - 1, k_steps - 1 - (kt + 1)));
+    landed(cur);
+    read(kt + 1, next);
+    __builtin_amdgcn_sched_barrier(0);
+    mma(cur);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step_full = [&](int kt, Step& cur, Step& next) __attribute__((always_inline)) {
+    issue(kt + kSmAhead);
+    small_wait_stage<kLoads>(kSmAhead - 1);
+    landed(cur);
+    read(kt + 1, next);
+    __builtin_amdgcn_sched_barrier(0);
+    mma(cur);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int kt = 0;
+  for (; kt + 1 + kSmAhead < k_steps; kt += 2) {
+    step_full(kt, s0, s1);
+    step_full(kt + 1, s1, s0);
+  }
+  for (; kt + 2 < k_steps; kt += 2) {
+    step(kt, s0, s1);
+    step(kt + 1, s1, s0);
+  }
+
+  // lane: rows m0 + 64wm + 32i + l32, columns ecol + 8j .. +3 in registers 4j .. 4j+3 of acc[i].  The residual
+  // is loaded in front of the last products, into the registers of the next fragments.
+  const int ecol = n0 + 32 * wn + 4 * g32;
+  f32x4 res[2][4];
+  auto load_res = [&]() __attribute__((always_inline)) {
+    if (p.epi.residual == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // rows past M repeat the last one (never stored)
+      const int64_t at = static_cast<int64_t>(min(m0 + 64 * wm + 32 * i + l32, p.m - 1)) * p.n + ecol;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) res[i][j] = load4(p.epi.residual, at + 8 * j, true);
+    }
+  };
+  if (kt + 1 < k_steps) {
+    step(kt, s0, s1);
+    load_res();
+    mma(s1);
+  } else {
+    load_res();
+    mma(s0);
+  }
+
+  const float tens = MX ? 1.0f : (p.a_scale ? p.a_scale[0] : 1.0f) * (p.b_scale ? p.b_scale[0] : 1.0f);
+  f32x4 bias[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bias[j] = epilogue_bias(p.epi, ecol + 8 * j);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = m0 + 64 * wm + 32 * i + l32;
+    if (r < p.m) {
+      float* dst = static_cast<float*>(p.c) + static_cast<int64_t>(r) * p.n + ecol;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 v{acc[i][4 * j] * tens, acc[i][4 * j + 1] * tens, acc[i][4 * j + 2] * tens, acc[i][4 * j + 3] * tens};
+        v = activate(v + bias[j], p.epi.act);
+        if (p.epi.residual != nullptr) v = v + res[i][j];
+        *reinterpret_cast<f32x4*>(dst + 8 * j) = v;
+      }
+    }
+  }
+}
+
+}  // namespace hkmoe

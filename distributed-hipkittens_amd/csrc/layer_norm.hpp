@@ -21,7 +21,7 @@
 
 namespace hkmoe {
 
-constexpr int kLnParts = 256;                                       // workgroups of the gradient, at most
+constexpr int kLnParts = 256;                                       // workgroups of the gradient, see layer_norm_parts
 constexpr int kLnRowThreads = 256;                                  // of a workgroup that has several rows
 constexpr int kLnMaxCols = 2 * kNormMaxThreads * kNormChunk;        // 16384
 // Threads of a workgroup, at most.  A row's chunks fit 1024 threads to 8192 columns; wider rows take
@@ -67,74 +67,142 @@ __device__ __forceinline__ int ln_col(int c) {
   return (c * w + l) * kNormChunk;
 }
 
+// Sums of the 16 lanes of a DPP row, the same on each (quad pairs, quad swap, half-row and row
+// mirrors), without the LDS crossbar of a shuffle.
+template <int CTRL, typename T>
+__device__ __forceinline__ T dpp_swap(T v) {
+  if constexpr (sizeof(T) == 8) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
+    const uint32_t l = __builtin_amdgcn_update_dpp(lo, lo, CTRL, 0xf, 0xf, false), h = __builtin_amdgcn_update_dpp(hi, hi, CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(T, (static_cast<uint64_t>(h) << 32) | l);
+  } else {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(u, u, CTRL, 0xf, 0xf, false));
+  }
+}
+template <typename T>
+__device__ __forceinline__ T dpp_row_sum(T v) {
+  v += dpp_swap<0xB1>(v);
+  v += dpp_swap<0x4E>(v);
+  v += dpp_swap<0x141>(v);
+  return v + dpp_swap<0x140>(v);
+}
+template <typename T>
+__device__ __forceinline__ T lane_value(T v, int lane) {
+  if constexpr (sizeof(T) == 8) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(u), lane), hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(u >> 32), lane);
+    return __builtin_bit_cast(T, (static_cast<uint64_t>(hi) << 32) | lo);
+  } else {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(uint32_t, v), lane));
+  }
+}
+
 // Two sums over a row's threads, the same on each of them.  `red` (LANES 0) holds two
 // values per wave and is free again after the caller's next barrier.
 template <int LANES, typename T>
 __device__ __forceinline__ void row_sums(T& a, T& b, T (*red)[2]) {
-#pragma unroll
-  for (int o = (LANES == 0 ? 64 : LANES) / 2; o >= 1; o >>= 1) {
-    a += __shfl_xor(a, o, kWave);
-    b += __shfl_xor(b, o, kWave);
+  a = dpp_row_sum(a);
+  b = dpp_row_sum(b);
+  if constexpr (LANES == 32) {
+    a += __shfl_xor(a, 16, kWave);
+    b += __shfl_xor(b, 16, kWave);
+  } else if constexpr (LANES != 16) {  // whole waves: the DPP rows' sums through scalar registers
+    a = (lane_value(a, 0) + lane_value(a, 16)) + (lane_value(a, 32) + lane_value(a, 48));
+    b = (lane_value(b, 0) + lane_value(b, 16)) + (lane_value(b, 32) + lane_value(b, 48));
   }
   if constexpr (LANES == 0) {
-    const int waves = blockDim.x / kWave;
+    const int waves = blockDim.x / kWave, l = threadIdx.x & 15;  // at most 16
     if ((threadIdx.x & 63) == 0) {
       red[threadIdx.x >> 6][0] = a;
       red[threadIdx.x >> 6][1] = b;
     }
     __syncthreads();
-    a = b = 0;
-    for (int w = 0; w < waves; ++w) {
-      a += red[w][0];
-      b += red[w][1];
-    }
+    a = l < waves ? red[l][0] : T(0);
+    b = l < waves ? red[l][1] : T(0);
+    a = dpp_row_sum(a);
+    b = dpp_row_sum(b);
   }
 }
 
+// 1 / sqrt(v): the hardware's estimate (about 2^-24 off) and one Newton step, 2^-46.  v at least 2^-260,
+// below which the caller's fp32 result is at its largest value anyway.
+__device__ __forceinline__ double inv_sqrt(double v) {
+  v = v < 0x1p-260 ? 0x1p-260 : v;  // a NaN stays
+  const double y = __builtin_amdgcn_rsq(v);
+  return y * __builtin_fma(-0.5 * v * y, y, 1.5);
+}
+
+// Eight values as they are stored, so that rows loaded ahead cost half the registers in bf16.
+template <bool F32>
+struct Raw8 {
+  uint4 u;
+  __device__ __forceinline__ void load(const void* p, int64_t i) { u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i); }
+  __device__ __forceinline__ F8v get() const { return unpack_bf16x8(u); }
+};
+template <>
+struct Raw8<true> {
+  F8v u;
+  __device__ __forceinline__ void load(const void* p, int64_t i) { u = load8<true>(p, i); }
+  __device__ __forceinline__ F8v get() const { return u; }
+};
+
+// Rows blockIdx.x * rows per workgroup, + gridDim.x * that, ...; the next row's loads go out before
+// the sums of this one are waited for.
 template <bool F32, int CH, int LANES>
 __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_kernel(LayerNormParams p) {
   __shared__ double red[2][LANES == 0 ? kNormMaxThreads / kWave : 1][2];
   const int cols = p.cols;
-  int turn = 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * ln_rows<LANES>();
   int64_t row = static_cast<int64_t>(blockIdx.x) * ln_rows<LANES>() + ln_slot<LANES>();
-  for (; row < p.rows; row += step, turn ^= 1) {
-    const int64_t base = row * cols;
-    F8v r[CH];
-    float first = F32 ? static_cast<const float*>(p.x)[base]
-                      : bf16_bits_to_f32(static_cast<const uint16_t*>(p.x)[base]);
-    if (p.residual != nullptr)
-      first += F32 ? static_cast<const float*>(p.residual)[base]
-                   : bf16_bits_to_f32(static_cast<const uint16_t*>(p.residual)[base]);
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int j = ln_col<LANES>(c);
-      if (j < cols) r[c] = load8<F32>(p.x, base + j);
-    }
-    if (p.residual != nullptr) {
+  const double inv_n = 1.0 / static_cast<double>(cols);
+  Raw8<F32> x[CH], o[CH];
+  float first = 0.0f;
+  auto load = [&](int64_t at) __attribute__((always_inline)) {
+    if (at < p.rows) {
+      const int64_t base = at * cols;
+      first = F32 ? static_cast<const float*>(p.x)[base] : bf16_bits_to_f32(static_cast<const uint16_t*>(p.x)[base]);
+      if (p.residual != nullptr)
+        first += F32 ? static_cast<const float*>(p.residual)[base]
+                     : bf16_bits_to_f32(static_cast<const uint16_t*>(p.residual)[base]);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int j = ln_col<LANES>(c);
         if (j < cols) {
-          const F8v o = load8<F32>(p.residual, base + j);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) r[c].v[i] += o.v[i];
-          if constexpr (!F32) r[c] = unpack_bf16x8(pack_bf16x8(r[c]));
+          x[c].load(p.x, base + j);
+          if (p.residual != nullptr) o[c].load(p.residual, base + j);
         }
       }
     }
+  };
+  load(row);
+  int turn = 0;
+  // LANES 0: the whole workgroup has one row, so the barriers are met together
+  for (; row < p.rows; row += step, turn ^= 1) {
+    const int64_t base = row * cols;
+    const float near = first;
+    F8v r[CH];
     double s1 = 0.0, s2 = 0.0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if (ln_col<LANES>(c) < cols) {
+        r[c] = x[c].get();
+        if (p.residual != nullptr) {
+          const F8v a = o[c].get();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) r[c].v[i] += a.v[i];
+          if constexpr (!F32) r[c] = unpack_bf16x8(pack_bf16x8(r[c]));
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const double d = static_cast<double>(r[c].v[i]) - static_cast<double>(first);
+          const double d = static_cast<double>(r[c].v[i]) - static_cast<double>(near);
           s1 += d;
           s2 = __builtin_fma(d, d, s2);
         }
       }
     }
+    load(row + step);
     // residual_out may be x or residual: every thread has read what it will overwrite, and `first`,
     // which all of them read, is overwritten after the barrier below (or by the same wave)
     row_sums<LANES>(s1, s2, red[turn]);
@@ -145,11 +213,10 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_kernel(Layer
         if (j < cols) store8<F32>(p.residual_out, base + j, r[c]);
       }
     }
-    const double inv_n = 1.0 / static_cast<double>(cols);
-    const double d1 = s1 * inv_n, mean = d1 + static_cast<double>(first), var = s2 * inv_n - d1 * d1;
+    const double d1 = s1 * inv_n, mean = d1 + static_cast<double>(near), var = s2 * inv_n - d1 * d1;
     const float mh = static_cast<float>(mean), ml = static_cast<float>(mean - static_cast<double>(mh));
     // past fp32 (constant rows with eps below 2^-256) the largest one, so that zeros stay zeros
-    const float inv = static_cast<float>(1.0 / sqrt((var > 0.0 ? var : var * 0.0) + p.eps)), most = 0x1.fffffep127f;
+    const float inv = static_cast<float>(inv_sqrt((var > 0.0 ? var : var * 0.0) + p.eps)), most = 0x1.fffffep127f;
     const float rstd = inv > most ? most : inv;
     if ((LANES == 0 ? threadIdx.x : threadIdx.x % LANES) == 0) p.stats[row] = f32x4{mh, ml, rstd, 0.0f};
 #pragma unroll
@@ -167,20 +234,6 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_kernel(Layer
     }
   }
 }
-
-// Eight values as they are stored, so that rows loaded ahead cost half the registers in bf16.
-template <bool F32>
-struct Raw8 {
-  uint4 u;
-  __device__ __forceinline__ void load(const void* p, int64_t i) { u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i); }
-  __device__ __forceinline__ F8v get() const { return unpack_bf16x8(u); }
-};
-template <>
-struct Raw8<true> {
-  F8v u;
-  __device__ __forceinline__ void load(const void* p, int64_t i) { u = load8<true>(p, i); }
-  __device__ __forceinline__ F8v get() const { return u; }
-};
 
 // Rows blockIdx.x * rows per workgroup, + gridDim.x * that, ...; the next row is loaded
 // before the sums of this one are waited for (kAhead).
@@ -300,24 +353,28 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_grad_kernel(
   }
 }
 
-// The partials of `count` workgroups added in order: 64 values per workgroup of 256
-// threads, each wave a quarter of the partials.
-__global__ __launch_bounds__(256) void layer_norm_sum_kernel(const float* __restrict__ part, int count, int cols,
-                                                             void* dw, void* db, int w_f32) {
-  __shared__ double red[4][64];
+// The partials of `count` workgroups added in order, in 64 bits: 64 values per workgroup, each of
+// its 16 waves a sixteenth of the partials (16 loads of a lane in flight: 256 partials in one round).
+constexpr int kLnSumThreads = 1024;
+__global__ __launch_bounds__(kLnSumThreads) void layer_norm_sum_kernel(const float* __restrict__ part, int count, int cols,
+                                                                       void* dw, void* db, int w_f32) {
+  constexpr int kWaves = kLnSumThreads / 64;
+  __shared__ double red[kWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = blockIdx.x * 64 + lane;
   const int64_t width = 2 * static_cast<int64_t>(cols);
   double s = 0.0;
   if (i < width) {
-    const int b0 = count * wave / 4, b1 = count * (wave + 1) / 4;
-#pragma unroll 8
+    const int b0 = count * wave / kWaves, b1 = count * (wave + 1) / kWaves;
+#pragma unroll 16
     for (int b = b0; b < b1; ++b) s += static_cast<double>(part[b * width + i]);
   }
   red[wave][lane] = s;
   __syncthreads();
   if (wave != 0 || i >= width) return;
-  const float v = static_cast<float>((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) s += red[w][lane];
+  const float v = static_cast<float>(s);
   void* to = i < cols ? dw : db;
   const int j = i < cols ? i : i - cols;
   if (to == nullptr) return;

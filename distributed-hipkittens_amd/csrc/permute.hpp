@@ -246,17 +246,27 @@ __global__ __launch_bounds__(kMoveThreads) void permute_rows_kernel(const uint8_
   }
 }
 
+// Eight values as they are stored, loaded non-temporally; unpacked where they are used, or the
+// loads of several rows would wait for each other.
 template <bool F32>
-__device__ __forceinline__ F8v load8_nt(const void* p, int64_t i) {
-  if constexpr (F32) {
-    const float* s = static_cast<const float*>(p) + i;
-    const uint4 a = ld_nt16(s), b = ld_nt16(s + 4);
-    return F8v{{__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z), __uint_as_float(a.w), __uint_as_float(b.x),
-                __uint_as_float(b.y), __uint_as_float(b.z), __uint_as_float(b.w)}};
-  } else {
-    return unpack_bf16x8(ld_nt16(static_cast<const uint16_t*>(p) + i));
+struct Rows8 {
+  uint4 u[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    if constexpr (F32) {
+      u[0] = ld_nt16(static_cast<const float*>(p) + i);
+      u[1] = ld_nt16(static_cast<const float*>(p) + i + 4);
+    } else {
+      u[0] = ld_nt16(static_cast<const uint16_t*>(p) + i);
+    }
   }
-}
+  __device__ __forceinline__ F8v get() const {
+    if constexpr (F32)
+      return F8v{{__uint_as_float(u[0].x), __uint_as_float(u[0].y), __uint_as_float(u[0].z), __uint_as_float(u[0].w),
+                  __uint_as_float(u[1].x), __uint_as_float(u[1].y), __uint_as_float(u[1].z), __uint_as_float(u[1].w)}};
+    else
+      return unpack_bf16x8(u[0]);
+  }
+};
 template <bool F32>
 __device__ __forceinline__ void store8_nt(void* p, int64_t i, const F8v& f) {
   if constexpr (F32) {
@@ -284,18 +294,18 @@ __global__ __launch_bounds__(kMoveThreads) void combine_rows_kernel(const void* 
     for (int c = threadIdx.x * 8; c < hidden; c += blockDim.x * 8) {
       F8v acc{};
       for (int j0 = 0; j0 < top_k; j0 += 8) {
-        F8v v[8];
+        Rows8<F32> v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          v[u] = F8v{};
-          if (j0 + u < top_k && static_cast<unsigned>(at[j0 + u]) < live) v[u] = load8_nt<F32>(y, static_cast<int64_t>(at[j0 + u]) * hidden + c);
+          if (j0 + u < top_k && static_cast<unsigned>(at[j0 + u]) < live) v[u].load(y, static_cast<int64_t>(at[j0 + u]) * hidden + c);
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           if (j0 + u < top_k && static_cast<unsigned>(at[j0 + u]) < live) {
             const float s = w != nullptr ? wt[j0 + u] : 1.0f;
+            const F8v r = v[u].get();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc.v[i] = __builtin_fmaf(s, v[u].v[i], acc.v[i]);
+            for (int i = 0; i < 8; ++i) acc.v[i] = __builtin_fmaf(s, r.v[i], acc.v[i]);
           }
         }
       }
@@ -324,12 +334,11 @@ __global__ __launch_bounds__(kMoveThreads) void combine_grad_kernel(const void* 
 #pragma unroll
       for (int u = 0; u < kAt; ++u) dot[u] = 0.0f;
       for (int c = threadIdx.x * 8; c < hidden; c += blockDim.x * 8) {
-        F8v v[kAt];
+        Rows8<F32> v[kAt];
         const F8v d = load8<F32>(dout, t * hidden + c);
 #pragma unroll
         for (int u = 0; u < kAt; ++u) {
-          v[u] = F8v{};
-          if (j0 + u < top_k && static_cast<unsigned>(at[j0 + u]) < live) v[u] = load8_nt<F32>(y, static_cast<int64_t>(at[j0 + u]) * hidden + c);
+          if (j0 + u < top_k && static_cast<unsigned>(at[j0 + u]) < live) v[u].load(y, static_cast<int64_t>(at[j0 + u]) * hidden + c);
         }
 #pragma unroll
         for (int u = 0; u < kAt; ++u) {
@@ -338,9 +347,10 @@ __global__ __launch_bounds__(kMoveThreads) void combine_grad_kernel(const void* 
             const float s = wt[j0 + u];
             F8v o{};
             if (in) {
+              const F8v r = v[u].get();
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                dot[u] = __builtin_fmaf(d.v[i], v[u].v[i], dot[u]);
+                dot[u] = __builtin_fmaf(d.v[i], r.v[i], dot[u]);
                 o.v[i] = s * d.v[i];
               }
             }

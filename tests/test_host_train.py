@@ -204,8 +204,8 @@ for line in log(): print(line)
 
 
 def test_epilogue_shapes_reach_every_kernel(fake):
-    """The GPU test's shapes run on every strip, on 128x128 tiles and, with bf16 C, on 256x256 ones; with fp32 C
-    never on those, whose products are the FP8 instructions'.  (strips: fp32 output, epilogue)"""
+    """The GPU test's shapes run on every strip, with bf16 C on 128x128 and 256x256 tiles of the FP8
+    instructions, with fp32 C on the tiles that widen the operands.  (strips: MX, fp32 output, epilogue)"""
     for mx in (0, 1):
         for f32 in (0, 1):
             out = hip_host.run(fake, LAUNCH + f"""
@@ -214,12 +214,12 @@ for line in log(): print(line)
 """)
             got = set()
             for line in out:
-                m = re.match(r"launch hkmoe::gemm_fp8_(skinny<(\d), *_?(\d), *_?(\d), *_?(\w+), *_?(\w+), *_?(\w+)>|small_act|persistent)", line)
+                m = re.match(r"launch hkmoe::gemm_fp8_(skinny<(\d), *_?(\d), *_?(\d), *_?(\w+), *_?(\w+), *_?(\w+)>|small_act|wide|persistent)", line)
                 if m.group(2):
                     assert m.group(5, 6, 7) == tuple("true" if v else "false" for v in (mx, f32, 1)), line
                 got.add(f"strip {m.group(2)}x{m.group(3)}" if m.group(2) else m.group(1))
-            want = {"strip 1x1", "strip 2x1", "strip 1x2", "strip 2x2", "strip 2x4", "strip 4x4", "small_act"}
-            assert got == want | (set() if f32 else {"persistent"}), (mx, f32, got)
+            want = {"strip 1x1", "strip 2x1", "strip 1x2", "strip 2x2", "strip 2x4", "strip 4x4"}
+            assert got == want | ({"wide"} if f32 else {"small_act", "persistent"}), (mx, f32, got)
 
 
 def test_small_batches_sort_in_one_launch(fake):
