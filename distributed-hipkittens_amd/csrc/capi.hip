@@ -741,6 +741,14 @@ int launch_layer_norm_grad(const LayerNormGradParams& p, hipStream_t s) {
 // ---------------------------------------------------------------------------
 // tokens by expert
 // ---------------------------------------------------------------------------
+// One launch sorts and copies where its comparisons (each token's workgroup passes over all slots, once per
+// four of its own) are few.  us, three launches / one: 64 tokens x 8, rows of 8 KiB 9.3 / 4.6, 777 x 4,
+// 4 KiB 11.1 / 6.5, 2048 x 2, 8 KiB 15.5 / 10.5; past the limit 4096 x 1, 2 KiB 11.2 / 14.8, 1024 x 8, 512 bytes
+// 10.7 / 15.8.
+bool sort_in_one(int64_t tokens, int64_t top_k) {
+  return tokens * (tokens * top_k) * ((top_k + kSortAtOnce - 1) / kSortAtOnce) <= 1 << 23;
+}
+
 int64_t sort_span(int64_t slots) {  // slots of a sorting workgroup
   const int64_t chunks = (slots + kSortSlots - 1) / kSortSlots;
   return (chunks + kSortBlocks - 1) / kSortBlocks * kSortSlots;
@@ -1886,7 +1894,7 @@ size_t hkmoe_permute_workspace_size(int64_t num_tokens, int32_t num_experts, int
   if (num_tokens <= 0 || num_tokens > kMaxRows || top_k < 1 || top_k > kMaxTopK || num_experts < 1 || num_experts > kMaxExperts)
     return 0;
   const int64_t slots = num_tokens * top_k;
-  return slots <= kSortSmall ? 0 : align256(static_cast<size_t>(sort_blocks(slots)) * (num_experts + 1) * sizeof(int32_t));
+  return sort_in_one(num_tokens, top_k) ? 0 : align256(static_cast<size_t>(sort_blocks(slots)) * (num_experts + 1) * sizeof(int32_t));
 }
 
 int hkmoe_permute(const void* x, const int32_t* ids, int64_t num_tokens, int32_t num_experts, int32_t top_k, int64_t hidden,
@@ -1907,9 +1915,11 @@ int hkmoe_permute(const void* x, const int32_t* ids, int64_t num_tokens, int32_t
     return fail(HKMOE_ERR_WORKSPACE, "permute: workspace needs %zu bytes, 16-byte aligned", need);
   const int64_t slots = num_tokens * top_k, row_bytes = hidden * (dtype == HKMOE_E4M3 ? 1 : dtype == HKMOE_BF16 ? 2 : 4);
   auto s = static_cast<hipStream_t>(stream);
-  if (slots <= kSortSmall) {
-    hipLaunchKernelGGL(permute_small_kernel, dim3(static_cast<unsigned>(slots + 1)), dim3(kSortThreads), 0, s, ids,
-                       static_cast<int>(slots), num_experts, top_k, static_cast<const uint8_t*>(x), row_bytes,
+  if (sort_in_one(num_tokens, top_k)) {
+    // the slots of a token shared among workgroups while those are few
+    const int parts = static_cast<int>(std::clamp<int64_t>(num_tokens == 0 ? 1 : 512 / num_tokens, 1, top_k));
+    hipLaunchKernelGGL(permute_small_kernel, dim3(static_cast<unsigned>(num_tokens * parts + 1)), dim3(kSortThreads), 0, s, ids,
+                       static_cast<int>(slots), num_experts, top_k, parts, static_cast<const uint8_t*>(x), row_bytes,
                        static_cast<uint8_t*>(xp), offsets, perm, inv_perm);
     return check_launch("permute_small_kernel");
   }

@@ -79,14 +79,6 @@ __device__ __forceinline__ f32x4 epilogue_bias(const EpilogueArgs& e, int col) {
   return e.bias != nullptr ? load4(e.bias, col, e.bias_f32) : f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
-// act(z + bias) + residual of the element at `at` (row * N + column).
-template <bool F32OUT>
-__device__ __forceinline__ f32x4 epilogue4(const EpilogueArgs& e, f32x4 z, f32x4 bias, int64_t at) {
-  z = activate(z + bias, e.act);
-  if (e.residual != nullptr) z = z + load4(e.residual, at, F32OUT);
-  return z;
-}
-
 // ---------------------------------------------------------------------------
 // Products to fp32's own precision, for fp32 C.  The FP8 matrix instructions line up the
 // products of eight neighbouring K to the largest of them and drop what is below 2^-16 of

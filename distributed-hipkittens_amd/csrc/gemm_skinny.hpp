@@ -166,6 +166,24 @@ __global__ __launch_bounds__(NW * 64, 1) void gemm_fp8_skinny(SkinnyParams p) {
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // EPI: the bias and the residual of the values that this thread stores, on their way first of all
+  // (read at the end, they cost 1 us of latency; rows past M repeat the last one)
+  constexpr int kOuts = (kRows * kCols / 4 + NW * 64 - 1) / (NW * 64);
+  using Stored = std::conditional_t<F32OUT, f32x4, uint2>;
+  Stored res[kOuts];
+  f32x4 bias[kOuts];
+  if constexpr (EPI) {
+#pragma unroll
+    for (int u = 0; u < kOuts; ++u) {
+      const int idx = min(tid + u * NW * 64, kRows * kCols / 4 - 1), r = min(m0 + idx / (kCols / 4), p.m - 1);
+      const int col = n0 + (idx % (kCols / 4)) * 4;
+      bias[u] = epilogue_bias(p.epi, col);
+      if (p.epi.residual != nullptr)
+        res[u] = *reinterpret_cast<const Stored*>(static_cast<const uint8_t*>(p.epi.residual) +
+                                                  (static_cast<int64_t>(r) * p.n + col) * (F32OUT ? 4 : 2));
+    }
+  }
+
   uint8_t* ring = smem + wave * D * kStep;
   // Step i of this wave into its slot.  Steps past the last one go through
   // empty descriptors (no memory traffic), so the loads in flight stay a
@@ -264,15 +282,20 @@ __global__ __launch_bounds__(NW * 64, 1) void gemm_fp8_skinny(SkinnyParams p) {
     for (int j = 0; j < NF; ++j)
       *reinterpret_cast<f32x4*>(part + (wave * kRows + 16 * i + l16) * kLd + 16 * j + 4 * lg) = acc[i][j];
   __syncthreads();
-  for (int idx = tid; idx < kRows * kCols / 4; idx += NW * 64) {
+#pragma unroll
+  for (int u = 0; u < kOuts; ++u) {
+    const int idx = tid + u * NW * 64;
     const int r = idx / (kCols / 4), cc = (idx % (kCols / 4)) * 4;
-    if (m0 + r >= p.m) continue;
+    if (idx >= kRows * kCols / 4 || m0 + r >= p.m) continue;
     f32x4 s = *reinterpret_cast<const f32x4*>(part + r * kLd + cc);
 #pragma unroll
     for (int w = 1; w < NW; ++w) s += *reinterpret_cast<const f32x4*>(part + (w * kRows + r) * kLd + cc);
     const int64_t at = static_cast<int64_t>(m0 + r) * p.n + n0 + cc;
     s = f32x4{s.x * tens, s.y * tens, s.z * tens, s.w * tens};
-    if constexpr (EPI) s = epilogue4<F32OUT>(p.epi, s, epilogue_bias(p.epi, n0 + cc), at);
+    if constexpr (EPI) {
+      s = activate(s + bias[u], p.epi.act);
+      if (p.epi.residual != nullptr) s = s + as_f32x4(res[u]);
+    }
     if constexpr (F32OUT) {
       *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + at) = s;
     } else {

@@ -238,6 +238,22 @@ __device__ __forceinline__ void gemm_small_tile(const SmallGemmParams& p) {
   }
   if (kt < k_steps) step(kt, af0, bf0, w0, af1, bf1, w1);
 
+  // EPI: the residual's rows, loaded as the output's are stored (whole rows; rows past M repeat the last one)
+  constexpr int kRowChunks = kSmTile * 16 / kSmThreads;
+  i32x4 rv[kRowChunks];
+  bool has_res = false;
+  if constexpr (EPI) {
+    has_res = p.epi.residual != nullptr;
+    if (has_res) {
+#pragma unroll
+      for (int u = 0; u < kRowChunks; ++u) {
+        const int idx = tid + kSmThreads * u, r = min(m0 + (idx >> 4), p.m - 1), c = idx & 15;
+        rv[u] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(static_cast<const uint16_t*>(p.epi.residual) +
+                                                                          static_cast<int64_t>(r) * p.n + n0 + c * 8));
+      }
+    }
+  }
+
   // ---- epilogue: lane holds row 64wm + 16i + l16, columns 32wn + 16j + 4lg .. +3
   // (M32: row 64wm + 32bi + l32, columns 32wn + 8q + 4g32 .. +3 in registers
   // 4q .. 4q+3 of acc32[bi])
@@ -257,11 +273,11 @@ __device__ __forceinline__ void gemm_small_tile(const SmallGemmParams& p) {
 #pragma unroll
     for (int j = 0; j < kColSteps; ++j) bias[j] = epilogue_bias(p.epi, ecol + kColStep * j);
   }
-  // the finished values of row step i (row r < M of C), columns j
-  auto finish = [&](int i, int j, int r) __attribute__((always_inline)) -> f32x4 {
+  // act(z + bias) of row step i, columns j
+  auto finish = [&](int i, int j) __attribute__((always_inline)) -> f32x4 {
     f32x4 v = value(i, j);
     v = f32x4{v.x * tens, v.y * tens, v.z * tens, v.w * tens};
-    if constexpr (EPI) v = epilogue4<F32OUT>(p.epi, v, bias[j], static_cast<int64_t>(r) * p.n + ecol + kColStep * j);
+    if constexpr (EPI) v = activate(v + bias[j], p.epi.act);
     return v;
   };
   if constexpr (F32OUT) {
@@ -271,24 +287,34 @@ __device__ __forceinline__ void gemm_small_tile(const SmallGemmParams& p) {
       if (r < p.m) {
         float* dst = static_cast<float*>(p.c) + static_cast<int64_t>(r) * p.n + ecol;
 #pragma unroll
-        for (int j = 0; j < kColSteps; ++j) *reinterpret_cast<f32x4*>(dst + kColStep * j) = finish(i, j, r);
+        for (int j = 0; j < kColSteps; ++j) *reinterpret_cast<f32x4*>(dst + kColStep * j) = finish(i, j);
       }
     }
   } else {
     // staged in LDS (rows of 256 bytes = 16 chunks, chunk c of row r at slot
     // c ^ (r & 15)) and stored as 16-byte chunks covering whole rows
     __syncthreads();  // every wave is done with the ring
+    if constexpr (EPI) {
+      // the residual first: each lane finds its values at the places that it writes its output to
+      if (has_res) {
+#pragma unroll
+        for (int u = 0; u < kRowChunks; ++u) {
+          const int idx = tid + kSmThreads * u, r = idx >> 4, c = idx & 15;
+          *reinterpret_cast<i32x4*>(smem + r * 256 + ((c ^ (r & 15)) << 4)) = rv[u];
+        }
+        __syncthreads();
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kRowSteps; ++i) {
       const int r = 64 * wm + (64 / kRowSteps) * i + er;
 #pragma unroll
       for (int j = 0; j < kColSteps; ++j) {
         const int c = 4 * wn + (M32 ? j : 2 * j + (lg >> 1)), half = M32 ? g32 : (lg & 1);
-        const f32x4 a = finish(i, j, min(m0 + r, p.m - 1));  // rows past M repeat the last one, and are not stored
-        uint2 v;
-        v.x = pack_bf16x2(a.x, a.y);
-        v.y = pack_bf16x2(a.z, a.w);
-        *reinterpret_cast<uint2*>(smem + r * 256 + ((c ^ (r & 15)) << 4) + half * 8) = v;
+        f32x4 a = finish(i, j);
+        uint2* at = reinterpret_cast<uint2*>(smem + r * 256 + ((c ^ (r & 15)) << 4) + half * 8);
+        if (has_res) a = a + as_f32x4(*at);
+        *at = uint2{pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w)};
       }
     }
     __syncthreads();

@@ -8,14 +8,17 @@
 // two 32x32 blocks, each eight v_mfma_f32_32x32x16_bf16 a K step, with six conversions per MFMA.
 // Those fit behind 32x32x16 (7.9 ns per 16x16x32 of work, two waves per SIMD, against 6.9 without
 // any) and not behind 16x16x32 (9.3 against 7.3).  The conversions of the next 16 K run beside
-// the MFMAs of this one, the LDS reads of step kt+1 beside step kt.  8192x4096x7168: 443 us, 1.09
-// PFLOP/s (a bf16 library product 1.4); with operands of ones 350 us, so the chip's power takes a
-// fifth.  4 waves of 64x64 outputs (fewer conversions per MFMA) and 16x16x32 MFMAs came to 1.05.
+// the MFMAs of this one, the LDS reads of step kt+1 beside step kt.  8192x4096x7168: 418 us, 1.15
+// PFLOP/s (a bf16 library product 1.4); before the last steps 443 us, and 350 with operands of ones, so
+// the chip's power takes a fifth.  4 waves of 64x64 outputs (fewer conversions per MFMA) and 16x16x32
+// MFMAs came to 1.05 where this kernel had 1.09.
 #pragma once
 
 #include "gemm_small.hpp"
 
 namespace hkmoe {
+
+static_assert(kSmTile * kSmTile * 4 <= sm_lds_bytes(false), "the output tile is staged in the ring");
 
 template <bool MX>
 __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p) {
@@ -72,18 +75,24 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
     int wa[2], wb[2];
   };
   const int sh_a = 8 * (l32 >> 4), sh_b = sh_a + 16 * (wn & 1);
+  auto read_a = [&](const uint8_t* st, int i, int h, Step& s) __attribute__((always_inline)) {
+    s.a[2 * i + h] = read_frag(st, 64 * wm + 32 * i + l32, 2 * h + g32, fx);
+  };
+  auto read_b = [&](const uint8_t* st, int h, Step& s) __attribute__((always_inline)) {
+    if constexpr (MX) {
+      const int32_t* words = reinterpret_cast<const int32_t*>(st + kSmStageBytes) + 16 * (2 * h + g32) + (l32 & 15);
+      s.wa[h] = words[wm * 64] >> sh_a;
+      s.wb[h] = words[kSmTile + (wn >> 1) * 64] >> sh_b;
+    }
+    s.b[h] = read_frag(st + kSmOperandBytes, 32 * wn + l32, 2 * h + g32, fx);
+  };
   auto read = [&](int kt, Step& s) __attribute__((always_inline)) {
     const uint8_t* st = smem + (kt % kSmStages) * kStg;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if constexpr (MX) {
-        const int32_t* words = reinterpret_cast<const int32_t*>(st + kSmStageBytes) + 16 * (2 * h + g32) + (l32 & 15);
-        s.wa[h] = words[wm * 64] >> sh_a;
-        s.wb[h] = words[kSmTile + (wn >> 1) * 64] >> sh_b;
-      }
-      s.b[h] = read_frag(st + kSmOperandBytes, 32 * wn + l32, 2 * h + g32, fx);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) s.a[2 * i + h] = read_frag(st, 64 * wm + 32 * i + l32, 2 * h + g32, fx);
+      read_b(st, h, s);
+      read_a(st, 0, h, s);
+      read_a(st, 1, h, s);
     }
   };
   // A step's fragments have landed by the wait in front of the next step's reads; without this the
@@ -107,15 +116,17 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
     return Ops{widen8(s.b[h][2 * q], s.b[h][2 * q + 1], sb), widen8(s.a[h][2 * q], s.a[h][2 * q + 1], s0),
                widen8(s.a[2 + h][2 * q], s.a[2 + h][2 * q + 1], s1)};
   };
+  // K 16t .. 16t + 15 of step s (o: its operands; left: the next ones)
+  auto mma_at = [&](const Step& s, int t, Ops& o) __attribute__((always_inline)) {
+    const Ops n = t < 7 ? conv(s, t + 1) : o;
+    acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.b, o.a0, acc[0], 0, 0, 0);
+    acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.b, o.a1, acc[1], 0, 0, 0);
+    o = n;
+  };
   auto mma = [&](const Step& s) __attribute__((always_inline)) {
     Ops o = conv(s, 0);
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const Ops n = t < 7 ? conv(s, t + 1) : o;
-      acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.b, o.a0, acc[0], 0, 0, 0);
-      acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.b, o.a1, acc[1], 0, 0, 0);
-      o = n;
-    }
+    for (int t = 0; t < 8; ++t) mma_at(s, t, o);
   };
 
   // The schedule of gemm_small.hpp: step kt's MFMAs beside the reads of kt+1 and the DMA of kt+3.
@@ -133,13 +144,24 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
     mma(cur);
     __builtin_amdgcn_sched_barrier(0);
   };
+  // Steady state: a third of the reads in front of each of the first three quarters of the MFMAs (all in
+  // front, they hold up the first MFMAs: 38.2 against 37.3 us for 1777x4096x2048).
   auto step_full = [&](int kt, Step& cur, Step& next) __attribute__((always_inline)) {
     issue(kt + kSmAhead);
     small_wait_stage<kLoads>(kSmAhead - 1);
     landed(cur);
-    read(kt + 1, next);
-    __builtin_amdgcn_sched_barrier(0);
-    mma(cur);
+    const uint8_t* st = smem + ((kt + 1) % kSmStages) * kStg;
+    Ops o = conv(cur, 0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (q == 0) read_b(st, 0, next), read_a(st, 0, 0, next);
+      if (q == 1) read_a(st, 1, 0, next), read_b(st, 1, next);
+      if (q == 2) read_a(st, 0, 1, next), read_a(st, 1, 1, next);
+      __builtin_amdgcn_sched_barrier(0);
+      mma_at(cur, 2 * q, o);
+      mma_at(cur, 2 * q + 1, o);
+    }
     __builtin_amdgcn_sched_barrier(0);
   };
   int kt = 0;
@@ -152,17 +174,19 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
     step(kt + 1, s1, s0);
   }
 
-  // lane: rows m0 + 64wm + 32i + l32, columns ecol + 8j .. +3 in registers 4j .. 4j+3 of acc[i].  The residual
-  // is loaded in front of the last products, into the registers of the next fragments.
-  const int ecol = n0 + 32 * wn + 4 * g32;
-  f32x4 res[2][4];
+  // The output goes through LDS and is stored as whole rows (thread: 16-byte chunks tid + 512u of the
+  // tile's rows of 32), and so is the residual loaded, in front of the last products, into the
+  // registers of the next fragments.  Rows past M repeat the last one and are not stored.
+  constexpr int kChunks = kSmTile * 32 / kSmThreads;
+  f32x4 res[kChunks];
+  const bool has_res = p.epi.residual != nullptr;
   auto load_res = [&]() __attribute__((always_inline)) {
-    if (p.epi.residual == nullptr) return;
+    if (!has_res) return;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {  // rows past M repeat the last one (never stored)
-      const int64_t at = static_cast<int64_t>(min(m0 + 64 * wm + 32 * i + l32, p.m - 1)) * p.n + ecol;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) res[i][j] = load4(p.epi.residual, at + 8 * j, true);
+    for (int u = 0; u < kChunks; ++u) {
+      const int idx = tid + kSmThreads * u, r = min(m0 + (idx >> 5), p.m - 1), c = idx & 31;
+      res[u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(static_cast<const float*>(p.epi.residual) +
+                                                                         static_cast<int64_t>(r) * p.n + n0 + c * 4));
     }
   };
   if (kt + 1 < k_steps) {
@@ -174,23 +198,28 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
     mma(s0);
   }
 
+  // lane: row 64wm + 32i + l32, columns 32wn + 8j + 4g32 .. +3 in registers 4j .. 4j+3 of acc[i]; chunk c of
+  // LDS row r at c ^ (r % 32)
   const float tens = MX ? 1.0f : (p.a_scale ? p.a_scale[0] : 1.0f) * (p.b_scale ? p.b_scale[0] : 1.0f);
-  f32x4 bias[4];
+  __syncthreads();  // every wave is done with the ring
 #pragma unroll
-  for (int j = 0; j < 4; ++j) bias[j] = epilogue_bias(p.epi, ecol + 8 * j);
+  for (int j = 0; j < 4; ++j) {
+    const f32x4 bias = epilogue_bias(p.epi, n0 + 32 * wn + 8 * j + 4 * g32);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = m0 + 64 * wm + 32 * i + l32;
-    if (r < p.m) {
-      float* dst = static_cast<float*>(p.c) + static_cast<int64_t>(r) * p.n + ecol;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f32x4 v{acc[i][4 * j] * tens, acc[i][4 * j + 1] * tens, acc[i][4 * j + 2] * tens, acc[i][4 * j + 3] * tens};
-        v = activate(v + bias[j], p.epi.act);
-        if (p.epi.residual != nullptr) v = v + res[i][j];
-        *reinterpret_cast<f32x4*>(dst + 8 * j) = v;
-      }
+    for (int i = 0; i < 2; ++i) {
+      const int r = 64 * wm + 32 * i + l32, c = 8 * wn + 2 * j + g32;
+      const f32x4 v{acc[i][4 * j] * tens, acc[i][4 * j + 1] * tens, acc[i][4 * j + 2] * tens, acc[i][4 * j + 3] * tens};
+      *reinterpret_cast<f32x4*>(smem + r * 512 + ((c ^ (r & 31)) << 4)) = activate(v + bias, p.epi.act);
     }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kChunks; ++u) {
+    const int idx = tid + kSmThreads * u, r = idx >> 5, c = idx & 31;
+    f32x4 v = *reinterpret_cast<const f32x4*>(smem + r * 512 + ((c ^ (r & 31)) << 4));
+    if (has_res) v = v + res[u];
+    if (m0 + r < p.m)
+      __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + static_cast<int64_t>(m0 + r) * p.n + n0 + c * 4));
   }
 }
 

@@ -24,7 +24,6 @@ namespace hkmoe {
 constexpr int kSortThreads = 256;
 constexpr int kSortSlots = 1024;   // slots that a sorting workgroup takes at a time
 constexpr int kSortBlocks = 256;   // sorting workgroups, at most
-constexpr int kSortSmall = 2048;   // slots up to which one launch sorts and copies
 constexpr int kMoveThreads = 512;  // of a workgroup that moves a token's rows, at most
 
 __device__ __forceinline__ int sort_key(int id, int experts) {
@@ -91,7 +90,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
       total[i] = before[i] = 0;
       if (i < per && e < n) {
         const int own = blockIdx.x;
-#pragma unroll 8
+#pragma unroll 32
         for (int b = 0; b < blocks; ++b) {
           const int c = counts[static_cast<int64_t>(b) * n + e];
           before[i] += b < own ? c : 0;
@@ -159,35 +158,30 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
   }
 }
 
-// 16 bytes copied or zeros, by 16-byte chunks of a row.
-__device__ __forceinline__ void put_row(void* row, const void* from, bool live, int chunks) {
-  for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
-    const uint4 v = live ? reinterpret_cast<const uint4*>(from)[c] : uint4{0, 0, 0, 0};
-    st_nt16(static_cast<uint4*>(row) + c, v);
-  }
-}
-
-// Up to kSortSmall slots in one launch: workgroup f counts the slots before slot f, and
-// copies its row; the last workgroup writes the offsets.
+// Small batches in one launch.  Workgroup (t, part) takes `each` slots of token t: it compares every slot's
+// expert with theirs, which gives their places, and copies the token's row there; the last workgroup
+// writes the offsets.
+constexpr int kSortAtOnce = 4;  // slots whose places one pass over the ids counts
 __global__ __launch_bounds__(kSortThreads) void permute_small_kernel(const int32_t* __restrict__ ids, int slots, int experts,
-                                                                     int top_k, const uint8_t* __restrict__ x,
+                                                                     int top_k, int parts, const uint8_t* __restrict__ x,
                                                                      int64_t row_bytes, uint8_t* __restrict__ xp,
                                                                      int32_t* __restrict__ offsets,
                                                                      int32_t* __restrict__ perm, int32_t* __restrict__ inv) {
-  __shared__ int red[kSortThreads / 64];
+  __shared__ int red[kSortThreads / 64][kSortAtOnce];
   const int tid = threadIdx.x;
-  if (static_cast<int>(blockIdx.x) == slots) {
+  if (blockIdx.x == gridDim.x - 1) {
     constexpr int kPer = (kMaxExperts + kSortThreads) / kSortThreads;
     __shared__ int hist[kMaxExperts + 1];
     const int n = experts + 1, per = (n + kSortThreads - 1) / kSortThreads;
     for (int e = tid; e < n; e += kSortThreads) hist[e] = 0;
     __syncthreads();
+#pragma unroll 4
     for (int f = tid; f < slots; f += kSortThreads) atomicAdd(&hist[sort_key(ids[f], experts)], 1);
     __syncthreads();
     int mine = 0;
     for (int i = 0; i < kPer; ++i)
       if (i < per && tid * per + i < n) mine += hist[tid * per + i];
-    int first = sort_scan(mine, red);
+    int first = sort_scan(mine, red[0]);
     for (int i = 0; i < kPer; ++i) {
       const int e = tid * per + i;
       if (i < per && e < n) {
@@ -197,24 +191,50 @@ __global__ __launch_bounds__(kSortThreads) void permute_small_kernel(const int32
     }
     return;
   }
-  const int f = blockIdx.x, key = sort_key(ids[f], experts);
-  int before = 0;
-  for (int g = tid; g < slots; g += kSortThreads) {
-    const int k = sort_key(ids[g], experts);
-    before += k < key || (k == key && g < f);
-  }
+  const int t = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int each = (top_k + parts - 1) / parts, j1 = min(top_k, (part + 1) * each);
+  const uint4* from = reinterpret_cast<const uint4*>(x + t * row_bytes);
+  const int chunks = static_cast<int>(row_bytes >> 4);
+  for (int j0 = part * each; j0 < j1; j0 += kSortAtOnce) {
+    const int f0 = t * top_k + j0;
+    int key[kSortAtOnce], before[kSortAtOnce];
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) before += __shfl_xor(before, o, 64);
-  if ((tid & 63) == 0) red[tid >> 6] = before;
-  __syncthreads();
-  int p = 0;
+    for (int u = 0; u < kSortAtOnce; ++u) {
+      key[u] = sort_key(ids[j0 + u < j1 ? f0 + u : f0], experts);
+      before[u] = 0;
+    }
+#pragma unroll 4
+    for (int g = tid; g < slots; g += kSortThreads) {
+      const int k = sort_key(ids[g], experts);
 #pragma unroll
-  for (int w = 0; w < kSortThreads / 64; ++w) p += red[w];
-  if (tid == 0) {
-    perm[p] = f;
-    inv[f] = p;
+      for (int u = 0; u < kSortAtOnce; ++u) before[u] += k < key[u] + (g < f0 + u);  // k < key, or equal and earlier
+    }
+#pragma unroll
+    for (int u = 0; u < kSortAtOnce; ++u) {
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) before[u] += __shfl_xor(before[u], o, 64);
+      if ((tid & 63) == 0) red[tid >> 6][u] = before[u];
+    }
+    __syncthreads();
+    int p[kSortAtOnce];
+#pragma unroll
+    for (int u = 0; u < kSortAtOnce; ++u) {
+      p[u] = 0;
+#pragma unroll
+      for (int w = 0; w < kSortThreads / 64; ++w) p[u] += red[w][u];
+      if (tid == u && j0 + u < j1) {
+        perm[p[u]] = f0 + u;
+        inv[f0 + u] = p[u];
+      }
+    }
+    for (int c = tid; c < chunks; c += kSortThreads) {
+      const uint4 v = from[c];
+#pragma unroll
+      for (int u = 0; u < kSortAtOnce; ++u)
+        if (j0 + u < j1) st_nt16(reinterpret_cast<uint4*>(xp + p[u] * row_bytes) + c, key[u] < experts ? v : uint4{0, 0, 0, 0});
+    }
+    __syncthreads();  // red is the next slots'
   }
-  put_row(xp + p * row_bytes, x + f / top_k * row_bytes, key < experts, static_cast<int>(row_bytes >> 4));
 }
 
 // Places in use, and whether a place is one: `inv` comes from the caller, and a row outside
@@ -394,9 +414,8 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const float* __restrict
   for (int e0 = 0; e0 < experts; e0 += 64) {
     float g = 0.0f;
     for (int j = 0; j < top_k; ++j) {
-      const int e = __shfl(ej, j, 64);
-      const float vj = __shfl(v, j, 64);
-      if (e == e0 + lane) g += vj;
+      const float vj = lane_value(v, j);
+      if (lane_value(ej, j) == e0 + lane) g += vj;
     }
     if (e0 + lane < experts) dlogits[t * experts + e0 + lane] = g;
   }

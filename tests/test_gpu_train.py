@@ -230,7 +230,7 @@ def _permute_case(hk, t, k, experts, hidden, dtype, away, seed=0):
 
 @pytest.mark.parametrize("t,k,experts,hidden", [
     (1, 1, 1, 8), (1, 8, 128, 4096), (3, 2, 5, 520), (64, 8, 128, 256), (255, 8, 256, 64), (256, 8, 60, 64), (257, 8, 60, 72),
-    (2048, 1, 1024, 16), (2049, 1, 1024, 16), (500, 6, 1, 128), (40, 32, 1024, 4104), (700, 32, 33, 32), (5000, 5, 7, 24),
+    (2048, 1, 1024, 16), (2049, 1, 1024, 16), (2048, 2, 1000, 16), (2049, 2, 1000, 16), (724, 8, 40, 24), (725, 8, 40, 24), (500, 6, 1, 128), (40, 32, 1024, 4104), (700, 32, 33, 32), (5000, 5, 7, 24),
     (33000, 8, 255, 16), (50, 3, 2, 9000)])
 @pytest.mark.parametrize("away", [0.0, 0.4])
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -238,18 +238,18 @@ def test_permute(hk, t, k, experts, hidden, away, dtype):
     _permute_case(hk, t, k, experts, hidden, dtype, away)
 
 
-@pytest.mark.parametrize("t,k", [(5, 3), (900, 4)])
+@pytest.mark.parametrize("t,k", [(5, 3), (3000, 4)])
 def test_permute_bytes(hk, t, k):
     _permute_case(hk, t, k, 40, 272, F8, 0.2)
 
 
-@pytest.mark.parametrize("t,k", [(7, 4), (900, 4)])
+@pytest.mark.parametrize("t,k", [(7, 4), (3000, 4)])
 def test_permute_nothing_here(hk, t, k):
     """No slot has an expert here: zeros everywhere, and no row is read back."""
     _permute_case(hk, t, k, 16, 64, BF16, 1.1)
 
 
-@pytest.mark.parametrize("t,k", [(7, 4), (900, 4)])
+@pytest.mark.parametrize("t,k", [(7, 4), (3000, 4)])
 def test_permute_one_expert(hk, t, k):
     """Every slot at one expert, the same twice in a row: their own order."""
     ids = torch.full((t, k), 3, dtype=torch.int32, device="cuda")
@@ -489,7 +489,7 @@ def _step(hk, b, x, s, dout, dr, w_all):
     return out, dlogits, dx, dnw, dnb
 
 
-@pytest.mark.parametrize("t", [50, 1500])
+@pytest.mark.parametrize("t", [50, 2500])
 def test_step_captured(hk, t):
     """Two captured steps that share no workspace, replayed with changing inputs between eager work."""
     b = Block(256, 32, 24, 4, BF16)

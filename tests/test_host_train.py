@@ -151,7 +151,7 @@ def test_route_gradient_refusals(lib, bad, says):
 
 def test_permute_workspace(lib):
     f = lambda t, e, k: lib.hkmoe_permute_workspace_size(i64(t), i32(e), i32(k))  # noqa: E731
-    assert f(4, 8, 2) == 0 and _permute(lib, t=0, x=None, ids=None, xp=None, perm=None, inv=None, e=0) == 1
+    assert f(4, 8, 2) == 0 and f(2048, 8, 2) == 0 and _permute(lib, t=0, x=None, ids=None, xp=None, perm=None, inv=None, e=0) == 1
     for t, e, k in ((0, 8, 2), (-1, 8, 2), (2 ** 62, 8, 2), (1 << 20, 0, 2), (1 << 20, 1025, 2), (1 << 20, 8, 0), (1 << 20, 8, 33)):
         assert f(t, e, k) == 0
     need = f(4096, 8, 2)
@@ -224,11 +224,11 @@ for line in log(): print(line)
 
 def test_small_batches_sort_in_one_launch(fake):
     out = hip_host.run(fake, LAUNCH + """
-for t, k in ((1, 1), (256, 8), (2048, 1), (257, 8), (2049, 1)):
+for t, k in ((1, 1), (256, 8), (2048, 2), (724, 8), (2049, 2), (725, 8), (1 << 24, 1)):
     assert lib.hkmoe_permute(P, P, i64(t), i32(64), i32(k), i64(64), 0, P, P, P, P, P, size(1 << 50), None) == 0
     print(len(log()))
 """)
-    assert [int(v) for v in out] == [1, 1, 1, 3, 3]
+    assert [int(v) for v in out] == [1, 1, 1, 1, 3, 3, 3]
 
 
 # ---------------------------------------------------------------------------
