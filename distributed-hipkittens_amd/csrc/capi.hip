@@ -716,14 +716,18 @@ int launch_layer_norm(const LayerNormParams& p, hipStream_t s) {
 //   8192x7168 bf16    94 /  99 / 104 / 111     16384x1024 bf16  45 / 34 / 31 / 38
 //   4096x4096 bf16    35 /  32 /  34 /  38     1999x2560 fp32   16 / 18 / 19 / 22
 int layer_norm_parts(int64_t rows, int64_t cols) {
-  int per = 1, each = 8, threads = 0;  // rows at a time, turns for each slot
+  int per = 1, each = 8, threads = 0, few = 4;  // rows at a time, turns for each slot, turns that one workgroup takes
   (void)with_layer_norm_shape(cols, [&](auto ch, auto lanes) {
     constexpr int LANES = decltype(lanes)::value;
     per = kLnRowThreads / (LANES ? LANES : kLnRowThreads);
     each = LANES ? 5 : 8;
     threads = LANES ? kLnRowThreads : row_threads(cols, decltype(ch)::value);
+    few = decltype(ch)::value == 4 ? 1 : 4;
     return HKMOE_OK;
   });
+  // one workgroup writes dw and db itself, without a workspace or a second launch (4 rows of 4096: 7.4 us a
+  // call, 5 rows in two launches 11.1; 4 rows of 16384 17.1 and 11.4, so wide rows only alone)
+  if (rows <= few * per) return 1;
   const int64_t fill = kLnParts * std::clamp(1024 / threads, 1, 3);
   return static_cast<int>(std::min((rows + per - 1) / per, std::max<int64_t>(kLnParts, std::min(fill, rows / (per * each)))));
 }
@@ -1805,7 +1809,8 @@ int hkmoe_rms_norm_quant(const void* x, const void* residual, const void* weight
 
 size_t hkmoe_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
   if (rows <= 0 || rows > kMaxRows || cols <= 0 || cols > kLnMaxCols) return 0;
-  return align256(static_cast<size_t>(layer_norm_parts(rows, cols)) * 2 * cols * sizeof(float));
+  const int parts = layer_norm_parts(rows, cols);
+  return parts == 1 ? 0 : align256(static_cast<size_t>(parts) * 2 * cols * sizeof(float));
 }
 
 // What both directions ask of the sizes and types.
@@ -1863,12 +1868,15 @@ int hkmoe_layer_norm_backward(const void* dy, const void* r, const void* weight,
   p.dr = dr;
   p.stats = reinterpret_cast<const f32x4*>(stats);
   p.dx = dx;
-  p.part = static_cast<float*>(workspace);
+  p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  p.dw = dweight;
+  p.db = dbias;
   p.rows = rows;
   p.cols = static_cast<int32_t>(cols);
   p.w_f32 = weight_dtype == HKMOE_F32;
   auto s = static_cast<hipStream_t>(stream);
   if (rows > 0) HK_TRY(x_dtype == HKMOE_F32 ? launch_layer_norm_grad<true>(p, s) : launch_layer_norm_grad<false>(p, s));
+  if (rows > 0 && need == 0) return HKMOE_OK;
   // without rows the sums are empty: zeros
   hipLaunchKernelGGL(layer_norm_sum_kernel, dim3(static_cast<unsigned>((2 * cols + 63) / 64)), dim3(kLnSumThreads), 0, s, p.part,
                      rows > 0 ? layer_norm_parts(rows, cols) : 0, p.cols, dweight, dbias, p.w_f32);

@@ -13,7 +13,8 @@
 // terms, because one would cost r - m as many bits as |m| is larger than its spread.
 // Backward: the row's two sums in fp32, and in the same pass every thread's own
 // columns of dw and db over the workgroup's rows, in registers; one partial per
-// workgroup goes to the workspace and a second launch adds them in order, in 64 bits.
+// workgroup goes to the workspace and a second launch adds them in order, in 64 bits (a few rows
+// take one workgroup, and no second launch).
 // Nothing is added atomically: the same call gives the same bits.
 #pragma once
 
@@ -49,7 +50,9 @@ struct LayerNormGradParams {
   const void* dr;      // may be null
   const f32x4* stats;
   void* dx;
-  float* part;  // [gridDim.x][2][cols]
+  float* part;  // [gridDim.x][2][cols], or null with one workgroup, which writes dw and db itself
+  void* dw;
+  void* db;  // may be null
   int64_t rows;
   int32_t cols;
   int32_t w_f32;
@@ -235,6 +238,15 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_kernel(Layer
   }
 }
 
+// Value j of dw or db (which may be null) in its type.
+__device__ __forceinline__ void put_sum(void* to, int j, float v, int w_f32) {
+  if (to == nullptr) return;
+  if (w_f32)
+    static_cast<float*>(to)[j] = v;
+  else
+    static_cast<uint16_t*>(to)[j] = static_cast<uint16_t>(bf16_rne_bits(v));
+}
+
 // Rows blockIdx.x * rows per workgroup, + gridDim.x * that, ...; the next row is loaded
 // before the sums of this one are waited for (kAhead).
 template <bool F32, int CH, int LANES>
@@ -329,8 +341,16 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_grad_kernel(
     for (int c = 0; c < CH; ++c) {
       const int j = ln_col<LANES>(c);
       if (j < cols) {
-        store8<true>(part, j, dw[c]);
-        store8<true>(part, cols + j, db[c]);
+        if (p.part != nullptr) {
+          store8<true>(part, j, dw[c]);
+          store8<true>(part, cols + j, db[c]);
+        } else if (p.w_f32) {
+          store8<true>(p.dw, j, dw[c]);
+          if (p.db != nullptr) store8<true>(p.db, j, db[c]);
+        } else {
+          store8<false>(p.dw, j, dw[c]);
+          if (p.db != nullptr) store8<false>(p.db, j, db[c]);
+        }
       }
     }
   } else {
@@ -347,7 +367,12 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_grad_kernel(
         const int l = u / 8, j = ((c % CH) * LANES + l) * kNormChunk + u % 8;
         float s = 0.0f;
         for (int q = 0; q < kLnRowThreads / LANES; ++q) s += meet[q * LANES + l][u % 8];
-        if (j < cols) part[(c < CH ? 0 : cols) + j] = s;
+        if (j < cols) {
+          if (p.part != nullptr)
+            part[(c < CH ? 0 : cols) + j] = s;
+          else
+            put_sum(c < CH ? p.dw : p.db, j, s, p.w_f32);
+        }
       }
     }
   }
@@ -374,14 +399,7 @@ __global__ __launch_bounds__(kLnSumThreads) void layer_norm_sum_kernel(const flo
   if (wave != 0 || i >= width) return;
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) s += red[w][lane];
-  const float v = static_cast<float>(s);
-  void* to = i < cols ? dw : db;
-  const int j = i < cols ? i : i - cols;
-  if (to == nullptr) return;
-  if (w_f32)
-    static_cast<float*>(to)[j] = v;
-  else
-    static_cast<uint16_t*>(to)[j] = static_cast<uint16_t>(bf16_rne_bits(v));
+  put_sum(i < cols ? dw : db, i < cols ? i : i - cols, static_cast<float>(s), w_f32);
 }
 
 }  // namespace hkmoe

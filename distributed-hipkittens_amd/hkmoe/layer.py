@@ -82,7 +82,7 @@ def gemm_fp8(a_q, b_q, scale_a=None, scale_b=None, out_dtype=torch.bfloat16, bia
     instruction gives (1.5e-5 of its size)."""
     _check_dev(a_q, b_q)
     act = _activation(activation)
-    c = a_q.new_empty((a_q.shape[0], b_q.shape[0]), dtype=out_dtype) if out is None else out
+    c = a_q.new_empty(a_q.shape[0], b_q.shape[0], dtype=out_dtype) if out is None else out
     if bias is None and activation is None and residual is None:
         tk_kernel.dispatch_gemm_fp8(a_q, b_q, c, scale_a, scale_b)
     else:
@@ -119,7 +119,7 @@ def gemm_mx(a_q, a_packed, b_q, b_packed, out_dtype=torch.float32, bias=None, ac
     the other arguments as in :func:`gemm_fp8`."""
     _check_dev(a_q, b_q)
     act = _activation(activation)
-    c = a_q.new_empty((a_q.shape[0], b_q.shape[0]), dtype=out_dtype) if out is None else out
+    c = a_q.new_empty(a_q.shape[0], b_q.shape[0], dtype=out_dtype) if out is None else out
     if bias is None and activation is None and residual is None:
         tk_kernel.dispatch_gemm_mx(a_q, a_packed, b_q, b_packed, c)
     else:

@@ -12,7 +12,6 @@ import torch
 
 import tk_kernel
 
-from .layer import _like
 
 
 # ----------------------------------------------------------------------------
@@ -27,14 +26,14 @@ def layer_norm_forward(x, weight, bias=None, residual=None, eps=1e-5, residual_o
     :func:`layer_norm_backward` wants back (fp32 [R, 4])."""
     if x.dim() != 2:
         raise RuntimeError("layer_norm: x must be [R, C]")
-    y = _like(x, x.dtype)
-    stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
+    y = torch.empty_like(x)
+    stats = x.new_empty(x.shape[0], 4, dtype=torch.float32)
     if residual is None:
         if residual_out is not None:
             raise RuntimeError("layer_norm: residual_out needs a residual")
         r = x
     else:
-        r = residual_out = _like(x, x.dtype) if residual_out is None else residual_out
+        r = residual_out = torch.empty_like(x) if residual_out is None else residual_out
     tk_kernel.dispatch_layer_norm(x, residual, weight, bias, eps, y, residual_out, stats)
     return y, r, stats
 
@@ -42,10 +41,10 @@ def layer_norm_forward(x, weight, bias=None, residual=None, eps=1e-5, residual_o
 def layer_norm_backward(dy, r, weight, stats, dr=None, with_bias=True):
     """``(dx, dweight, dbias)`` for the gradient ``dy`` of y and, where given, ``dr`` of the new
     stream r.  dx is the gradient of both x and the residual; dbias is None without ``with_bias``."""
-    dx, dw = _like(r, r.dtype), _like(weight, weight.dtype)
-    db = _like(weight, weight.dtype) if with_bias else None
+    dx, dw = torch.empty_like(r), torch.empty_like(weight)
+    db = torch.empty_like(weight) if with_bias else None
     need = tk_kernel.layer_norm_backward_workspace_size(*r.shape)
-    ws = r.new_empty((need,), dtype=torch.uint8) if need else None
+    ws = r.new_empty(need, dtype=torch.uint8) if need else None
     tk_kernel.dispatch_layer_norm_backward(dy, r, weight, dr, stats, dx, dw, db, ws)
     return dx, dw, db
 
@@ -86,16 +85,16 @@ def route_topk_forward(logits, top_k):
     if logits.dim() != 2:
         raise RuntimeError("route_topk: logits must be [T, E]")
     t, e = logits.shape
-    idx = logits.new_empty((t, top_k), dtype=torch.int32)
-    w = logits.new_empty((t, top_k))
-    counts = logits.new_empty((tk_kernel.route_blocks(t), e), dtype=torch.int32)
+    idx = logits.new_empty(t, top_k, dtype=torch.int32)
+    w = logits.new_empty(t, top_k)
+    counts = logits.new_empty(tk_kernel.route_blocks(t), e, dtype=torch.int32)
     tk_kernel.dispatch_route_topk(logits, idx, w, counts)
     return idx, w
 
 
 def route_topk_backward(dw, w, idx, num_experts):
     """Gradient of the logits (fp32 [T, E]) for the gradient ``dw`` of the weights ``w``."""
-    dlogits = dw.new_empty((dw.shape[0], num_experts))
+    dlogits = dw.new_empty(dw.shape[0], num_experts)
     tk_kernel.dispatch_route_topk_backward(dw, w, idx, dlogits)
     return dlogits
 
@@ -118,7 +117,7 @@ class _RouteTopk(torch.autograd.Function):
 
 def route_topk(logits, top_k):
     """:func:`route_topk_forward` with the gradient of w to the logits recorded."""
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         return _RouteTopk.apply(logits, top_k)
     return route_topk_forward(logits, top_k)
 
@@ -144,17 +143,17 @@ def moe_permute_forward(x, ids, num_experts):
     if num_experts < 1:
         raise RuntimeError("moe_permute: num_experts must be positive")
     t, k = ids.shape
-    xp = x.new_empty((t * k, x.shape[1]))
-    order = MoEOrder(ids.new_empty((num_experts + 1,)), ids.new_empty((t * k,)), ids.new_empty((t, k)))
+    xp = x.new_empty(t * k, x.shape[1])
+    order = MoEOrder(ids.new_empty(num_experts + 1), ids.new_empty(t * k), torch.empty_like(ids))
     need = tk_kernel.permute_workspace_size(t, num_experts, k)
-    ws = x.new_empty((need,), dtype=torch.uint8) if need else None
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     tk_kernel.dispatch_permute(x, ids, xp, *order, ws)
     return xp, order
 
 
 def moe_permute_backward(dxp, order):
     """Gradient of x [T, H]: the sum of its slots' rows of ``dxp`` [T*k, H]."""
-    dx = dxp.new_empty((order.inv_perm.shape[0], dxp.shape[1]))
+    dx = dxp.new_empty(order.inv_perm.shape[0], dxp.shape[1])
     tk_kernel.dispatch_combine_rows(dxp, None, order.offsets, order.inv_perm, dx)
     return dx
 
@@ -162,14 +161,14 @@ def moe_permute_backward(dxp, order):
 def moe_combine_forward(y, w, order):
     """out[t] = sum_j w[t, j] y[inv_perm[t, j]] over the slots that have an expert here: y [T*k, H]
     bf16 or fp32, w fp32 [T, k]; summed in fp32, rounded to y's dtype."""
-    out = y.new_empty((order.inv_perm.shape[0], y.shape[1]))
+    out = y.new_empty(order.inv_perm.shape[0], y.shape[1])
     tk_kernel.dispatch_combine_rows(y, w, order.offsets, order.inv_perm, out)
     return out
 
 
 def moe_combine_backward(dout, y, w, order):
     """``(dy, dw)``: gradients of y (zeros behind the last expert's rows) and w."""
-    dy, dw = _like(y, y.dtype), _like(w, w.dtype)
+    dy, dw = torch.empty_like(y), torch.empty_like(w)
     tk_kernel.dispatch_combine_rows_backward(dout, y, w, order.offsets, order.inv_perm, dy, dw)
     return dy, dw
 
@@ -203,7 +202,7 @@ class _Combine(torch.autograd.Function):
 
 def moe_permute(x, ids, num_experts):
     """:func:`moe_permute_forward` with the gradient of x recorded (not for e4m3 rows)."""
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         xp, *order = _Permute.apply(x, ids, num_experts)
         return xp, MoEOrder(*order)
     return moe_permute_forward(x, ids, num_experts)
@@ -211,6 +210,6 @@ def moe_permute(x, ids, num_experts):
 
 def moe_combine(y, w, order):
     """:func:`moe_combine_forward` with the gradients of y and w recorded."""
-    if torch.is_grad_enabled() and (y.requires_grad or w.requires_grad):
+    if (y.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         return _Combine.apply(y, w, *order)
     return moe_combine_forward(y, w, order)

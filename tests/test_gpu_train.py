@@ -55,7 +55,7 @@ def _norm_case(hk, rows, cols, dtype, wdtype, residual=True, bias=True, dr=True,
     got = hk.layer_norm_backward(dy, r, w, stats, dr=back, with_bias=bias)
     torch.cuda.synchronize()
     args = (dy.double(), r64, w64, eps, None if back is None else back.double())
-    each = math.ceil(rows / PARTS) + 16
+    each = max(4, math.ceil(rows / PARTS)) + 16
     for name, g, v, bd in zip(("dx", "dw", "db"), got, ref.layer_norm_grad(*args), ref.layer_norm_grad_bound(*args, dtype, wdtype, each)):
         if name == "db" and not bias:
             assert g is None
@@ -70,8 +70,8 @@ def test_norm_widths(hk, cols, dtype, rows):
     _norm_case(hk, rows, cols, dtype, (BF16, F32)[cols // 8 % 2], residual=rows == 5)
 
 
-@pytest.mark.parametrize("rows", [2, 63, 255, 256, 257, 1000, 4099])
-@pytest.mark.parametrize("cols", [64, 384, 1000, 1400])
+@pytest.mark.parametrize("rows", [2, 4, 16, 17, 32, 33, 63, 64, 255, 256, 257, 1000, 4099])
+@pytest.mark.parametrize("cols", [64, 200, 384, 1000, 1400])
 def test_norm_rows(hk, rows, cols):
     _norm_case(hk, rows, cols, (BF16, F32)[rows % 2], F32, residual=rows % 3 != 0, bias=rows % 5 != 0, dr=rows % 2 == 0,
                in_place=rows % 2 == 1)

@@ -91,9 +91,10 @@ def test_norm_gradient_refusals(lib, bad, says):
 
 
 def test_norm_workspace(lib):
-    need = lib.hkmoe_layer_norm_backward_workspace_size(i64(4), i64(256))
-    assert need > 0
-    assert _norm_grad(lib, ws=None) == 4 and _norm_grad(lib, ws_bytes=need - 1) == 4 and _norm_grad(lib, ws=ODD) == 4
+    need = lib.hkmoe_layer_norm_backward_workspace_size(i64(400), i64(256))
+    assert need > 0 and lib.hkmoe_layer_norm_backward_workspace_size(i64(4), i64(256)) == 0  # one workgroup
+    for bad in (dict(ws=None), dict(ws_bytes=need - 1), dict(ws=ODD)):
+        assert _norm_grad(lib, rows=400, **bad) == 4
     for rows, cols in ((0, 256), (-1, 256), (2 ** 62, 256), (4, 0), (4, 2 ** 62), (4, 16392)):
         assert lib.hkmoe_layer_norm_backward_workspace_size(i64(rows), i64(cols)) == 0
     assert lib.hkmoe_layer_norm_backward_workspace_size(i64(1 << 24), i64(16384)) >= 2 * 16384 * 4
@@ -220,6 +221,16 @@ for line in log(): print(line)
                 got.add(f"strip {m.group(2)}x{m.group(3)}" if m.group(2) else m.group(1))
             want = {"strip 1x1", "strip 2x1", "strip 1x2", "strip 2x2", "strip 2x4", "strip 4x4"}
             assert got == want | ({"wide"} if f32 else {"small_act", "persistent"}), (mx, f32, got)
+
+
+def test_few_rows_need_one_launch_for_the_gradient(fake):
+    """Four turns of one workgroup's rows (16 lanes to a row of 128 columns: 16 rows a turn), and one more."""
+    out = hip_host.run(fake, LAUNCH + """
+for rows, cols in ((1, 4096), (4, 4096), (64, 128), (1, 16384), (5, 4096), (65, 128), (2, 16384), (0, 128)):
+    assert lib.hkmoe_layer_norm_backward(P, P, P, P, P, i64(rows), i64(cols), 0, 0, P, P, P, P, size(1 << 50), None) == 0
+    print(len(log()))
+""")
+    assert [int(v) for v in out] == [1, 1, 1, 1, 2, 2, 2, 1]
 
 
 def test_small_batches_sort_in_one_launch(fake):
