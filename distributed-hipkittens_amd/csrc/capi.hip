@@ -1926,7 +1926,8 @@ int hkmoe_permute(const void* x, const int32_t* ids, int64_t num_tokens, int32_t
   if (sort_in_one(num_tokens, top_k)) {
     // the slots of a token shared among workgroups while those are few
     const int parts = static_cast<int>(std::clamp<int64_t>(num_tokens == 0 ? 1 : 512 / num_tokens, 1, top_k));
-    hipLaunchKernelGGL(permute_small_kernel, dim3(static_cast<unsigned>(num_tokens * parts + 1)), dim3(kSortThreads), 0, s, ids,
+    auto kern = parts == top_k ? permute_small_kernel<1> : permute_small_kernel<kSortAtOnce>;
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(num_tokens * parts + 1)), dim3(kSortThreads), 0, s, ids,
                        static_cast<int>(slots), num_experts, top_k, parts, static_cast<const uint8_t*>(x), row_bytes,
                        static_cast<uint8_t*>(xp), offsets, perm, inv_perm);
     return check_launch("permute_small_kernel");

@@ -161,13 +161,16 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int32_t*
 // Small batches in one launch.  Workgroup (t, part) takes `each` slots of token t: it compares every slot's
 // expert with theirs, which gives their places, and copies the token's row there; the last workgroup
 // writes the offsets.
-constexpr int kSortAtOnce = 4;  // slots whose places one pass over the ids counts
+// N: slots whose places one pass over the ids counts (1 where a workgroup has one: 64 tokens x 8, rows of
+// 8 KiB 3.4 us in a graph, with 4 4.4).
+constexpr int kSortAtOnce = 4;
+template <int N>
 __global__ __launch_bounds__(kSortThreads) void permute_small_kernel(const int32_t* __restrict__ ids, int slots, int experts,
                                                                      int top_k, int parts, const uint8_t* __restrict__ x,
                                                                      int64_t row_bytes, uint8_t* __restrict__ xp,
                                                                      int32_t* __restrict__ offsets,
                                                                      int32_t* __restrict__ perm, int32_t* __restrict__ inv) {
-  __shared__ int red[kSortThreads / 64][kSortAtOnce];
+  __shared__ int red[kSortThreads / 64][N];
   const int tid = threadIdx.x;
   if (blockIdx.x == gridDim.x - 1) {
     constexpr int kPer = (kMaxExperts + kSortThreads) / kSortThreads;
@@ -195,11 +198,11 @@ __global__ __launch_bounds__(kSortThreads) void permute_small_kernel(const int32
   const int each = (top_k + parts - 1) / parts, j1 = min(top_k, (part + 1) * each);
   const uint4* from = reinterpret_cast<const uint4*>(x + t * row_bytes);
   const int chunks = static_cast<int>(row_bytes >> 4);
-  for (int j0 = part * each; j0 < j1; j0 += kSortAtOnce) {
+  for (int j0 = part * each; j0 < j1; j0 += N) {
     const int f0 = t * top_k + j0;
-    int key[kSortAtOnce], before[kSortAtOnce];
+    int key[N], before[N];
 #pragma unroll
-    for (int u = 0; u < kSortAtOnce; ++u) {
+    for (int u = 0; u < N; ++u) {
       key[u] = sort_key(ids[j0 + u < j1 ? f0 + u : f0], experts);
       before[u] = 0;
     }
@@ -207,18 +210,18 @@ __global__ __launch_bounds__(kSortThreads) void permute_small_kernel(const int32
     for (int g = tid; g < slots; g += kSortThreads) {
       const int k = sort_key(ids[g], experts);
 #pragma unroll
-      for (int u = 0; u < kSortAtOnce; ++u) before[u] += k < key[u] + (g < f0 + u);  // k < key, or equal and earlier
+      for (int u = 0; u < N; ++u) before[u] += k < key[u] + (g < f0 + u);  // k < key, or equal and earlier
     }
 #pragma unroll
-    for (int u = 0; u < kSortAtOnce; ++u) {
+    for (int u = 0; u < N; ++u) {
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) before[u] += __shfl_xor(before[u], o, 64);
       if ((tid & 63) == 0) red[tid >> 6][u] = before[u];
     }
     __syncthreads();
-    int p[kSortAtOnce];
+    int p[N];
 #pragma unroll
-    for (int u = 0; u < kSortAtOnce; ++u) {
+    for (int u = 0; u < N; ++u) {
       p[u] = 0;
 #pragma unroll
       for (int w = 0; w < kSortThreads / 64; ++w) p[u] += red[w][u];
@@ -230,7 +233,7 @@ __global__ __launch_bounds__(kSortThreads) void permute_small_kernel(const int32
     for (int c = tid; c < chunks; c += kSortThreads) {
       const uint4 v = from[c];
 #pragma unroll
-      for (int u = 0; u < kSortAtOnce; ++u)
+      for (int u = 0; u < N; ++u)
         if (j0 + u < j1) st_nt16(reinterpret_cast<uint4*>(xp + p[u] * row_bytes) + c, key[u] < experts ? v : uint4{0, 0, 0, 0});
     }
     __syncthreads();  // red is the next slots'
