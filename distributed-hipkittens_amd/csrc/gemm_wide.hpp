@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
 
   // Fragments of a step: a[2i + h] bytes 64h + 32g32 .. +31 of row 64wm + 32i + l32, b[h] of column
   // 32wn + l32; MX: block 2h + g32, whose exponents are bytes 2i + l32/16 (columns: 2(wn % 2) + l32/16)
-  // of word 16(2h + g32) + l32 % 16 of the 64-row group, here shifted so that i = 0 is byte 0.
+  // of word 16(2h + g32) + l32 % 16 of the 64-row group.
   struct Step {
     i32x8 a[4], b[2];
     int wa[2], wb[2];
@@ -81,8 +81,8 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
   auto read_b = [&](const uint8_t* st, int h, Step& s) __attribute__((always_inline)) {
     if constexpr (MX) {
       const int32_t* words = reinterpret_cast<const int32_t*>(st + kSmStageBytes) + 16 * (2 * h + g32) + (l32 & 15);
-      s.wa[h] = words[wm * 64] >> sh_a;
-      s.wb[h] = words[kSmTile + (wn >> 1) * 64] >> sh_b;
+      s.wa[h] = words[wm * 64];
+      s.wb[h] = words[kSmTile + (wn >> 1) * 64];
     }
     s.b[h] = read_frag(st + kSmOperandBytes, 32 * wn + l32, 2 * h + g32, fx);
   };
@@ -99,6 +99,7 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
   // compiler, which does not see that wait, waits for those reads as well.
   auto landed = [&](Step& s) __attribute__((always_inline)) {
     asm volatile("" : "+v"(s.a[0]), "+v"(s.a[1]), "+v"(s.a[2]), "+v"(s.a[3]), "+v"(s.b[0]), "+v"(s.b[1]));
+    if constexpr (MX) asm volatile("" : "+v"(s.wa[0]), "+v"(s.wa[1]), "+v"(s.wb[0]), "+v"(s.wb[1]));
   };
 
   f32x16 acc[2];
@@ -111,8 +112,8 @@ __global__ __launch_bounds__(kSmThreads, 2) void gemm_fp8_wide(SmallGemmParams p
   };
   auto conv = [&](const Step& s, int t) __attribute__((always_inline)) -> Ops {
     const int h = t >> 2, q = t & 3;  // K bytes 8q .. 8q + 7 of half h's 32
-    const float sb = MX ? e8m0_scale<0>(s.wb[h]) : 1.0f, s0 = MX ? e8m0_scale<0>(s.wa[h]) : 1.0f,
-                s1 = MX ? e8m0_scale<2>(s.wa[h]) : 1.0f;
+    const float sb = MX ? e8m0_scale<0>(s.wb[h] >> sh_b) : 1.0f, s0 = MX ? e8m0_scale<0>(s.wa[h] >> sh_a) : 1.0f,
+                s1 = MX ? e8m0_scale<2>(s.wa[h] >> sh_a) : 1.0f;
     return Ops{widen8(s.b[h][2 * q], s.b[h][2 * q + 1], sb), widen8(s.a[h][2 * q], s.a[h][2 * q + 1], s0),
                widen8(s.a[2 + h][2 * q], s.a[2 + h][2 * q + 1], s1)};
   };
