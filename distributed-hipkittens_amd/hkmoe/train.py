@@ -55,12 +55,15 @@ class _LayerNorm(torch.autograd.Function):
         y, r, stats = layer_norm_forward(x, weight, bias, residual, eps)
         ctx.save_for_backward(r, weight, stats)
         ctx.has_bias, ctx.has_residual = bias is not None, residual is not None
+        ctx.set_materialize_grads(False)  # of y and r, where one has no use: no zeros to read
         return (y, r) if residual is not None else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dr=None):
         r, weight, stats = ctx.saved_tensors
+        if dy is None:  # the norm has no use: the stream's own gradient is all there is
+            return dr, None, None, dr, None
         dx, dw, db = layer_norm_backward(dy.contiguous(), r, weight, stats, None if dr is None else dr.contiguous(),
                                          ctx.has_bias)
         return dx, dw, db, dx if ctx.has_residual else None, None

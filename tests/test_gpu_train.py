@@ -77,6 +77,20 @@ def test_norm_rows(hk, rows, cols):
                in_place=rows % 2 == 1)
 
 
+@pytest.mark.parametrize("cols", [64, 1000, 4096, 10000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_stream_in_place(hk, cols, dtype):
+    """The new stream over x, and over the residual, with more rows than workgroups."""
+    x, w, b, gen = _norm_inputs(1500, cols, dtype, dtype, 8)
+    res = _randn(gen, 1500, cols).to(dtype)
+    y, r, stats = hk.layer_norm_forward(x, w, b, res)
+    for which in (0, 1):
+        t = [x.clone(), res.clone()]
+        y1, r1, stats1 = hk.layer_norm_forward(t[0], w, b, t[1], residual_out=t[which])
+        assert r1 is t[which] and torch.equal(r1, r) and torch.equal(y1, y) and torch.equal(stats1, stats)
+        assert torch.equal(t[1 - which], (x, res)[1 - which])
+
+
 def test_norm_far_from_zero(hk):
     """A mean of 2^12 times the spread (the stream is what it is rounded to): the bits of r - mean stay."""
     for cols in (128, 1000, 4096):
@@ -469,6 +483,13 @@ def test_gradients_only_where_asked(hk):
     sel[::2] = 1
     n = ref.layer_norm(r.double(), torch.ones(64, device="cuda").double(), None, 1e-5)[0] * sel
     _check(g, n.sum(0), 60 * ref.U * n.abs().sum(0))
+    xr = x.clone().requires_grad_()
+    y, r = hk.layer_norm(xr, w, residual=x)  # the norm, and then the stream, without a use
+    gx, gw = torch.autograd.grad(r.sum(), [xr, w], allow_unused=True, retain_graph=True)
+    assert bool((gx == 1).all()) and gw is None
+    gx, _ = torch.autograd.grad((y * y).sum(), [xr, w])
+    y2, r2, stats2 = hk.layer_norm_forward(x, w.detach(), None, x)
+    assert torch.equal(gx, hk.layer_norm_backward(2 * y2, r2, w.detach(), stats2)[0])
     idx, tw = hk.route_topk(torch.randn((6, 9), device="cuda", requires_grad=True), 2)
     assert tw.requires_grad and not idx.requires_grad
     xp, order = hk.moe_permute(x, idx, 9)
