@@ -970,7 +970,7 @@ static int epilogue_check(const char* name, const void* c, int64_t m, int64_t n,
                           int activation, const void* residual, EpilogueArgs* e) {
   HK_REQUIRE(activation >= HKMOE_ACT_NONE && activation <= HKMOE_ACT_GELU_TANH, "%s: bad activation %d", name, activation);
   HK_REQUIRE(!bias || bias_dtype == HKMOE_BF16 || bias_dtype == HKMOE_F32, "%s: bad bias_dtype %d", name, bias_dtype);
-  HK_REQUIRE(n <= (1 << 22), "%s: N=%lld must be at most 2^22", name, (long long)n);
+  HK_REQUIRE(n <= (1 << 21), "%s: N=%lld must be at most 2^21", name, (long long)n);  // a 256-row tile below 2^31 bytes
   HK_REQUIRE(aligned16(bias) && aligned16(residual) && aligned16(c), "%s: bias, residual and C must be 16-byte aligned", name);
   *e = EpilogueArgs{bias, m > 0 ? residual : nullptr, static_cast<Act>(activation), bias_dtype == HKMOE_F32};
   return HKMOE_OK;

@@ -10,6 +10,7 @@ import torch
 
 import hip_host
 import test_gpu_epilogue
+import test_host_block
 import train_ref as ref
 
 P = ctypes.c_void_p(0x1000)  # never dereferenced: validation fails first
@@ -50,7 +51,7 @@ def _mx(lib, a=P, b=P, c=P, m=4, n=256, k=128, out=0, bias=None, bt=0, act=1, re
 @pytest.mark.parametrize("call", [_fp8, _mx])
 @pytest.mark.parametrize("bad,says", [
     (dict(a=None), "null"), (dict(b=None), "null"), (dict(c=None), "null"), (dict(m=-1), "shape"), (dict(n=0), "shape"),
-    (dict(k=130), "multiple of 128"), (dict(n=128), "multiple of 256"), (dict(n=(1 << 22) + 256), "2^22"), (dict(out=2), "out_dtype"),
+    (dict(k=130), "multiple of 128"), (dict(n=128), "multiple of 256"), (dict(n=(1 << 21) + 256), "2^21"), (dict(out=2), "out_dtype"),
     (dict(m=1 << 26), "too large"), (dict(act=5), "activation"), (dict(act=-1), "activation"), (dict(bias=P, bt=2), "bias_dtype"),
     (dict(bias=ODD), "aligned"), (dict(res=ODD), "aligned"), (dict(c=ODD), "aligned")])
 def test_epilogue_refusals(lib, call, bad, says):
@@ -159,6 +160,64 @@ def test_permute_workspace(lib):
     assert need > 0
     assert _permute(lib, t=4096, ws=None) == 4 and _permute(lib, t=4096, ws_bytes=need - 1) == 4 and _permute(lib, t=4096, ws=ODD) == 4
     assert f(1 << 24, 1024, 32) < 1 << 22  # the sorting workgroups are few, however many slots there are
+
+
+STAND_IN = test_host_block.STAND_IN + """
+f8, bf = "torch.float8_e4m3fn", "torch.bfloat16"
+def gemm(a=T([4, 128], f8), b=T([256, 128], f8), c=T([4, 256]), bias=None, res=None):
+    tk_kernel.dispatch_gemm_fp8_epilogue(a, b, c, None, None, bias, 1, res)
+def norm(x=T([4, 64]), w=T([64]), b=None, y=T([4, 64]), st=T([4, 4], f32), r=None, ro=None):
+    tk_kernel.dispatch_layer_norm(x, r, w, b, 1e-5, y, ro, st)
+def norm_grad(dy=T([400, 64]), r=T([400, 64]), w=T([64]), dr=None, st=T([400, 4], f32), dx=T([400, 64]), dw=T([64]), ws=T([1 << 20], u8)):
+    tk_kernel.dispatch_layer_norm_backward(dy, r, w, dr, st, dx, dw, None, ws)
+def permute(x=T([4, 64]), ids=T([4, 2], i32), xp=T([8, 64]), off=T([9], i32), perm=T([8], i32), inv=T([4, 2], i32)):
+    tk_kernel.dispatch_permute(x, ids, xp, off, perm, inv, None)
+def combine(y=T([8, 64]), w=T([4, 2], f32), off=T([9], i32), inv=T([4, 2], i32), out=T([4, 64])):
+    tk_kernel.dispatch_combine_rows(y, w, off, inv, out)
+def combine_grad(dout=T([4, 64]), y=T([8, 64]), w=T([4, 2], f32), off=T([9], i32), inv=T([4, 2], i32), dy=T([8, 64]), dw=T([4, 2], f32)):
+    tk_kernel.dispatch_combine_rows_backward(dout, y, w, off, inv, dy, dw)
+def route_grad(dw=T([4, 2], f32), w=T([4, 2], f32), idx=T([4, 2], i32), out=T([4, 8], f32)):
+    tk_kernel.dispatch_route_topk_backward(dw, w, idx, out)
+"""
+
+
+def test_tensors_of_another_device_and_shape(fake):
+    """What the binding asks of each tensor, and the stream that every launch goes to."""
+    out = hip_host.run(fake, STAND_IN + """
+for f in (gemm, norm, norm_grad, permute, combine, combine_grad, route_grad): f()
+for line in log(): print(line)
+other = dict(dev=1)
+refused(lambda: gemm(res=T([4, 256], **other)))
+refused(lambda: gemm(bias=T([256], dev=-1)))
+refused(lambda: gemm(bias=T([2, 128])))
+refused(lambda: gemm(c=T([4, 256], strides=(512, 1))))
+refused(lambda: norm(x=T([4, 64], **other)))
+refused(lambda: norm(st=T([4, 4])))
+refused(lambda: norm(r=T([4, 64])))
+refused(lambda: norm_grad(dy=T([400, 64], f32)))
+refused(lambda: norm_grad(ws=T([1 << 20], i32)))
+refused(lambda: permute(ids=T([4, 2], i32, **other)))
+refused(lambda: permute(xp=T([7, 64])))
+refused(lambda: permute(perm=T([8], f32)))
+refused(lambda: permute(inv=T([2, 4], i32)))
+refused(lambda: combine(w=T([4, 2])))
+refused(lambda: combine(off=T([9, 1], i32)))
+refused(lambda: combine_grad(dy=T([8, 64], strides=(128, 1))))
+refused(lambda: combine_grad(dw=T([4, 3], f32)))
+refused(lambda: route_grad(idx=T([4, 2], f32)))
+refused(lambda: route_grad(out=T([5, 8], f32)))
+""")
+    launches = [l for l in out if l.startswith("launch")]
+    assert len(launches) == 8 and all(l.endswith("stream=7") for l in launches), out
+    said = [l.split(": ", 1)[1] for l in out if l.startswith("refused")]
+    wanted = ["residual: tensor must be on the current device", "bias: tensor must be on a GPU device", "bias must be [N]",
+              "C: tensor must be contiguous", "x: tensor must be on the current device", "stats must be [R, 4] float32",
+              "residual and residual_out come together", "dy must have r's shape and dtype",
+              "workspace: expected dtype torch.uint8, got torch.int32", "ids: tensor must be on the current device",
+              "xp: expected [8, 64] torch.bfloat16", "perm: expected 8 int32 values", "ids must be [T, k] int32",
+              "topk_w: expected [4, 2] torch.float32", "offsets: expected 1-D tensor", "dy: tensor must be contiguous",
+              "dw: expected [4, 2] torch.float32", "topk_idx: expected dtype torch.int32", "dlogits: expected [4, 8] torch.float32"]
+    assert said == wanted and "taken" not in out, said
 
 
 # ---------------------------------------------------------------------------
