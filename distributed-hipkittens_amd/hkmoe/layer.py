@@ -71,6 +71,12 @@ def _activation(name):
     return _ACTIVATIONS[name]
 
 
+def _check_out(out, like):
+    """What the plain products' binding does not ask of C, which it takes to be new."""
+    if out is not None and (out.device != like.device or out.data_ptr() % 16):
+        raise RuntimeError("out must be on the operands' device, 16-byte aligned")
+
+
 def gemm_fp8(a_q, b_q, scale_a=None, scale_b=None, out_dtype=torch.bfloat16, bias=None, activation=None,
              residual=None, out=None):
     """C = act((sa*sb) A . B^T + bias) + residual for e4m3 A [M,K], B [N,K], in one launch.
@@ -84,6 +90,7 @@ def gemm_fp8(a_q, b_q, scale_a=None, scale_b=None, out_dtype=torch.bfloat16, bia
     act = _activation(activation)
     c = a_q.new_empty(a_q.shape[0], b_q.shape[0], dtype=out_dtype) if out is None else out
     if bias is None and activation is None and residual is None:
+        _check_out(out, a_q)
         tk_kernel.dispatch_gemm_fp8(a_q, b_q, c, scale_a, scale_b)
     else:
         tk_kernel.dispatch_gemm_fp8_epilogue(a_q, b_q, c, scale_a, scale_b, bias, act, residual)
@@ -121,6 +128,7 @@ def gemm_mx(a_q, a_packed, b_q, b_packed, out_dtype=torch.float32, bias=None, ac
     act = _activation(activation)
     c = a_q.new_empty(a_q.shape[0], b_q.shape[0], dtype=out_dtype) if out is None else out
     if bias is None and activation is None and residual is None:
+        _check_out(out, a_q)
         tk_kernel.dispatch_gemm_mx(a_q, a_packed, b_q, b_packed, c)
     else:
         tk_kernel.dispatch_gemm_mx_epilogue(a_q, a_packed, b_q, b_packed, c, bias, act, residual)

@@ -2,16 +2,15 @@
 choice, tokens sorted by expert and back, each with its gradient.
 
 Every operator comes in two forms.  ``layer_norm``, ``route_topk``, ``moe_permute`` and
-``moe_combine`` record gradients where an input asks for them.  The ``*_forward`` /
-``*_backward`` functions are the plain calls that those make, for programs that run
-their own backward pass or capture it into a graph.
+``moe_combine`` record gradients where an input asks for them (first derivatives only).  The
+``*_forward`` / ``*_backward`` functions are the plain calls that those make, on the current
+stream, for programs that run their own backward pass or capture it into a graph.
 """
 from typing import NamedTuple
 
 import torch
 
 import tk_kernel
-
 
 
 # ----------------------------------------------------------------------------
@@ -61,9 +60,9 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dr=None):
-        r, weight, stats = ctx.saved_tensors
         if dy is None:  # the norm has no use: the stream's own gradient is all there is
-            return dr, None, None, dr, None
+            return dr, None, None, dr if ctx.has_residual else None, None
+        r, weight, stats = ctx.saved_tensors
         dx, dw, db = layer_norm_backward(dy.contiguous(), r, weight, stats, None if dr is None else dr.contiguous(),
                                          ctx.has_bias)
         return dx, dw, db, dx if ctx.has_residual else None, None
@@ -109,11 +108,14 @@ class _RouteTopk(torch.autograd.Function):
         ctx.save_for_backward(idx, w)
         ctx.num_experts = logits.shape[1]
         ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)  # no zeros in idx's place
         return idx, w
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, _, dw):
+        if dw is None:
+            return None, None
         idx, w = ctx.saved_tensors
         return route_topk_backward(dw.contiguous(), w, idx, ctx.num_experts), None
 
@@ -182,11 +184,14 @@ class _Permute(torch.autograd.Function):
         xp, order = moe_permute_forward(x, ids, num_experts)
         ctx.save_for_backward(*order)
         ctx.mark_non_differentiable(*order)
+        ctx.set_materialize_grads(False)  # no zeros in the order's place
         return (xp, *order)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dxp, *_):
+        if dxp is None:
+            return None, None, None
         return moe_permute_backward(dxp.contiguous(), MoEOrder(*ctx.saved_tensors)), None, None
 
 

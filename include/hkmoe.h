@@ -87,7 +87,8 @@ int hkmoe_gemm_fp8(const void* a, const void* b, void* c, int64_t m, int64_t n, 
  *     HKMOE_ACT_GELU       z Phi(z), Phi the normal distribution function (the erf form)
  *     HKMOE_ACT_GELU_TANH  z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2
  *   to a few ulp of fp32; for large |z| the exponential costs more: (16 + z^2) 2^-23 of
- *   Phi(-|z|), (4 + |z|) 2^-23 of SiLU.  C, bias and residual 16-byte aligned, N <= 2^21.  hkmoe_set_dense_mfma does not apply.
+ *   Phi(-|z|), (4 + |z|) 2^-23 of SiLU.  C, bias and residual 16-byte aligned, N <= 2^21.
+ *   hkmoe_set_dense_mfma does not apply.
  * No reference counterpart (its GEMMs store C as it is).
  */
 enum hkmoe_activation {
@@ -509,7 +510,7 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
  *   residual_out both NULL: r = x.  residual_out may be x or residual; dx may be dr or dy;
  *   other outputs overlap nothing.  C % 8 == 0, C <= 16384, R <= 2^24.  R = 0 writes zeros to dweight
  *   and dbias.  workspace: hkmoe_layer_norm_backward_workspace_size(R, C) bytes (0 for sizes out of
- *   range), not shared by calls that overlap in time.
+ *   range, and for few rows, which need none), not shared by calls that overlap in time.
  * The same call gives the same bits; dweight's and dbias' last bits depend on R.
  */
 int hkmoe_layer_norm(const void* x, const void* residual, const void* weight, const void* bias, int64_t rows, int64_t cols,

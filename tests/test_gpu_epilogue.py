@@ -211,6 +211,27 @@ def test_refusals(hk):
                    torch.zeros((1, 256), dtype=torch.int32, device="cuda"), activation="relu")
 
 
+def test_out_of_the_plain_products(hk):
+    """C in a given tensor, without an epilogue as well; one that the stores would not fit is refused."""
+    aq = torch.ones((4, 128), device="cuda").to(torch.float8_e4m3fn)
+    bq = torch.ones((256, 128), device="cuda").to(torch.float8_e4m3fn)
+    sa = hk.mx_pack_scales(torch.full((4, 4), 127, dtype=torch.uint8, device="cuda"))
+    sb = hk.mx_pack_scales(torch.full((256, 4), 127, dtype=torch.uint8, device="cuda"))
+    for call in (lambda out: hk.gemm_fp8(aq, bq, out=out), lambda out: hk.gemm_mx(aq, sa, bq, sb, out=out)):
+        for dtype in (BF16, F32):
+            buf = torch.zeros((6, 256), device="cuda", dtype=dtype)
+            assert call(buf[1:5]).data_ptr() == buf[1:5].data_ptr()
+            assert bool((buf[1:5] == 128).all()) and not buf[0].any() and not buf[5].any()
+            with pytest.raises(RuntimeError, match="aligned"):
+                call(buf.view(-1)[1:1025].view(4, 256))
+            with pytest.raises(RuntimeError, match="device"):
+                call(torch.zeros((4, 256), dtype=dtype))
+        with pytest.raises(RuntimeError):
+            call(torch.zeros((3, 256), device="cuda"))
+        with pytest.raises(RuntimeError):
+            call(torch.zeros((4, 256), device="cuda", dtype=torch.float16))
+
+
 def test_streams_and_graph(hk):
     """Calls on two streams at once, and replays of a captured call with changing inputs, next to
     eager work."""

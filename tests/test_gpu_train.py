@@ -465,6 +465,18 @@ def test_block_gradients(hk):
         assert float((got.detach().double() - v).norm() / v.norm()) < 1e-4
 
 
+class _Undefined(torch.autograd.Function):
+    """Passes a value on and no gradient back."""
+
+    @staticmethod
+    def forward(ctx, t):
+        return t.clone()
+
+    @staticmethod
+    def backward(ctx, _):
+        return None
+
+
 def test_gradients_only_where_asked(hk):
     """Frozen inputs get none; without a graph nothing is recorded; dbias without a bias is none; a
     broadcast or strided output gradient is taken as it is."""
@@ -490,6 +502,11 @@ def test_gradients_only_where_asked(hk):
     gx, _ = torch.autograd.grad((y * y).sum(), [xr, w])
     y2, r2, stats2 = hk.layer_norm_forward(x, w.detach(), None, x)
     assert torch.equal(gx, hk.layer_norm_backward(2 * y2, r2, w.detach(), stats2)[0])
+    ids = torch.zeros((6, 2), device="cuda", dtype=torch.int32)
+    logits = torch.randn((6, 9), device="cuda", requires_grad=True)
+    xs = x.clone().requires_grad_()
+    for leaf, out in ((xs, hk.moe_permute(xs, ids, 9)[0]), (logits, hk.route_topk(logits, 2)[1])):
+        assert torch.autograd.grad(_Undefined.apply(out).sum(), leaf, allow_unused=True) == (None,)
     idx, tw = hk.route_topk(torch.randn((6, 9), device="cuda", requires_grad=True), 2)
     assert tw.requires_grad and not idx.requires_grad
     xp, order = hk.moe_permute(x, idx, 9)
