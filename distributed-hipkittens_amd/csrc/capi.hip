@@ -716,28 +716,39 @@ int launch_layer_norm(const LayerNormParams& p, hipStream_t s) {
 //   8192x7168 bf16    94 /  99 / 104 / 111     16384x1024 bf16  45 / 34 / 31 / 38
 //   4096x4096 bf16    35 /  32 /  34 /  38     1999x2560 fp32   16 / 18 / 19 / 22
 int layer_norm_parts(int64_t rows, int64_t cols) {
-  int per = 1, each = 8, threads = 0, few = 4;  // rows at a time, turns for each slot, turns that one workgroup takes
+  int per = 1, each = 8, threads = 0;  // rows at a time, turns for each slot
   (void)with_layer_norm_shape(cols, [&](auto ch, auto lanes) {
     constexpr int LANES = decltype(lanes)::value;
     per = kLnRowThreads / (LANES ? LANES : kLnRowThreads);
     each = LANES ? 5 : 8;
     threads = LANES ? kLnRowThreads : row_threads(cols, decltype(ch)::value);
-    few = decltype(ch)::value == 4 ? 1 : 4;
     return HKMOE_OK;
   });
-  // one workgroup writes dw and db itself, without a workspace or a second launch (4 rows of 4096: 7.4 us a
-  // call, 5 rows in two launches 11.1; 4 rows of 16384 17.1 and 11.4, so wide rows only alone)
-  if (rows <= few * per) return 1;
   const int64_t fill = kLnParts * std::clamp(1024 / threads, 1, 3);
   return static_cast<int>(std::min((rows + per - 1) / per, std::max<int64_t>(kLnParts, std::min(fill, rows / (per * each)))));
 }
 
+// The gradient in one launch, dw and db in workgroups of their own, which read r and dy once more.  us a call
+// (as a graph), bf16, two launches / one:
+//   64 x 128 12.7 / 8.6 (4.9 / 3.3)      512 x 1024 13.2 / 8.4 (8.6 / 6.6)    1024 x 1024 13.0 / 10.4 (7.9 / 10.1)
+//   4 x 4096 12.8 / 8.5 (5.3 / 3.2)      512 x 4096 13.0 / 8.2 (12.0 / 5.8)   2048 x 4096 18.6 / 23.0
+//   64 x 16384 15.3 / 8.4 (14.8 / 7.6)   1024 x 8192 19.3 / 16.2              1024 x 16384 41.9 / 38.0
+// and fp32, 512 x 8192 19.5 / 16.4, 1024 x 8192 28.8 / 30.3.
+bool layer_norm_in_one(int64_t rows, int64_t cols) { return rows <= (cols > 4096 ? 1024 : 512); }
+
 template <bool F32>
-int launch_layer_norm_grad(const LayerNormGradParams& p, hipStream_t s) {
+int launch_layer_norm_grad(LayerNormGradParams p, hipStream_t s) {
   return with_layer_norm_shape(p.cols, [&](auto ch, auto lanes) {
     constexpr int CH = decltype(ch)::value, LANES = decltype(lanes)::value;
     const int threads = LANES ? kLnRowThreads : row_threads(p.cols, CH);
-    hipLaunchKernelGGL((layer_norm_grad_kernel<F32, CH, LANES>), dim3(layer_norm_parts(p.rows, p.cols)), dim3(threads), 0, s, p);
+    if (layer_norm_in_one(p.rows, p.cols)) {
+      constexpr int rows = kLnRowThreads / (LANES ? LANES : kLnRowThreads);  // of a workgroup
+      p.col_groups = (p.cols + 63) / 64;
+      const int64_t grid = p.col_groups + (p.rows + rows - 1) / rows;
+      hipLaunchKernelGGL((layer_norm_grad_kernel<F32, CH, LANES, true>), dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, p);
+    } else {
+      hipLaunchKernelGGL((layer_norm_grad_kernel<F32, CH, LANES, false>), dim3(layer_norm_parts(p.rows, p.cols)), dim3(threads), 0, s, p);
+    }
     return check_launch("layer_norm_grad_kernel");
   });
 }
@@ -1809,8 +1820,7 @@ int hkmoe_rms_norm_quant(const void* x, const void* residual, const void* weight
 
 size_t hkmoe_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
   if (rows <= 0 || rows > kMaxRows || cols <= 0 || cols > kLnMaxCols) return 0;
-  const int parts = layer_norm_parts(rows, cols);
-  return parts == 1 ? 0 : align256(static_cast<size_t>(parts) * 2 * cols * sizeof(float));
+  return layer_norm_in_one(rows, cols) ? 0 : align256(static_cast<size_t>(layer_norm_parts(rows, cols)) * 2 * cols * sizeof(float));
 }
 
 // What both directions ask of the sizes and types.
@@ -1855,6 +1865,7 @@ int hkmoe_layer_norm_backward(const void* dy, const void* r, const void* weight,
                               void* dbias, void* workspace, size_t workspace_bytes, hkmoe_stream_t stream) {
   HK_TRY(layer_norm_check("layer_norm_backward", rows, cols, x_dtype, weight_dtype));
   HK_REQUIRE(weight && dweight && (rows == 0 || (dy && r && stats && dx)), "layer_norm_backward: null pointer");
+  HK_REQUIRE(rows == 0 || (dx != dy && dx != r), "layer_norm_backward: dx must be neither dy nor r");  // read for dweight meanwhile
   HK_REQUIRE(aligned16(dy) && aligned16(r) && aligned16(weight) && aligned16(dr) && aligned16(stats) && aligned16(dx) &&
                  aligned16(dweight) && aligned16(dbias),
              "layer_norm_backward: tensors must be 16-byte aligned");
@@ -1868,7 +1879,7 @@ int hkmoe_layer_norm_backward(const void* dy, const void* r, const void* weight,
   p.dr = dr;
   p.stats = reinterpret_cast<const f32x4*>(stats);
   p.dx = dx;
-  p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  p.part = static_cast<float*>(workspace);
   p.dw = dweight;
   p.db = dbias;
   p.rows = rows;

@@ -13,8 +13,9 @@
 // terms, because one would cost r - m as many bits as |m| is larger than its spread.
 // Backward: the row's two sums in fp32, and in the same pass every thread's own
 // columns of dw and db over the workgroup's rows, in registers; one partial per
-// workgroup goes to the workspace and a second launch adds them in order, in 64 bits (a few rows
-// take one workgroup, and no second launch).
+// workgroup goes to the workspace and a second launch adds them in order, in 64 bits.  While rows
+// are few, a launch costs more than their bytes: there dw and db, which need no sums over a row
+// (n comes from the forward pass's stats), get workgroups of their own beside the rows'.
 // Nothing is added atomically: the same call gives the same bits.
 #pragma once
 
@@ -50,12 +51,13 @@ struct LayerNormGradParams {
   const void* dr;      // may be null
   const f32x4* stats;
   void* dx;
-  float* part;  // [gridDim.x][2][cols], or null with one workgroup, which writes dw and db itself
+  float* part;  // [gridDim.x][2][cols] (not COLS)
   void* dw;
   void* db;  // may be null
   int64_t rows;
   int32_t cols;
   int32_t w_f32;
+  int32_t col_groups;  // COLS: workgroups of 64 columns, in front of the rows'
 };
 
 // Threads of a row: LANES lanes of a wave (one wave's rows need no barrier), or with
@@ -247,16 +249,67 @@ __device__ __forceinline__ void put_sum(void* to, int j, float v, int w_f32) {
     static_cast<uint16_t*>(to)[j] = static_cast<uint16_t>(bf16_rne_bits(v));
 }
 
+// dw and db of columns 64 blockIdx.x .. + 63 over all rows: 8 lanes of 8 columns to a row, the lanes'
+// sums and then the waves' added in order.
+template <bool F32>
+__device__ __forceinline__ void layer_norm_grad_cols(const LayerNormGradParams& p) {
+  __shared__ float red[kNormMaxThreads / kWave][128];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x / kWave;
+  const int j = blockIdx.x * 64 + (lane & 7) * kNormChunk;
+  F8v dw{}, db{};
+  if (j < p.cols) {
+#pragma unroll 4
+    for (int64_t row = wave * 8 + (lane >> 3); row < p.rows; row += waves * 8) {
+      const f32x4 st = p.stats[row];
+      Raw8<F32> r, dy;
+      r.load(p.r, row * p.cols + j);
+      dy.load(p.dy, row * p.cols + j);
+      const F8v x = r.get(), d = dy.get();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dw.v[i] = __builtin_fmaf(d.v[i], ((x.v[i] - st.x) - st.y) * st.z, dw.v[i]);
+        db.v[i] += d.v[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int o = 8; o <= 32; o <<= 1) {
+      dw.v[i] += __shfl_xor(dw.v[i], o, kWave);
+      db.v[i] += __shfl_xor(db.v[i], o, kWave);
+    }
+  }
+  if (lane < 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      red[wave][lane * 8 + i] = dw.v[i];
+      red[wave][64 + lane * 8 + i] = db.v[i];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63);
+    float s = 0.0f;
+    for (int w = 0; w < waves; ++w) s += red[w][threadIdx.x];
+    if (col < p.cols) put_sum(threadIdx.x < 64 ? p.dw : p.db, col, s, p.w_f32);
+  }
+}
+
 // Rows blockIdx.x * rows per workgroup, + gridDim.x * that, ...; the next row is loaded
-// before the sums of this one are waited for (kAhead).
-template <bool F32, int CH, int LANES>
+// before the sums of this one are waited for (kAhead).  COLS: dw and db in workgroups of their own.
+template <bool F32, int CH, int LANES, bool COLS>
 __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_grad_kernel(LayerNormGradParams p) {
+  const int first = COLS ? p.col_groups : 0;
+  if constexpr (COLS) {
+    if (static_cast<int>(blockIdx.x) < first) return layer_norm_grad_cols<F32>(p);
+  }
   __shared__ float red[2][LANES == 0 ? kNormMaxThreads / kWave : 1][2];
   // wide rows leave no registers for a row ahead, nor for keeping g and n
   constexpr bool kAhead = LANES != 0 || CH == 1;
   const int cols = p.cols;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * ln_rows<LANES>();
-  int64_t row = static_cast<int64_t>(blockIdx.x) * ln_rows<LANES>() + ln_slot<LANES>();
+  const int64_t step = static_cast<int64_t>(gridDim.x - first) * ln_rows<LANES>();
+  int64_t row = static_cast<int64_t>(blockIdx.x - first) * ln_rows<LANES>() + ln_slot<LANES>();
   const float inv_n = 1.0f / static_cast<float>(cols);
   F8v dw[CH], db[CH];
   Raw8<F32> r[CH], dy[CH];
@@ -306,8 +359,10 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_grad_kernel(
         terms(c, g[c], n[c], d);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          dw[c].v[i] = __builtin_fmaf(d.v[i], n[c].v[i], dw[c].v[i]);
-          db[c].v[i] += d.v[i];
+          if constexpr (!COLS) {
+            dw[c].v[i] = __builtin_fmaf(d.v[i], n[c].v[i], dw[c].v[i]);
+            db[c].v[i] += d.v[i];
+          }
           s1 += g[c].v[i];
           s2 = __builtin_fmaf(g[c].v[i], n[c].v[i], s2);
         }
@@ -335,22 +390,15 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_grad_kernel(
     }
     if constexpr (!kAhead) load(row + step);
   }
+  if constexpr (COLS) return;
   float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * cols;
   if constexpr (LANES == 0) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int j = ln_col<LANES>(c);
       if (j < cols) {
-        if (p.part != nullptr) {
-          store8<true>(part, j, dw[c]);
-          store8<true>(part, cols + j, db[c]);
-        } else if (p.w_f32) {
-          store8<true>(p.dw, j, dw[c]);
-          if (p.db != nullptr) store8<true>(p.db, j, db[c]);
-        } else {
-          store8<false>(p.dw, j, dw[c]);
-          if (p.db != nullptr) store8<false>(p.db, j, db[c]);
-        }
+        store8<true>(part, j, dw[c]);
+        store8<true>(part, cols + j, db[c]);
       }
     }
   } else {
@@ -367,12 +415,7 @@ __global__ __launch_bounds__(ln_threads(CH, LANES)) void layer_norm_grad_kernel(
         const int l = u / 8, j = ((c % CH) * LANES + l) * kNormChunk + u % 8;
         float s = 0.0f;
         for (int q = 0; q < kLnRowThreads / LANES; ++q) s += meet[q * LANES + l][u % 8];
-        if (j < cols) {
-          if (p.part != nullptr)
-            part[(c < CH ? 0 : cols) + j] = s;
-          else
-            put_sum(c < CH ? p.dw : p.db, j, s, p.w_f32);
-        }
+        if (j < cols) part[(c < CH ? 0 : cols) + j] = s;
       }
     }
   }

@@ -507,7 +507,7 @@ int hkmoe_lora_add(const void* y, int64_t y_stride, const void* x, int64_t x_str
  *     comes back along the new stream.
  *   x, residual, residual_out, y, dy, r, dr, dx [R, C] bf16 or fp32 (x_dtype); weight, bias,
  *   dweight, dbias [C] bf16 or fp32 (weight_dtype); bias and dbias may be NULL.  residual and
- *   residual_out both NULL: r = x.  residual_out may be x or residual; dx may be dr or dy;
+ *   residual_out both NULL: r = x.  residual_out may be x or residual; dx may be dr;
  *   other outputs overlap nothing.  C % 8 == 0, C <= 16384, R <= 2^24.  R = 0 writes zeros to dweight
  *   and dbias.  workspace: hkmoe_layer_norm_backward_workspace_size(R, C) bytes (0 for sizes out of
  *   range, and for few rows, which need none), not shared by calls that overlap in time.

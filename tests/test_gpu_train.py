@@ -55,7 +55,9 @@ def _norm_case(hk, rows, cols, dtype, wdtype, residual=True, bias=True, dr=True,
     got = hk.layer_norm_backward(dy, r, w, stats, dr=back, with_bias=bias)
     torch.cuda.synchronize()
     args = (dy.double(), r64, w64, eps, None if back is None else back.double())
-    each = max(4, math.ceil(rows / PARTS)) + 16
+    # additions behind each other: a part's rows, or a lane's share of up to 512 rows in 24 or 1024 in 64 (22,
+    # 16); and then 8 to 16 parts or lanes and waves
+    each = max(22, math.ceil(rows / PARTS)) + 16
     for name, g, v, bd in zip(("dx", "dw", "db"), got, ref.layer_norm_grad(*args), ref.layer_norm_grad_bound(*args, dtype, wdtype, each)):
         if name == "db" and not bias:
             assert g is None
@@ -75,6 +77,12 @@ def test_norm_widths(hk, cols, dtype, rows):
 def test_norm_rows(hk, rows, cols):
     _norm_case(hk, rows, cols, (BF16, F32)[rows % 2], F32, residual=rows % 3 != 0, bias=rows % 5 != 0, dr=rows % 2 == 0,
                in_place=rows % 2 == 1)
+
+
+@pytest.mark.parametrize("rows", [511, 512, 513, 1023, 1024, 1025])
+@pytest.mark.parametrize("cols", [72, 520, 1160, 4096, 4104, 8200])
+def test_norm_rows_where_launches_change(hk, rows, cols):
+    _norm_case(hk, rows, cols, (BF16, F32)[cols // 8 % 2], (BF16, F32)[rows % 2], residual=False, bias=rows % 2 == 0)
 
 
 @pytest.mark.parametrize("cols", [64, 1000, 4096, 10000])
@@ -138,19 +146,21 @@ def test_norm_no_rows(hk):
 
 
 def test_norm_gradient_in_place(hk):
-    """dx over dr and over dy, as the C entry point allows."""
-    for cols in (256, 4096, 9000):
-        x, w, b, gen = _norm_inputs(300, cols, BF16, BF16, 5)
-        y, r, stats = hk.layer_norm_forward(x, w, b)
-        dy, dr = _randn(gen, 300, cols).to(BF16), _randn(gen, 300, cols).to(BF16)
-        want = hk.layer_norm_backward(dy, r, w, stats, dr=dr)
-        need = hk.tk_kernel.layer_norm_backward_workspace_size(300, cols)
-        for which in (0, 1):
-            t = [dy.clone(), dr.clone()]
-            dw, db = torch.empty_like(w), torch.empty_like(w)
-            hk.tk_kernel.dispatch_layer_norm_backward(t[0], r, w, t[1], stats, t[which], dw, db,
-                                                      torch.empty(need, dtype=torch.uint8, device="cuda"))
-            assert torch.equal(t[which], want[0]) and torch.equal(dw, want[1]) and torch.equal(db, want[2])
+    """dx over dr, as the C entry point allows; over dy and r, which others still read, it is refused."""
+    for rows in (300, 3000):
+        for cols in (256, 4096, 9000):
+            x, w, b, gen = _norm_inputs(rows, cols, BF16, BF16, 5)
+            y, r, stats = hk.layer_norm_forward(x, w, b)
+            dy, dr = _randn(gen, rows, cols).to(BF16), _randn(gen, rows, cols).to(BF16)
+            want = hk.layer_norm_backward(dy, r, w, stats, dr=dr)
+            need = hk.tk_kernel.layer_norm_backward_workspace_size(rows, cols)
+            dw, db, ws = torch.empty_like(w), torch.empty_like(w), torch.empty(need, dtype=torch.uint8, device="cuda")
+            dx = dr.clone()
+            hk.tk_kernel.dispatch_layer_norm_backward(dy, r, w, dx, stats, dx, dw, db, ws)
+            assert torch.equal(dx, want[0]) and torch.equal(dw, want[1]) and torch.equal(db, want[2])
+            for bad in (dy, r):
+                with pytest.raises(RuntimeError, match="neither dy nor r"):
+                    hk.tk_kernel.dispatch_layer_norm_backward(dy, r, w, dr, stats, bad, dw, db, ws)
 
 
 def test_norm_far_rows(hk):

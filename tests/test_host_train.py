@@ -14,6 +14,7 @@ import test_host_block
 import train_ref as ref
 
 P = ctypes.c_void_p(0x1000)  # never dereferenced: validation fails first
+Q = ctypes.c_void_p(0x2000)
 ODD = ctypes.c_void_p(0x1008)
 i64, i32, dbl, size = ctypes.c_int64, ctypes.c_int32, ctypes.c_double, ctypes.c_size_t
 
@@ -68,7 +69,7 @@ def _norm(lib, x=P, residual=None, weight=P, bias=None, rows=4, cols=256, xt=0, 
     return lib.hkmoe_layer_norm(x, residual, weight, bias, i64(rows), i64(cols), xt, wt, dbl(eps), y, residual_out, stats, None)
 
 
-def _norm_grad(lib, dy=P, r=P, weight=P, dr=None, stats=P, rows=4, cols=256, xt=0, wt=0, dx=P, dw=P, db=None, ws=P, ws_bytes=1 << 40):
+def _norm_grad(lib, dy=P, r=P, weight=P, dr=None, stats=P, rows=4, cols=256, xt=0, wt=0, dx=Q, dw=P, db=None, ws=P, ws_bytes=1 << 40):
     return lib.hkmoe_layer_norm_backward(dy, r, weight, dr, stats, i64(rows), i64(cols), xt, wt, dx, dw, db, ws, size(ws_bytes), None)
 
 
@@ -86,16 +87,16 @@ def test_norm_refusals(lib, bad, says):
     (dict(dy=None), "null"), (dict(r=None), "null"), (dict(weight=None), "null"), (dict(stats=None), "null"), (dict(dx=None), "null"),
     (dict(dw=None), "null"), (dict(rows=-1), "shape"), (dict(cols=4), "multiple of 8"), (dict(cols=16392), "16384"), (dict(xt=3), "dtype"),
     (dict(wt=-1), "dtype"), (dict(dy=ODD), "aligned"), (dict(dr=ODD), "aligned"), (dict(dx=ODD), "aligned"), (dict(dw=ODD), "aligned"),
-    (dict(db=ODD), "aligned")])
+    (dict(db=ODD), "aligned"), (dict(dx=P), "neither dy nor r"), (dict(dx=P, dy=Q), "neither dy nor r"), (dict(dx=P, r=Q), "neither dy nor r")])
 def test_norm_gradient_refusals(lib, bad, says):
     _refused(lib, _norm_grad, bad, says)
 
 
 def test_norm_workspace(lib):
-    need = lib.hkmoe_layer_norm_backward_workspace_size(i64(400), i64(256))
-    assert need > 0 and lib.hkmoe_layer_norm_backward_workspace_size(i64(4), i64(256)) == 0  # one workgroup
+    need = lib.hkmoe_layer_norm_backward_workspace_size(i64(600), i64(256))
+    assert need > 0 and lib.hkmoe_layer_norm_backward_workspace_size(i64(4), i64(256)) == 0  # one launch
     for bad in (dict(ws=None), dict(ws_bytes=need - 1), dict(ws=ODD)):
-        assert _norm_grad(lib, rows=400, **bad) == 4
+        assert _norm_grad(lib, rows=600, **bad) == 4
     for rows, cols in ((0, 256), (-1, 256), (2 ** 62, 256), (4, 0), (4, 2 ** 62), (4, 16392)):
         assert lib.hkmoe_layer_norm_backward_workspace_size(i64(rows), i64(cols)) == 0
     assert lib.hkmoe_layer_norm_backward_workspace_size(i64(1 << 24), i64(16384)) >= 2 * 16384 * 4
@@ -163,12 +164,14 @@ def test_permute_workspace(lib):
 
 
 STAND_IN = test_host_block.STAND_IN + """
+class There(T):
+    def data_ptr(self): return 0x2000
 f8, bf = "torch.float8_e4m3fn", "torch.bfloat16"
 def gemm(a=T([4, 128], f8), b=T([256, 128], f8), c=T([4, 256]), bias=None, res=None):
     tk_kernel.dispatch_gemm_fp8_epilogue(a, b, c, None, None, bias, 1, res)
 def norm(x=T([4, 64]), w=T([64]), b=None, y=T([4, 64]), st=T([4, 4], f32), r=None, ro=None):
     tk_kernel.dispatch_layer_norm(x, r, w, b, 1e-5, y, ro, st)
-def norm_grad(dy=T([400, 64]), r=T([400, 64]), w=T([64]), dr=None, st=T([400, 4], f32), dx=T([400, 64]), dw=T([64]), ws=T([1 << 20], u8)):
+def norm_grad(dy=T([600, 64]), r=T([600, 64]), w=T([64]), dr=None, st=T([600, 4], f32), dx=There([600, 64]), dw=T([64]), ws=T([1 << 20], u8)):
     tk_kernel.dispatch_layer_norm_backward(dy, r, w, dr, st, dx, dw, None, ws)
 def permute(x=T([4, 64]), ids=T([4, 2], i32), xp=T([8, 64]), off=T([9], i32), perm=T([8], i32), inv=T([4, 2], i32)):
     tk_kernel.dispatch_permute(x, ids, xp, off, perm, inv, None)
@@ -224,10 +227,11 @@ refused(lambda: route_grad(out=T([5, 8], f32)))
 # launches
 # ---------------------------------------------------------------------------
 LAUNCH = """
+Q = ctypes.c_void_p(0x2000)
 size, dbl = ctypes.c_size_t, ctypes.c_double
 def norm(rows, cols, xt=0):
     assert lib.hkmoe_layer_norm(P, P, P, P, i64(rows), i64(cols), xt, 0, dbl(1e-5), P, P, P, None) == 0, lib.hkmoe_last_error()
-    assert lib.hkmoe_layer_norm_backward(P, P, P, P, P, i64(rows), i64(cols), xt, 0, P, P, P, P, size(1 << 50), None) == 0
+    assert lib.hkmoe_layer_norm_backward(P, P, P, P, P, i64(rows), i64(cols), xt, 0, Q, P, P, P, size(1 << 50), None) == 0
 def tokens(t, e, k, h, dt=0):
     assert lib.hkmoe_permute(P, P, i64(t), i32(e), i32(k), i64(h), dt, P, P, P, P, P, size(1 << 50), None) == 0
     assert lib.hkmoe_combine_rows(P, P, P, P, i64(t), i32(e), i32(k), i64(h), dt, P, None) == 0
@@ -257,7 +261,7 @@ for line in log(): print(line)
 """)
     launches = [l for l in out if l.startswith("launch")]
     names = {l.split()[1] for l in launches}
-    assert len([n for n in names if "layer_norm_kernel" in n]) == 12 and len([n for n in names if "layer_norm_grad_kernel" in n]) == 12
+    assert len([n for n in names if "layer_norm_kernel" in n]) == 12 and len([n for n in names if "layer_norm_grad_kernel" in n]) == 24
     for l in launches:
         v = {k: int(n) for k, n in (f.split("=") for f in l.split()[2:])}
         assert 1 <= v["grid"] and v["grid"] * v["threads"] < 1 << 32 and v["y"] == v["z"] == 1 and 64 <= v["threads"] <= 1024, l
@@ -283,13 +287,13 @@ for line in log(): print(line)
 
 
 def test_few_rows_need_one_launch_for_the_gradient(fake):
-    """Four turns of one workgroup's rows (16 lanes to a row of 128 columns: 16 rows a turn), and one more."""
+    """Workgroups for the columns beside the rows', and past some rows partial sums and a second launch."""
     out = hip_host.run(fake, LAUNCH + """
-for rows, cols in ((1, 4096), (4, 4096), (64, 128), (1, 16384), (5, 4096), (65, 128), (2, 16384), (0, 128)):
-    assert lib.hkmoe_layer_norm_backward(P, P, P, P, P, i64(rows), i64(cols), 0, 0, P, P, P, P, size(1 << 50), None) == 0
+for rows, cols in ((1, 4096), (512, 4096), (512, 128), (1024, 4104), (1024, 16384), (513, 4096), (513, 128), (1025, 16384), (0, 128)):
+    assert lib.hkmoe_layer_norm_backward(P, P, P, P, P, i64(rows), i64(cols), 0, 0, Q, P, P, P, size(1 << 50), None) == 0
     print(len(log()))
 """)
-    assert [int(v) for v in out] == [1, 1, 1, 1, 2, 2, 2, 1]
+    assert [int(v) for v in out] == [1, 1, 1, 1, 1, 2, 2, 2, 1]
 
 
 def test_small_batches_sort_in_one_launch(fake):
