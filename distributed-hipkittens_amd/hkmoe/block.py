@@ -2,7 +2,7 @@
 makes their operands, the router's product, and the adapters added beside a
 projection; and the two places where a model calls them together.
 
-Serving only, as the rest of the package: nothing here records gradients.
+Serving only: nothing here records gradients (:mod:`hkmoe.train` does).
 """
 import torch
 
