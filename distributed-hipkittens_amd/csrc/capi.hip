@@ -690,7 +690,7 @@ int with_layer_norm_shape(int64_t cols, F&& f) {
   if (cols <= 512) return f(integral_constant<int, 1>{}, integral_constant<int, 64>{});
   if (cols <= 1024) return f(integral_constant<int, 2>{}, integral_constant<int, 64>{});
   if (cols <= kNormMaxThreads * kNormChunk) return f(integral_constant<int, 1>{}, integral_constant<int, 0>{});
-  return f(integral_constant<int, 4>{}, integral_constant<int, 0>{});
+  return f(integral_constant<int, 2>{}, integral_constant<int, 0>{});
 }
 
 // Threads of a workgroup that has a whole row of `ch` chunks a thread.
@@ -732,25 +732,25 @@ int layer_norm_parts(int64_t rows, int64_t cols) {
 // (as a graph), bf16, two launches / one:
 //   64 x 128 12.7 / 8.6 (4.9 / 3.3)      512 x 1024 13.2 / 8.4 (8.6 / 6.6)    1024 x 1024 13.0 / 10.4 (7.9 / 10.1)
 //   4 x 4096 12.8 / 8.5 (5.3 / 3.2)      512 x 4096 13.0 / 8.2 (12.0 / 5.8)   2048 x 4096 18.6 / 23.0
-//   64 x 16384 15.3 / 8.4 (14.8 / 7.6)   1024 x 8192 19.3 / 16.2              1024 x 16384 41.9 / 38.0
+//   1024 x 8192 19.3 / 16.2              1024 x 16384 36.5 / 35.0
 // and fp32, 512 x 8192 19.5 / 16.4, 1024 x 8192 28.8 / 30.3.
 bool layer_norm_in_one(int64_t rows, int64_t cols) { return rows <= (cols > 4096 ? 1024 : 512); }
 
-template <bool F32>
+template <bool F32, bool COLS>
 int launch_layer_norm_grad(LayerNormGradParams p, hipStream_t s) {
   return with_layer_norm_shape(p.cols, [&](auto ch, auto lanes) {
     constexpr int CH = decltype(ch)::value, LANES = decltype(lanes)::value;
+    constexpr int rows = kLnRowThreads / (LANES ? LANES : kLnRowThreads);  // of a workgroup
     const int threads = LANES ? kLnRowThreads : row_threads(p.cols, CH);
-    if (layer_norm_in_one(p.rows, p.cols)) {
-      constexpr int rows = kLnRowThreads / (LANES ? LANES : kLnRowThreads);  // of a workgroup
-      p.col_groups = (p.cols + 63) / 64;
-      const int64_t grid = p.col_groups + (p.rows + rows - 1) / rows;
-      hipLaunchKernelGGL((layer_norm_grad_kernel<F32, CH, LANES, true>), dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, p);
-    } else {
-      hipLaunchKernelGGL((layer_norm_grad_kernel<F32, CH, LANES, false>), dim3(layer_norm_parts(p.rows, p.cols)), dim3(threads), 0, s, p);
-    }
+    p.col_groups = COLS ? (p.cols + 63) / 64 : 0;
+    const int64_t grid = COLS ? p.col_groups + (p.rows + rows - 1) / rows : layer_norm_parts(p.rows, p.cols);
+    hipLaunchKernelGGL((layer_norm_grad_kernel<F32, CH, LANES, COLS>), dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, p);
     return check_launch("layer_norm_grad_kernel");
   });
+}
+template <bool F32>
+int launch_layer_norm_grad(const LayerNormGradParams& p, hipStream_t s) {
+  return layer_norm_in_one(p.rows, p.cols) ? launch_layer_norm_grad<F32, true>(p, s) : launch_layer_norm_grad<F32, false>(p, s);
 }
 
 // ---------------------------------------------------------------------------

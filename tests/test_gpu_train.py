@@ -55,8 +55,8 @@ def _norm_case(hk, rows, cols, dtype, wdtype, residual=True, bias=True, dr=True,
     got = hk.layer_norm_backward(dy, r, w, stats, dr=back, with_bias=bias)
     torch.cuda.synchronize()
     args = (dy.double(), r64, w64, eps, None if back is None else back.double())
-    # additions behind each other: a part's rows, or a lane's share of up to 512 rows in 24 or 1024 in 64 (22,
-    # 16); and then 8 to 16 parts or lanes and waves
+    # additions behind each other: a part's rows, or a lane's share of up to 512 rows in 24 or 1024 in 72 (22,
+    # 15); and then 8 to 16 parts or lanes and waves
     each = max(22, math.ceil(rows / PARTS)) + 16
     for name, g, v, bd in zip(("dx", "dw", "db"), got, ref.layer_norm_grad(*args), ref.layer_norm_grad_bound(*args, dtype, wdtype, each)):
         if name == "db" and not bias:
