@@ -190,11 +190,10 @@ std::atomic<int> g_dense_mfma{32};
 
 // The dense GEMM on 128x128 tiles (gemm_small.hpp): one workgroup per tile,
 // the grid a whole number of 4x8 tile blocks.
-template <bool MX, typename K>
-int launch_tile128(K kern, bool (&attr_set)[kMaxDevices], const SmallGemmParams& p, hipStream_t stream) {
+template <typename K>
+int launch_tile128(K kern, int lds, bool (&attr_set)[kMaxDevices], const SmallGemmParams& p, hipStream_t stream) {
   int dev = 0;
   (void)hipGetDevice(&dev);
-  constexpr int lds = sm_lds_bytes(MX);
   if (dev >= 0 && dev < kMaxDevices && !attr_set[dev]) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -208,18 +207,23 @@ int launch_tile128(K kern, bool (&attr_set)[kMaxDevices], const SmallGemmParams&
 template <bool F32OUT, bool M32, bool MX>
 int launch_gemm_small(const SmallGemmParams& p, hipStream_t stream) {
   static bool attr_set[kMaxDevices] = {false};
-  return launch_tile128<MX>(gemm_fp8_small<F32OUT, M32, MX>, attr_set, p, stream);
+  return launch_tile128(gemm_fp8_small<F32OUT, M32, MX>, sm_lds_bytes(MX), attr_set, p, stream);
 }
 // With an epilogue: bf16 C on the FP8 instructions, fp32 C on the bf16 ones.
 template <bool MX>
 int launch_gemm_small_act(const SmallGemmParams& p, hipStream_t stream) {
   static bool attr_set[kMaxDevices] = {false};
-  return launch_tile128<MX>(gemm_fp8_small_act<MX>, attr_set, p, stream);
+  return launch_tile128(gemm_fp8_small_act<MX>, sm_lds_bytes(MX), attr_set, p, stream);
 }
 template <bool MX>
 int launch_gemm_wide(const SmallGemmParams& p, hipStream_t stream) {
   static bool attr_set[kMaxDevices] = {false};
-  return launch_tile128<MX>(gemm_fp8_wide<MX>, attr_set, p, stream);
+  return launch_tile128(gemm_fp8_wide<MX>, sm_lds_bytes(MX), attr_set, p, stream);
+}
+template <bool MX>
+int launch_gemm_wide256(const SmallGemmParams& p, hipStream_t stream) {
+  static bool attr_set[kMaxDevices] = {false};
+  return launch_tile128(gemm_fp8_wide256<MX>, wb_lds_bytes(MX), attr_set, p, stream);
 }
 
 template <int MF, int NF, int NW, bool MX, bool F32OUT, bool EPI>
@@ -258,10 +262,10 @@ int launch_gemm_skinny(SkinnyParams p, bool f32out, hipStream_t stream) {
 //     6.4 / 7.0, 512x2048x2048 8.2 / 10.4 (and losing: 512x4096x4096 20.8 / 17.3)
 //   128x128 against 256x256 tiles: 2048^3 13.9 / 25.6 us, 2048x4096x4096 40.8 / 48.1
 //     (MX 44.8 / 52.5), 4096^3 79 / 51, 2048x8192x1024 28.3 / 21.2
-// MX: the scaled MFMA's steps take longer in every kernel.  Wide (fp32 C with an epilogue: bf16 products,
-// strips or gemm_fp8_wide): the same on 60 shapes (M = 1 .. 2048, N x K = 1024 x 2048 .. 14336 x 4096, both
-// modes, a residual, launches as a graph): the pick costs 2% over the best
-// strip or tile on average, 11% at most.
+// MX: the scaled MFMA's steps take longer in every kernel.  Wide (fp32 C with an epilogue: bf16 products on
+// strips, gemm_fp8_wide or, in place of the 256x256 tiles, gemm_fp8_wide256): the same on 120 cases (M = 48 ..
+// 6000, N x K = 1024 x 2048 .. 14336 x 2048, both modes, a residual, launches as a graph): the pick costs 0.8%
+// over the best of the larger strips and the tiles on average, 7% at most.
 enum class DenseKernel { kStrip11, kStrip21, kStrip12, kStrip22, kStrip24, kStrip44, kTile128, kTile256 };
 
 // Tile blocks of the dense 256x256 kernel: 2^b M tiles x 32 / 2^b N tiles, one
@@ -301,18 +305,23 @@ DenseKernel pick_dense(int64_t m, int64_t n, int64_t k, bool f32out, bool mx, bo
     const double last = rounds == 1 ? tiles : std::max(1.0, std::min(cus, tiles - full * cus));
     offer(DenseKernel::kTile256, 5.4 + full * (ramp + ks * step(cus)) + ramp + ks * step(last), 0);
   }
-  {
-    // M tiles in fours: the workgroups that a 4x8 block has past M exit at once, but they
-    // take their turns in the dispatch, and the live ones share a part of the CUs
-    // (65x11264x2048, 88 live ones: 24 us, as two rounds would)
-    const uint64_t mt = (um + kSmTile - 1) / kSmTile, nt = un / kSmTile, tiles = (mt + 3) / 4 * 4 * nt;
+  // M tiles in fours: the workgroups that a 4x8 block has past M exit at once, but they
+  // take their turns in the dispatch, and the live ones share a part of the CUs
+  // (65x11264x2048, 88 live ones: 24 us, as two rounds would; wide, 200x14336x2048, 224 live ones: 33, the
+  // steps of both rounds as fast as on a half-full chip)
+  auto offer_tiles = [&](DenseKernel kern, int rows, double ramp, double busy, double idle) {  // per step, chip full / half full
+    const uint64_t mt = (um + rows - 1) / rows, nt = un / kSmTile, tiles = (mt + 3) / 4 * 4 * nt;
     const double full = static_cast<double>(tiles / ncu), part = static_cast<double>(tiles % ncu);
     const double live = std::min(part, static_cast<double>(mt * nt));  // of the last round
-    // per step, chip full / half full
-    const double busy = wide ? (mx ? 1.07 : 0.95) : mx ? 0.58 : 0.52, idle = wide ? (mx ? 0.77 : 0.69) : mx ? 0.51 : 0.40;
-    const double ramp = wide ? 5.0 : f32out ? 4.0 : 2.6;
-    offer(DenseKernel::kTile128,
-          1.75 + full * (ramp + ks * busy) + (part > 0 ? ramp + ks * (live <= cus / 2 ? idle : busy) : 0), 3 + nk / 2.0e6);
+    const bool sparse = wide && mt * nt * 2 <= tiles;
+    offer(kern, 1.75 + full * (ramp + ks * (sparse ? idle : busy)) +
+                    (part > 0 ? ramp + ks * (sparse || live <= cus / 2 ? idle : busy) : 0), 3 + nk / 2.0e6);
+  };
+  if (wide) {
+    offer_tiles(DenseKernel::kTile128, kSmTile, 5.0, mx ? 0.95 : 0.83, mx ? 0.77 : 0.69);
+    offer_tiles(DenseKernel::kTile256, kWbRows, 9.7, mx ? 1.46 : 1.36, mx ? 1.14 : 1.11);
+  } else {
+    offer_tiles(DenseKernel::kTile128, kSmTile, f32out ? 4.0 : 2.6, mx ? 0.58 : 0.52, mx ? 0.51 : 0.40);
   }
   const struct {
     DenseKernel kern;
@@ -325,7 +334,7 @@ DenseKernel pick_dense(int64_t m, int64_t n, int64_t k, bool f32out, bool mx, bo
     const uint64_t wgs = ((um + (1u << c.rows_log2) - 1) >> c.rows_log2) * (un >> c.cols_log2);
     const double rounds = static_cast<double>((wgs + ncu - 1) / ncu);
     const double steps = static_cast<double>(((k / kBK + (1 << c.waves_log2) - 1) >> c.waves_log2) << c.waves_log2);
-    const double ramp = wide ? c.wide_ramp : c.ramp, step = wide ? c.wide_step * (mx ? 1.2 : 1.0) : c.step * (mx ? 1.1 : 1.0);
+    const double ramp = wide ? c.wide_ramp : c.ramp, step = wide ? c.wide_step * (mx ? 1.05 : 1.0) : c.step * (mx ? 1.1 : 1.0);
     offer(c.kern, (mx ? 1.6 : 1.3) + rounds * (ramp + steps * step), 3 + nk / 5.5e6);
   }
   return best;
@@ -338,7 +347,8 @@ int launch_dense(const void* a, const void* b, void* c, int64_t m, int64_t n, in
                  const float* scale_b, int out_dtype, hipStream_t s, const EpilogueArgs& epi = {}) {
   const bool f32out = out_dtype == HKMOE_F32;
   const int32_t m64 = static_cast<int32_t>((m + 63) / 64 * 64);
-  const DenseKernel kern = pick_dense(m, n, k, f32out, MX, EPI && f32out);
+  const bool wide = EPI && f32out;
+  const DenseKernel kern = pick_dense(m, n, k, f32out, MX, wide);
   if (kern < DenseKernel::kTile128) {
     SkinnyParams q{};
     q.a = static_cast<const uint8_t*>(a);
@@ -360,7 +370,7 @@ int launch_dense(const void* a, const void* b, void* c, int64_t m, int64_t n, in
       default: return launch_gemm_skinny<4, 4, 4, MX, EPI>(q, f32out, s);
     }
   }
-  if (kern == DenseKernel::kTile128) {
+  if (kern == DenseKernel::kTile128 || wide) {
     SmallGemmParams q{};
     q.a = static_cast<const uint8_t*>(a);
     q.b = static_cast<const uint8_t*>(b);
@@ -377,7 +387,12 @@ int launch_dense(const void* a, const void* b, void* c, int64_t m, int64_t n, in
     q.n_tiles = static_cast<int32_t>(n / kSmTile);
     q.nbn = (q.n_tiles + 7) / 8;
     q.epi = epi;
-    if constexpr (EPI) return f32out ? launch_gemm_wide<MX>(q, s) : launch_gemm_small_act<MX>(q, s);
+    if constexpr (EPI) {
+      if (!wide) return launch_gemm_small_act<MX>(q, s);
+      if (kern == DenseKernel::kTile128) return launch_gemm_wide<MX>(q, s);
+      q.m_tiles = static_cast<int32_t>((m + kWbRows - 1) / kWbRows);  // 256x128
+      return launch_gemm_wide256<MX>(q, s);
+    }
     if constexpr (!MX) {
       if (g_dense_mfma.load() == 32)
         return f32out ? launch_gemm_small<true, true, false>(q, s) : launch_gemm_small<false, true, false>(q, s);

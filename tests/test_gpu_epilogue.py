@@ -15,7 +15,8 @@ BF16, F32 = torch.bfloat16, torch.float32
 SHAPES = [(1, 256, 128), (16, 256, 256), (17, 512, 1152), (31, 8192, 384), (33, 512, 384), (48, 256, 16384),
           (64, 2048, 4224), (65, 2048, 1024), (129, 256, 2048), (300, 1024, 1152), (257, 4096, 4096), (63, 768, 640),
           (1000, 4096, 256), (2001, 2048, 384), (1, 4352, 128), (16, 7168, 2048), (65, 32768, 1152), (4095, 4096, 384),
-          (1000, 1024, 2176), (50, 16384, 256), (2000, 768, 128), (3000, 1024, 512), (2049, 1024, 640)]
+          (1000, 1024, 2176), (50, 16384, 256), (2000, 768, 128), (3000, 1024, 512), (2049, 1024, 640),
+          (1777, 4096, 1152), (2047, 4096, 128), (1537, 8192, 256), (4097, 3840, 896)]
 
 
 def _operands(m, n, k, mx, seed):

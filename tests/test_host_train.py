@@ -269,7 +269,7 @@ for line in log(): print(line)
 
 def test_epilogue_shapes_reach_every_kernel(fake):
     """The GPU test's shapes run on every strip, with bf16 C on 128x128 and 256x256 tiles of the FP8
-    instructions, with fp32 C on the tiles that widen the operands.  (strips: MX, fp32 output, epilogue)"""
+    instructions, with fp32 C on both tiles that widen the operands.  (strips: MX, fp32 output, epilogue)"""
     for mx in (0, 1):
         for f32 in (0, 1):
             out = hip_host.run(fake, LAUNCH + f"""
@@ -278,12 +278,12 @@ for line in log(): print(line)
 """)
             got = set()
             for line in out:
-                m = re.match(r"launch hkmoe::gemm_fp8_(skinny<(\d), *_?(\d), *_?(\d), *_?(\w+), *_?(\w+), *_?(\w+)>|small_act|wide|persistent)", line)
+                m = re.match(r"launch hkmoe::gemm_fp8_(skinny<(\d), *_?(\d), *_?(\d), *_?(\w+), *_?(\w+), *_?(\w+)>|small_act|wide256|wide|persistent)", line)
                 if m.group(2):
                     assert m.group(5, 6, 7) == tuple("true" if v else "false" for v in (mx, f32, 1)), line
                 got.add(f"strip {m.group(2)}x{m.group(3)}" if m.group(2) else m.group(1))
             want = {"strip 1x1", "strip 2x1", "strip 1x2", "strip 2x2", "strip 2x4", "strip 4x4"}
-            assert got == want | ({"wide"} if f32 else {"small_act", "persistent"}), (mx, f32, got)
+            assert got == want | ({"wide", "wide256"} if f32 else {"small_act", "persistent"}), (mx, f32, got)
 
 
 def test_few_rows_need_one_launch_for_the_gradient(fake):
