@@ -19,7 +19,7 @@ import tk_kernel
 def layer_norm_forward(x, weight, bias=None, residual=None, eps=1e-5, residual_out=None):
     """Layer norm of ``x`` (+ ``residual``): returns ``(y, r, stats)``.
 
-    x [R, C] bf16 or fp32, residual like x, weight and bias [C] bf16 or fp32.  r is the new
+    x [R, C] bf16 or fp32, residual like x, weight and bias [C] both bf16 or both fp32.  r is the new
     stream x + residual in x's dtype (x itself without a residual; ``residual_out`` where given, which
     may be x or residual), y the norm of r in x's dtype, stats what
     :func:`layer_norm_backward` wants back (fp32 [R, 4])."""
