@@ -294,7 +294,9 @@ DenseKernel pick_dense(int64_t m, int64_t n, int64_t k, bool f32out, bool mx, bo
     const double t = std::max(compute, hbm) + 0.1 * compute;
     if (t < best_t) best = kern, best_t = t;
   };
-  if (!wide) {
+  // the 256x256 kernel's bf16 output goes through a descriptor of a tile's whole rows: 256 of them within 2^31 bytes
+  const bool far = !f32out && n > (1 << 22);
+  if (!wide && !far) {
     const double tiles = static_cast<double>((m + kBM - 1) / kBM) * (n / kBN);
     auto step = [&](double t) {  // per step, t tiles in the round
       return t <= cus / 4 ? (mx ? 1.12 : 0.95) : t <= cus / 2 ? (mx ? 1.27 : 1.13) : (mx ? 1.45 : 1.3);

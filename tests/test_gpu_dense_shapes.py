@@ -56,3 +56,23 @@ def test_dense_exact(hk, m, n, k, mx):
                 hk.tk_kernel.dispatch_gemm_fp8(a_q, b_q, c, *scales)
                 torch.cuda.synchronize()
                 assert torch.equal(c, (factor * ref).to(torch.float32).to(dtype)), scales
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("m,n", [(256, 1 << 23), (3, (1 << 24) + 256), (300, (1 << 22) + 256)])
+def test_far_columns(hk, m, n, mx):
+    """bf16 rows whose 256 make 2^32 bytes and more: every value, and the row behind the last one untouched."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    a, b = _pm1((m, 128), gen), _pm1((n, 128), gen)
+    a_q, b_q = a.to(torch.float8_e4m3fn), b.to(torch.float8_e4m3fn)
+    buf = torch.full((m + 1, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    if mx:
+        ones = lambda rows: hk.mx_pack_scales(torch.full((rows, 4), 127, dtype=torch.uint8, device="cuda"))  # noqa: E731
+        hk.tk_kernel.dispatch_gemm_mx(a_q, ones(m), b_q, ones(n), buf[:m])
+    else:
+        hk.tk_kernel.dispatch_gemm_fp8(a_q, b_q, buf[:m])
+    torch.cuda.synchronize()
+    for n0 in range(0, n, 1 << 20):  # sums of 128 values of +-1 are exact in bf16
+        want = a @ b[n0:n0 + (1 << 20)].T
+        assert torch.equal(buf[:m, n0:n0 + (1 << 20)].float(), want), n0
+    assert bool((buf[m] == 7.0).all())

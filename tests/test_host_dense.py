@@ -79,3 +79,16 @@ def test_mfma_shapes_of_the_128_kernel(fake):
             form = f"gemm_fp8_small<{'true' if f32 else 'false'},_{'true' if mfma == 32 else 'false'},_false>"
             for c, line in zip(calls, launches(fake, calls, mfma)):
                 assert form in line, (c, line)
+
+
+def test_far_columns(fake):
+    """The 256x256 kernel stores bf16 C through 32-bit offsets into a tile's 256 whole rows, 2^31 bytes at
+    N = 2^22; past that the kernels with 64-bit addresses take the product.  fp32 C always has those."""
+    calls = [(m, n, 128, f32, mx) for n in (1 << 22, (1 << 22) + 256, 1 << 23, (1 << 25) - 256) for m in (1, 100, 256, 1024)
+             for f32 in (0, 1) for mx in (0, 1)]
+    for (m, n, _, f32, mx), line in zip(calls, launches(fake, calls, 32)):
+        if f32 == 0 and n > 1 << 22:
+            assert "persistent" not in line, (m, n, mx, line)
+        v = {k: int(x) for k, x in (f.split("=") for f in line.split()[2:])}
+        assert v["grid"] * v["threads"] < 1 << 32, line
+    assert kernels(fake, [(256, 1 << 22, 128, 0, 0), (256, 1 << 23, 128, 1, 0)]) == ["256", "256"]
