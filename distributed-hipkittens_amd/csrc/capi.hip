@@ -983,6 +983,7 @@ static int gemm_fp8_check(const char* name, const void* a, const void* b, void* 
   HK_REQUIRE(k <= (1 << 20) && n * k < (1ll << 32) && m * k < (1ll << 32) && m < (1ll << 31),
              "%s: operand too large for 32-bit buffer offsets (M*K and N*K must be < 2^32)", name);
   HK_REQUIRE(out_dtype == HKMOE_BF16 || out_dtype == HKMOE_F32, "%s: bad out_dtype %d", name, out_dtype);
+  HK_REQUIRE(aligned16(a) && aligned16(b), "%s: A and B must be 16-byte aligned", name);
   return HKMOE_OK;
 }
 
@@ -2160,6 +2161,8 @@ static int gemm_mx_check(const char* name, const void* a, const void* a_scale, c
                  m64 * (k / 32) < (1ll << 32) && n * (k / 32) < (1ll << 32),
              "%s: operand too large for 32-bit buffer offsets (M*K and N*K must be < 2^32)", name);
   HK_REQUIRE(out_dtype == HKMOE_BF16 || out_dtype == HKMOE_F32, "%s: bad out_dtype %d", name, out_dtype);
+  HK_REQUIRE(aligned16(a) && aligned16(b) && aligned16(a_scale) && aligned16(b_scale),
+             "%s: A, B and their exponent words must be 16-byte aligned", name);
   return HKMOE_OK;
 }
 

@@ -60,9 +60,9 @@ const char* hkmoe_last_error(void);
  * Dense FP8 GEMM  C[M,N] = (sa*sb) * sum_k A[m,k] * B[n,k]   (A . B^T, "TN")
  *   A [M,K] e4m3, B [N,K] e4m3, C [M,N] bf16 (RNE) or fp32.
  *   scale_a, scale_b: device fp32 scalars, or NULL for 1.0.
- *   Requires K % 128 == 0 and N % 256 == 0; M is arbitrary.  fp32 accumulation;
- *   the kernel, and with it the order of a row's sum over K, follows from M, N and
- *   K, so a row's last bits may differ with the number of rows beside it.
+ *   Requires K % 128 == 0 and N % 256 == 0; M is arbitrary.  A and B 16-byte aligned.
+ *   fp32 accumulation; the kernel, and with it the order of a row's sum over K,
+ *   follows from M, N and K, so a row's last bits may differ with the number of rows beside it.
  * Replaces the reference's dispatch_micro(A, B, C) (C = A . B^T, fp32 out):
  *   kernels/cdna3/gemm/fp8fp32/mi300x/8192_256_256_64_32/data_logs/
  *   0613_003858_outputs/256_256_64_32.cpp:202-212 and the FP8 GEMM kernels named
@@ -589,8 +589,9 @@ int hkmoe_mx_pack_scales(const void* s, int64_t rows, int64_t cols, void* packed
  *     2^(sa[m,kb] - 127) * 2^(sb[n,kb] - 127) * sum_{k in kb} A[m,k] * B[n,k]
  *   A [M,K] e4m3 with packed scales a_scale [K/128, M64]; B [N,K] e4m3 with
  *   packed scales b_scale [K/128, N] (hkmoe_mx_pack_scales); fp32 accumulate,
- *   C bf16 (RNE) or fp32.  K % 128 == 0, N % 256 == 0, M arbitrary.  The order of a
- *   row's sum follows from M, N and K, as in hkmoe_gemm_fp8.
+ *   C bf16 (RNE) or fp32.  K % 128 == 0, N % 256 == 0, M arbitrary.  A, B and their
+ *   scales 16-byte aligned.  The order of a row's sum follows from M, N and K, as in
+ *   hkmoe_gemm_fp8.
  *   Replaces mxfp8_gemm_4wave_kernel (4_wave.cu:77-292), which is launched
  *   with the packed scales of prepare_mxfp8_data (4_wave.cu:377-448).
  */

@@ -395,3 +395,18 @@ def test_tensors_on_the_cpu_are_refused(name):
     args = dict(layer_norm=(x, torch.ones(64)), route_topk=(x, 2), moe_permute=(x, ids, 8), moe_combine=(torch.zeros((8, 64)), w, order))
     with pytest.raises(RuntimeError, match="GPU"):
         getattr(hkmoe, name)(*args[name])
+
+
+def _plain(lib, a=P, b=P):
+    return lib.hkmoe_gemm_fp8(a, b, P, i64(4), i64(256), i64(128), None, None, 0, None)
+
+
+def _plain_mx(lib, a=P, b=P, sa=P, sb=P):
+    return lib.hkmoe_gemm_mx(a, sa, b, sb, P, i64(4), i64(256), i64(128), 0, None)
+
+
+@pytest.mark.parametrize("call,name", [(c, n) for c in (_plain, _plain_mx, _fp8, _mx) for n in ("a", "b")] +
+                         [(c, n) for c in (_plain_mx, _mx) for n in ("sa", "sb")])
+def test_operands_of_odd_addresses_are_refused(lib, call, name):
+    """The operands, and the MX words, are fetched 16 bytes a lane."""
+    _refused(lib, call, {name: ODD}, "aligned")
