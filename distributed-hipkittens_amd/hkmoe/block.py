@@ -8,7 +8,7 @@ import torch
 
 import tk_kernel
 
-from .layer import F8, GROUP, MoELayer, MoELayerMX, _check_dev, _like, gemm_fp8, gemm_mx, mx_pack_scales
+from .layer import F8, GROUP, MoELayer, MoELayerMX, _check_dev, _like, _written, gemm_fp8, gemm_mx, mx_pack_scales
 
 _MODES = {"group": tk_kernel.SCALE_BLOCK, "mx": tk_kernel.SCALE_MX, "tensor": tk_kernel.SCALE_TENSOR}
 
@@ -44,6 +44,7 @@ def rms_norm_quant(x, weight, residual=None, scales="group", scale=None, eps=1e-
         raise RuntimeError('rms_norm_quant: a given scale is for scales="tensor"')
     q = _like(x, F8)
     n = _like(x, torch.bfloat16) if with_norm else None
+    given = residual_out
     if residual is None:
         if residual_out is not None:
             raise RuntimeError("rms_norm_quant: residual_out needs a residual")
@@ -51,14 +52,17 @@ def rms_norm_quant(x, weight, residual=None, scales="group", scale=None, eps=1e-
     else:
         r = residual_out = _like(x, x.dtype) if residual_out is None else residual_out
     tk_kernel.dispatch_rms_norm_quant(x, residual, weight, eps, _MODES[scales], q, s, scale, residual_out, n, ws)
+    _written(given)
     return q, scale if s is None else s, r, n
 
 
 def router_logits(x, w, out=None):
     """fp32 [T, E] router logits of bf16 x [T, H] and the router's bf16 weight w [E, H]."""
+    given = out
     if out is None:
         out = x.new_empty((x.shape[0], w.shape[0]), dtype=torch.float32)
     tk_kernel.dispatch_router_logits(x, w, out)
+    _written(given)
     return out
 
 
@@ -72,6 +76,7 @@ def lora_add(y, x, a, b, ids, scaling=None, out=None, workspace=None):
     tk_kernel.lora_workspace_size(T, H, R) bytes, allocated per call if None."""
     if a.dim() != 3:
         raise RuntimeError("lora_add: a must be [L, R, H]")
+    given = out
     if out is None:
         out = _like(y, y.dtype)
     if workspace is None:
@@ -79,6 +84,7 @@ def lora_add(y, x, a, b, ids, scaling=None, out=None, workspace=None):
         need = tk_kernel.lora_workspace_size(y.shape[0], hidden, rank)
         workspace = a.new_empty((need,), dtype=torch.uint8) if need else None
     tk_kernel.dispatch_lora_add(y, x, a, b, ids, scaling, out, workspace)
+    _written(given)
     return out
 
 

@@ -12,6 +12,8 @@ import torch
 
 import tk_kernel
 
+from .layer import _written
+
 
 # ----------------------------------------------------------------------------
 # layer norm
@@ -27,6 +29,7 @@ def layer_norm_forward(x, weight, bias=None, residual=None, eps=1e-5, residual_o
         raise RuntimeError("layer_norm: x must be [R, C]")
     y = torch.empty_like(x)
     stats = x.new_empty(x.shape[0], 4, dtype=torch.float32)
+    given = residual_out
     if residual is None:
         if residual_out is not None:
             raise RuntimeError("layer_norm: residual_out needs a residual")
@@ -34,6 +37,7 @@ def layer_norm_forward(x, weight, bias=None, residual=None, eps=1e-5, residual_o
     else:
         r = residual_out = torch.empty_like(x) if residual_out is None else residual_out
     tk_kernel.dispatch_layer_norm(x, residual, weight, bias, eps, y, residual_out, stats)
+    _written(given)
     return y, r, stats
 
 

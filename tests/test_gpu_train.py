@@ -609,3 +609,19 @@ def test_dense_half_of_a_block(hk):
     mag = (c.to(d).abs() @ q2.to(d).abs().T) * (sc.to(d) * s2.to(d)) + b2.to(d).abs() + r.to(d).abs()
     _check(h, want_h, 1.2 * (hidden + 64) * ref.U * mag_h)
     _check(stream, want, (inter + 64) * ref.U * mag)
+
+
+def test_an_overwritten_stream_has_no_gradient(hk):
+    """The norm's gradient reads the stream: after a product into it, or another norm's new stream, the backward
+    pass raises; without one it runs."""
+    aq, bq = torch.ones((4, 128), device="cuda").to(F8), torch.ones((256, 128), device="cuda").to(F8)
+    w = torch.ones(256, device="cuda", dtype=BF16, requires_grad=True)
+    x = torch.randn((4, 256), device="cuda").to(BF16)
+    for write in (lambda r: hk.gemm_fp8(aq, bq, residual=r, out=r), lambda r: hk.gemm_fp8(aq, bq, out=r),
+                  lambda r: hk.layer_norm_forward(x, w, residual=r, residual_out=r)):
+        y, r = hk.layer_norm(x, w, residual=torch.randn_like(x))
+        y.sum().backward(retain_graph=True)
+        with torch.no_grad():
+            write(r)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
