@@ -5,6 +5,7 @@ workspace) and for the current stream; every operation is one of the HIP
 kernels behind ``tk_kernel``.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 import tk_kernel
@@ -32,6 +33,20 @@ def _written(t):
     own in-place calls.  0.6 us of the host."""
     if t is not None:
         increment_version(t)
+
+
+def _asks_gradient(t):
+    """Whether a gradient of the tensor is being recorded, backward or forward (0.2 us: outside every dual level,
+    -1, there is no tangent to look for)."""
+    if getattr(t, "requires_grad", False) and torch.is_grad_enabled():  # what is no tensor the binding refuses
+        return True
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
+def _no_gradient(t, name):
+    """Refuses a tensor whose gradient would be lost."""
+    if _asks_gradient(t):
+        raise RuntimeError(f"{name} asks for a gradient, and none is recorded here: detach it, or call under torch.no_grad()")
 
 
 # ----------------------------------------------------------------------------
@@ -94,8 +109,15 @@ def gemm_fp8(a_q, b_q, scale_a=None, scale_b=None, out_dtype=torch.bfloat16, bia
     "gelu_tanh"; ``residual`` [M,N] in C's dtype.  C is rounded once, to ``out_dtype``, or to the dtype of
     ``out``, which may be the residual.  With any of these three, "none" included, an fp32 C is the
     product to fp32's own precision, at half the matrix rate; without, it is what the FP8 matrix
-    instruction gives (1.5e-5 of its size)."""
+    instruction gives (1.5e-5 of its size).  Records no gradient: where bias, residual or out ask for
+    one, the call is refused."""
     _check_dev(a_q, b_q)
+    if bias is not None:
+        _no_gradient(bias, "bias")
+    if residual is not None:
+        _no_gradient(residual, "residual")
+    if out is not None:
+        _no_gradient(out, "out")
     act = _activation(activation)
     c = a_q.new_empty(a_q.shape[0], b_q.shape[0], dtype=out_dtype) if out is None else out
     if bias is None and activation is None and residual is None:
@@ -135,6 +157,12 @@ def gemm_mx(a_q, a_packed, b_q, b_packed, out_dtype=torch.float32, bias=None, ac
     """C = act(A . B^T + bias) + residual with 1x32 e8m0 block scales (packed by mx_pack_scales);
     the other arguments as in :func:`gemm_fp8`."""
     _check_dev(a_q, b_q)
+    if bias is not None:
+        _no_gradient(bias, "bias")
+    if residual is not None:
+        _no_gradient(residual, "residual")
+    if out is not None:
+        _no_gradient(out, "out")
     act = _activation(activation)
     c = a_q.new_empty(a_q.shape[0], b_q.shape[0], dtype=out_dtype) if out is None else out
     if bias is None and activation is None and residual is None:

@@ -12,7 +12,7 @@ import torch
 
 import tk_kernel
 
-from .layer import _written
+from .layer import _no_gradient, _written
 
 
 # ----------------------------------------------------------------------------
@@ -24,7 +24,8 @@ def layer_norm_forward(x, weight, bias=None, residual=None, eps=1e-5, residual_o
     x [R, C] bf16 or fp32, residual like x, weight and bias [C] both bf16 or both fp32.  r is the new
     stream x + residual in x's dtype (x itself without a residual; ``residual_out`` where given, which
     may be x or residual), y the norm of r in x's dtype, stats what
-    :func:`layer_norm_backward` wants back (fp32 [R, 4])."""
+    :func:`layer_norm_backward` wants back (fp32 [R, 4]).  Records no gradient; a ``residual_out`` that
+    asks for one is refused."""
     if x.dim() != 2:
         raise RuntimeError("layer_norm: x must be [R, C]")
     y = torch.empty_like(x)
@@ -35,6 +36,8 @@ def layer_norm_forward(x, weight, bias=None, residual=None, eps=1e-5, residual_o
             raise RuntimeError("layer_norm: residual_out needs a residual")
         r = x
     else:
+        if residual_out is not None:
+            _no_gradient(residual_out, "residual_out")
         r = residual_out = torch.empty_like(x) if residual_out is None else residual_out
     tk_kernel.dispatch_layer_norm(x, residual, weight, bias, eps, y, residual_out, stats)
     _written(given)

@@ -261,3 +261,15 @@ def test_streams_and_graph(hk):
         eager = c1(hk, bias=bias, activation="gelu", residual=res)
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+def test_tensors_that_ask_for_a_gradient_are_refused(hk):
+    aq, bq = torch.ones((4, 128), device="cuda").to(torch.float8_e4m3fn), torch.ones((256, 128), device="cuda").to(torch.float8_e4m3fn)
+    bias, r = torch.zeros(256, device="cuda", requires_grad=True), torch.zeros((4, 256), device="cuda", dtype=BF16, requires_grad=True) * 1
+    for bad in (dict(bias=bias), dict(residual=r), dict(out=r), dict(residual=r, out=r)):
+        with pytest.raises(RuntimeError, match="asks for a gradient"):
+            hk.gemm_fp8(aq, bq, **bad)
+        assert not r.any()  # nothing ran
+    assert bool((hk.gemm_fp8(aq, bq, bias=bias.detach(), residual=r.detach()) == 128).all())
+    with torch.no_grad():
+        assert bool((hk.gemm_fp8(aq, bq, bias=bias, residual=r, out=r) == 128).all())

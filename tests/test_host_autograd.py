@@ -139,3 +139,35 @@ def test_a_stream_that_is_left_alone_has_one(hk):
         _overwrites(hk, kept)["gemm_fp8"]()
     y.backward(torch.ones_like(y))
     assert torch.allclose(w.grad, ref.layer_norm_grad(torch.ones(4, 256).double(), r.detach().double(), w.detach().double(), 1e-5, None)[1].float())
+
+
+PRODUCTS = {"gemm_fp8": lambda hk, **e: hk.gemm_fp8(_f8(4, 128), _f8(256, 128), **e),
+            "gemm_mx": lambda hk, **e: hk.gemm_mx(_f8(4, 128), None, _f8(256, 128), None, **{"out_dtype": BF16, **e})}
+
+
+@pytest.mark.parametrize("call", PRODUCTS.values(), ids=PRODUCTS)
+@pytest.mark.parametrize("name", ["bias", "residual", "out"])
+def test_products_refuse_tensors_that_ask_for_a_gradient(hk, call, name):
+    """The products record none: without an error, C would carry no gradient of the bias or the residual, and
+    the old history of a given tensor.  Detached, or without gradients being recorded, they are taken."""
+    t = torch.zeros(256 if name == "bias" else (4, 256), dtype=BF16, requires_grad=True)
+    for given in (t, t * 1):
+        with pytest.raises(RuntimeError, match=f"{name} asks for a gradient"):
+            call(hk, **{name: given})
+        assert not call(hk, **{name: given.detach()}).requires_grad
+        with torch.no_grad():
+            call(hk, **{name: given})
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(t.detach(), torch.ones_like(t))
+        with torch.no_grad(), pytest.raises(RuntimeError, match=f"{name} asks for a gradient"):
+            call(hk, **{name: dual})
+        call(hk, **{name: t.detach()})
+
+
+def test_the_stream_in_place_refuses_a_gradient(hk):
+    """layer_norm_forward records none; a new stream written into a tensor that has a history would keep it."""
+    r = torch.zeros((4, 64), requires_grad=True) * 1
+    with pytest.raises(RuntimeError, match="residual_out asks for a gradient"):
+        hk.layer_norm_forward(torch.ones(4, 64), torch.ones(64), residual=r, residual_out=r)
+    with torch.no_grad():
+        hk.layer_norm_forward(torch.ones(4, 64), torch.ones(64), residual=r, residual_out=r)
