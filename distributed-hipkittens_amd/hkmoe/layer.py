@@ -35,17 +35,16 @@ def _written(t):
         increment_version(t)
 
 
-def _asks_gradient(t):
-    """Whether a gradient of the tensor is being recorded, backward or forward (0.2 us: outside every dual level,
-    -1, there is no tangent to look for)."""
-    if getattr(t, "requires_grad", False) and torch.is_grad_enabled():  # what is no tensor the binding refuses
-        return True
-    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
+def _dual(*ts):
+    """Whether one of these tensors (or None) carries a tangent of forward mode.  (Outside every dual level, -1,
+    there is none to look for, which costs 1 us a tensor.)"""
+    return forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _no_gradient(t, name):
-    """Refuses a tensor whose gradient would be lost."""
-    if _asks_gradient(t):
+    """Refuses a tensor whose gradient would be lost (what is no tensor the binding refuses)."""
+    if (getattr(t, "requires_grad", False) and torch.is_grad_enabled()) or _dual(t):
         raise RuntimeError(f"{name} asks for a gradient, and none is recorded here: detach it, or call under torch.no_grad()")
 
 

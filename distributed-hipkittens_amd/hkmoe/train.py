@@ -2,9 +2,10 @@
 choice, tokens sorted by expert and back, each with its gradient.
 
 Every operator comes in two forms.  ``layer_norm``, ``route_topk``, ``moe_permute`` and
-``moe_combine`` record gradients where an input asks for them (first derivatives only).  The
-``*_forward`` / ``*_backward`` functions are the plain calls that those make, on the current
-stream, for programs that run their own backward pass or capture it into a graph.
+``moe_combine`` record gradients where an input asks for them (first derivatives, backward only:
+dual tensors of forward mode are refused, by autograd, for want of a jvp).  The ``*_forward`` /
+``*_backward`` functions are the plain calls that those make, on the current stream, for
+programs that run their own backward pass or capture it into a graph.
 """
 from typing import NamedTuple
 
@@ -12,7 +13,7 @@ import torch
 
 import tk_kernel
 
-from .layer import _no_gradient, _written
+from .layer import _dual, _no_gradient, _written
 
 
 # ----------------------------------------------------------------------------
@@ -79,7 +80,8 @@ def layer_norm(x, weight, bias=None, residual=None, eps=1e-5):
     """``(y, r)``: the layer norm y of the new stream r = x + residual (x itself without one), both
     in x's dtype; gradients of x, weight, bias and residual are recorded.  Arguments as in
     :func:`layer_norm_forward`."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+            or _dual(x, weight, bias, residual)):
         out = _LayerNorm.apply(x, weight, bias, residual, eps)
         return out if residual is not None else (out, x)
     return layer_norm_forward(x, weight, bias, residual, eps)[:2]
@@ -129,7 +131,7 @@ class _RouteTopk(torch.autograd.Function):
 
 def route_topk(logits, top_k):
     """:func:`route_topk_forward` with the gradient of w to the logits recorded."""
-    if logits.requires_grad and torch.is_grad_enabled():
+    if logits.requires_grad and torch.is_grad_enabled() or _dual(logits):
         return _RouteTopk.apply(logits, top_k)
     return route_topk_forward(logits, top_k)
 
@@ -217,7 +219,7 @@ class _Combine(torch.autograd.Function):
 
 def moe_permute(x, ids, num_experts):
     """:func:`moe_permute_forward` with the gradient of x recorded (not for e4m3 rows)."""
-    if x.requires_grad and torch.is_grad_enabled():
+    if x.requires_grad and torch.is_grad_enabled() or _dual(x):
         xp, *order = _Permute.apply(x, ids, num_experts)
         return xp, MoEOrder(*order)
     return moe_permute_forward(x, ids, num_experts)
@@ -225,6 +227,6 @@ def moe_permute(x, ids, num_experts):
 
 def moe_combine(y, w, order):
     """:func:`moe_combine_forward` with the gradients of y and w recorded."""
-    if (y.requires_grad or w.requires_grad) and torch.is_grad_enabled():
+    if (y.requires_grad or w.requires_grad) and torch.is_grad_enabled() or _dual(y, w):
         return _Combine.apply(y, w, *order)
     return moe_combine_forward(y, w, order)

@@ -171,3 +171,34 @@ def test_the_stream_in_place_refuses_a_gradient(hk):
         hk.layer_norm_forward(torch.ones(4, 64), torch.ones(64), residual=r, residual_out=r)
     with torch.no_grad():
         hk.layer_norm_forward(torch.ones(4, 64), torch.ones(64), residual=r, residual_out=r)
+
+
+def _recorded(hk):
+    """The recorded calls: name -> (the tensors that may ask for a gradient, the call on them)."""
+    order = hk.MoEOrder(torch.tensor([0, 4, 8], dtype=torch.int32), torch.arange(8, dtype=torch.int32),
+                        torch.arange(8, dtype=torch.int32).view(4, 2))
+    rows, w = torch.randn(8, 64), torch.rand(4, 2)
+    return {
+        "layer_norm": ([torch.randn(4, 64), torch.ones(64), torch.zeros(64), torch.randn(4, 64)],
+                       lambda x, w, b, s: hk.layer_norm(x, w, b, s)),
+        "layer_norm alone": ([torch.randn(4, 64), torch.ones(64)], lambda x, w: hk.layer_norm(x, w)),
+        "route_topk": ([torch.randn(4, 8)], lambda x: hk.route_topk(x, 2)),
+        "moe_permute": ([torch.randn(4, 64)], lambda x: hk.moe_permute(x, torch.zeros((4, 2), dtype=torch.int32), 2)),
+        "moe_combine": ([rows, w], lambda y, w: hk.moe_combine(y, w, order)),
+    }
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "layer_norm alone", "route_topk", "moe_permute", "moe_combine"])
+def test_forward_mode_is_refused(hk, monkeypatch, name):
+    """Only backward gradients are recorded: a dual tensor's tangent is never dropped without an error, whether or
+    not gradients are on, and calls without one run inside a dual level."""
+    for kernel, places in dict(route_topk=(1, 2), permute=(2, 3, 4, 5), combine_rows=(4,)).items():
+        monkeypatch.setattr(hk.tk_kernel, "dispatch_" + kernel, _fill(*places))
+    tensors, call = _recorded(hk)[name]
+    with torch.autograd.forward_ad.dual_level():
+        call(*tensors)
+        for i, t in enumerate(tensors):
+            dual = tensors[:i] + [torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))] + tensors[i + 1:]
+            for ctx in (torch.enable_grad(), torch.no_grad()):
+                with ctx, pytest.raises(RuntimeError, match="jvp"):
+                    call(*dual)
