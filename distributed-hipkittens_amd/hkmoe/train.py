@@ -16,6 +16,13 @@ import tk_kernel
 from .layer import _dual, _no_gradient, _written
 
 
+def _rows(g):
+    """A gradient from autograd as the kernels read rows: contiguous and 16-byte aligned, which a slice of a
+    flattened concatenation's gradient, for one, is not."""
+    g = g.contiguous()
+    return g if g.data_ptr() % 16 == 0 else g.clone()
+
+
 # ----------------------------------------------------------------------------
 # layer norm
 # ----------------------------------------------------------------------------
@@ -71,8 +78,7 @@ class _LayerNorm(torch.autograd.Function):
         if dy is None:  # the norm has no use: the stream's own gradient is all there is
             return dr, None, None, dr if ctx.has_residual else None, None
         r, weight, stats = ctx.saved_tensors
-        dx, dw, db = layer_norm_backward(dy.contiguous(), r, weight, stats, None if dr is None else dr.contiguous(),
-                                         ctx.has_bias)
+        dx, dw, db = layer_norm_backward(_rows(dy), r, weight, stats, None if dr is None else _rows(dr), ctx.has_bias)
         return dx, dw, db, dx if ctx.has_residual else None, None
 
 
@@ -201,7 +207,7 @@ class _Permute(torch.autograd.Function):
     def backward(ctx, dxp, *_):
         if dxp is None:
             return None, None, None
-        return moe_permute_backward(dxp.contiguous(), MoEOrder(*ctx.saved_tensors)), None, None
+        return moe_permute_backward(_rows(dxp), MoEOrder(*ctx.saved_tensors)), None, None
 
 
 class _Combine(torch.autograd.Function):
@@ -214,7 +220,7 @@ class _Combine(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         y, w, *order = ctx.saved_tensors
-        return (*moe_combine_backward(dout.contiguous(), y, w, MoEOrder(*order)), None, None, None)
+        return (*moe_combine_backward(_rows(dout), y, w, MoEOrder(*order)), None, None, None)
 
 
 def moe_permute(x, ids, num_experts):

@@ -625,3 +625,28 @@ def test_an_overwritten_stream_has_no_gradient(hk):
             write(r)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradients_at_odd_addresses(hk, dtype):
+    """A gradient that autograd hands back as a slice at an odd address: the same bits as from an aligned one."""
+    gen = _gen(17)
+    t, h, k, e = 6, 264, 2, 4
+    leaf = lambda *s: _randn(gen, *s).to(dtype).requires_grad_()  # noqa: E731
+    x, s, w, b, y = leaf(t, h), leaf(t, h), leaf(h), leaf(h), leaf(t * k, h)
+    tw = torch.rand((t, k), generator=gen, device="cuda").requires_grad_()
+    ids = torch.randint(-1, e, (t, k), generator=gen, device="cuda", dtype=torch.int32)
+    weights = _randn(gen, 4 * t * k * h + 1).to(dtype)
+
+    def gradients(odd):
+        n, r = hk.layer_norm(x, w, b, s)
+        xp, order = hk.moe_permute(n, ids, e)
+        flat = lambda v: torch.cat([torch.zeros(odd, device="cuda", dtype=dtype), v.reshape(-1)]) if odd else v.reshape(-1)  # noqa: E731
+        loss = 0.0
+        for v in (n, r, xp, hk.moe_combine(y, tw, order)):
+            f = flat(v)
+            loss = loss + (f.float() * weights[1 - odd:][: f.numel()].float()).sum()
+        return torch.autograd.grad(loss, (x, s, w, b, y, tw))
+
+    for got, want in zip(gradients(1), gradients(0)):
+        assert torch.equal(got, want)

@@ -202,3 +202,43 @@ def test_forward_mode_is_refused(hk, monkeypatch, name):
             for ctx in (torch.enable_grad(), torch.no_grad()):
                 with ctx, pytest.raises(RuntimeError, match="jvp"):
                     call(*dual)
+
+
+def _needs_aligned(kernel, *places):
+    """A kernel that refuses what the library refuses: these of its arguments at other than 16-byte addresses."""
+    def run(*args):
+        for i in places:
+            if args[i] is not None and (args[i].data_ptr() % 16 or not args[i].is_contiguous()):
+                raise RuntimeError("tensors must be contiguous and 16-byte aligned")
+        kernel(*args)
+    return run
+
+
+def _odd_gradient(t):
+    """A scalar whose gradient comes back to t as a slice at an odd address: t behind one value, flattened together."""
+    flat = torch.cat([torch.zeros(1, dtype=t.dtype), t.reshape(-1)])
+    return (flat * torch.arange(flat.numel()).to(t.dtype)).sum()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradients_at_odd_addresses(hk, monkeypatch, dtype):
+    """Where autograd lays out a gradient is not the caller's choice: one that is contiguous but not 16-byte
+    aligned (a slice of a flattened concatenation) is taken."""
+    tk = hk.tk_kernel
+    monkeypatch.setattr(tk, "dispatch_layer_norm_backward", _needs_aligned(_layer_norm_backward, 0, 1, 3))
+    monkeypatch.setattr(tk, "dispatch_permute", _fill(2, 3, 4, 5))
+    monkeypatch.setattr(tk, "dispatch_combine_rows", _needs_aligned(_fill(4), 0))
+    monkeypatch.setattr(tk, "dispatch_combine_rows_backward", _needs_aligned(_fill(5, 6), 0, 1))
+    leaf = lambda *s: torch.randn(s).to(dtype).requires_grad_()  # noqa: E731
+    x, s, w = leaf(4, 64), leaf(4, 64), torch.ones(64, dtype=dtype, requires_grad=True)
+    y, r = hk.layer_norm(x, w, residual=s)
+    (_odd_gradient(y) + _odd_gradient(r)).backward()
+    dy = torch.arange(1, 257).to(dtype).view(4, 64).double()
+    want = ref.layer_norm_grad(dy, r.detach().double(), w.detach().double(), 1e-5, dy)[0].to(dtype)
+    assert torch.allclose(x.grad, want) and torch.equal(x.grad, s.grad) and x.grad.data_ptr() != s.grad.data_ptr()
+    x = leaf(4, 64)
+    xp, order = hk.moe_permute(x, torch.zeros((4, 2), dtype=torch.int32), 2)
+    _odd_gradient(xp).backward()
+    tw = torch.rand((4, 2), requires_grad=True)
+    _odd_gradient(hk.moe_combine(leaf(8, 64), tw, order)).backward()
+    assert x.grad is not None and tw.grad is not None
