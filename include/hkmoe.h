@@ -86,8 +86,10 @@ int hkmoe_gemm_fp8(const void* a, const void* b, void* c, int64_t m, int64_t n, 
  *     HKMOE_ACT_SILU       z / (1 + e^-z)
  *     HKMOE_ACT_GELU       z Phi(z), Phi the normal distribution function (the erf form)
  *     HKMOE_ACT_GELU_TANH  z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2
- *   to a few ulp of fp32; for large |z| the exponential costs more: (16 + z^2) 2^-23 of
- *   Phi(-|z|), (4 + |z|) 2^-23 of SiLU.  C, bias and residual 16-byte aligned, N <= 2^21.
+ *   to a few ulp of fp32; for large |z| the rounding of the exponent costs more: (16 + z^2) 2^-23 of
+ *   Phi(-|z|), (4 + |z|) 2^-23 of SiLU, (4 + 2.5 e) 2^-23 of GELU_TANH with e = sqrt(8/pi) (|z| +
+ *   0.044715 |z|^3).  Activations of magnitude below 2^-119 may be 0.
+ *   C, bias and residual 16-byte aligned, N <= 2^21.
  *   hkmoe_set_dense_mfma does not apply.
  * No reference counterpart (its GEMMs store C as it is).
  */

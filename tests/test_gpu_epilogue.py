@@ -273,3 +273,30 @@ def test_tensors_that_ask_for_a_gradient_are_refused(hk):
     assert bool((hk.gemm_fp8(aq, bq, bias=bias.detach(), residual=r.detach()) == 128).all())
     with torch.no_grad():
         assert bool((hk.gemm_fp8(aq, bq, bias=bias, residual=r, out=r) == 128).all())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_tails(hk, act):
+    """Small negative results keep the header's relative bounds down to 2^-119, rounded to bf16 as well, in strips
+    and on every tile."""
+    lo, hi = {"silu": (-105.0, -75.0), "gelu": (-14.0, -11.0), "gelu_tanh": (-11.0, -8.0)}[act]
+    n = 1024
+    z = torch.linspace(lo, hi, n, device="cuda")
+    v = z.double()
+    if act == "gelu":
+        want, bound = v * ref.phi(v), (16 + v * v) * 2.0 ** -23
+    else:
+        e = v if act == "silu" else math.sqrt(8 / math.pi) * (v + 0.044715 * v ** 3)
+        want, bound = v / (1 + torch.exp(-e)), (4 + (1.0 if act == "silu" else 2.5) * e.abs()) * 2.0 ** -23
+    far = want.abs() >= 2.0 ** -119
+    assert bool(far.any()) and not bool(far.all())
+    bq = torch.zeros((n, 128), device="cuda").to(torch.float8_e4m3fn)
+    for m in (1, 300, 2000, 5000, 20000):
+        aq = torch.zeros((m, 128), device="cuda").to(torch.float8_e4m3fn)
+        for dtype in (F32, BF16):
+            got = hk.gemm_fp8(aq, bq, bias=z, activation=act, out_dtype=dtype)
+            assert torch.equal(got, got[:1].expand_as(got))
+            off = (got[0].double() - want).abs()
+            allow = (bound + (0 if dtype == F32 else ref.half(dtype)) * (1 + bound)) * want.abs()
+            assert bool((off <= allow)[far].all()), (m, dtype, float((off / want.abs())[far].max()))
+            assert bool((off[~far] <= 2.0 ** -119).all())

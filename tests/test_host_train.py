@@ -410,3 +410,25 @@ def _plain_mx(lib, a=P, b=P, sa=P, sb=P):
 def test_operands_of_odd_addresses_are_refused(lib, call, name):
     """The operands, and the MX words, are fetched 16 bytes a lane."""
     _refused(lib, call, {name: ODD}, "aligned")
+
+
+def test_tails_of_silu_and_gelu_tanh():
+    """The kernel's form of z / (1 + 2^x), operation by operation in fp32 (exp2 and reciprocal rounded where the
+    hardware's are an ulp off, 0 below the normal numbers): within the header's bounds down to 2^-119, and no
+    further off than that below."""
+    f = np.float32
+    z = np.arange(-105, 40, 1 / 64, dtype=f)
+    t = np.arange(-11, 11, 1 / 512, dtype=f)
+    slope = ((t * t).astype(np.float64) * f(-0.10294324) + np.float64(f(-2.3022082))).astype(f)  # one FMA
+    for v, x, name in ((z, z * f(-1.44269504), "silu"), (t, t * slope, "gelu_tanh")):
+        with np.errstate(over="ignore", under="ignore"):
+            r = 1 / (f(1) + np.exp2(x.astype(np.float64)).astype(f)).astype(np.float64)
+            got = v * np.where(r < 2.0 ** -126, 0, r).astype(f)
+        v = torch.from_numpy(v.astype(np.float64))
+        e = v if name == "silu" else (8 / np.pi) ** 0.5 * (v + 0.044715 * v ** 3)
+        want = v / (1 + torch.exp(-e))
+        bound = (4 + (1.0 if name == "silu" else 2.5) * e.abs()) * 2.0 ** -23 * want.abs()
+        off = (torch.from_numpy(got.astype(np.float64)) - want).abs()
+        far = want.abs() >= 2.0 ** -119
+        assert bool((off <= bound)[far].all()) and bool((off[~far] <= 2.0 ** -119).all()), name
+        assert not bool(far.all()) and float(want[far & (v < -1)].abs().min()) < 2.0 ** -118  # the grid passes the limit
