@@ -94,7 +94,8 @@ __device__ __forceinline__ f32x4 epilogue_bias(const EpilogueArgs& e, int col) {
 // ---------------------------------------------------------------------------
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
-// 2^(byte - 127) of byte I of a word of e8m0 exponents.
+// 2^(byte - 127) of byte I of a word of e8m0 exponents.  255, e8m0's NaN, becomes an infinite scale, of which the
+// conversion reads the exponent field: it gives NaN for every element, zeros too, as the scaled MFMA does.
 template <int I>
 __device__ __forceinline__ float e8m0_scale(int word) {
   const uint32_t e = (static_cast<uint32_t>(word) >> (8 * I)) & 0xffu;

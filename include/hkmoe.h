@@ -79,7 +79,7 @@ int hkmoe_gemm_fp8(const void* a, const void* b, void* c, int64_t m, int64_t n, 
  *   what is below about 2^-16 of the largest product (1.5e-5 of a random sum, in the plain
  *   entry points, too).  For fp32 C, z is summed to fp32's own precision at half the matrix rate;
  *   MX operands, element times its block's power of two, are then exact between 2^-133 and 2^128,
- *   smaller ones lose bits and larger ones become infinite.
+ *   smaller ones lose bits and larger ones become infinite.  A block whose exponent is 255 is NaN in either.
  *   bias [N] bf16 or fp32 (bias_dtype) or NULL; residual [M, N] in C's type or NULL, may be C.
  *   activation:
  *     HKMOE_ACT_RELU       max(z, 0)

@@ -300,3 +300,30 @@ def test_tails(hk, act):
             allow = (bound + (0 if dtype == F32 else ref.half(dtype)) * (1 + bound)) * want.abs()
             assert bool((off <= allow)[far].all()), (m, dtype, float((off / want.abs())[far].max()))
             assert bool((off[~far] <= 2.0 ** -119).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 256, 256), (40, 512, 1152), (2000, 1024, 256), (5000, 1024, 256)])
+def test_nan_exponents(hk, m, n, k):
+    """Exponent byte 255, e8m0's NaN, in blocks of A, of B and of zeros: NaN in the row or the column that the
+    block is part of and nowhere else, on the widened operands (fp32 C), the FP8 instructions (bf16 C), and in
+    the plain product alike."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    pm1 = lambda *s: (torch.randint(0, 2, s, generator=gen, device="cuda") * 2 - 1).float()  # noqa: E731
+    a, b = pm1(m, k), pm1(n, k)
+    ea = torch.full((m, k // 32), 127, dtype=torch.uint8, device="cuda")
+    eb = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda")
+    rows, cols = [0, m // 2, m - 1], [1, n // 2 + 3, n - 1]
+    for i, (r, c) in enumerate(zip(rows, cols)):
+        ea[r, (3 * i) % (k // 32)] = 255
+        eb[c, (5 * i + 1) % (k // 32)] = 255
+    z = ((3 * 2) % (k // 32)) * 32
+    a[m - 1, z:z + 32] = 0.0
+    aq, bq = a.to(torch.float8_e4m3fn), b.to(torch.float8_e4m3fn)
+    want = aq.double() @ bq.double().T
+    want[rows, :] = math.nan
+    want[:, cols] = math.nan
+    pa, pb = hk.mx_pack_scales(ea), hk.mx_pack_scales(eb)
+    for dtype in (F32, BF16):
+        for act in ("none", None):
+            got = hk.gemm_mx(aq, pa, bq, pb, activation=act, out_dtype=dtype)
+            assert torch.equal(got.double().nan_to_num(nan=1e9), want.float().to(dtype).double().nan_to_num(nan=1e9)), (dtype, act)
