@@ -750,7 +750,8 @@ int layer_norm_parts(int64_t rows, int64_t cols) {
 //   64 x 128 12.7 / 8.6 (4.9 / 3.3)      512 x 1024 13.2 / 8.4 (8.6 / 6.6)    1024 x 1024 13.0 / 10.4 (7.9 / 10.1)
 //   4 x 4096 12.8 / 8.5 (5.3 / 3.2)      512 x 4096 13.0 / 8.2 (12.0 / 5.8)   2048 x 4096 18.6 / 23.0
 //   1024 x 8192 19.3 / 16.2              1024 x 16384 36.5 / 35.0
-// and fp32, 512 x 8192 19.5 / 16.4, 1024 x 8192 28.8 / 30.3.
+// and fp32, 512 x 8192 19.5 / 16.4, 1024 x 8192 28.8 / 30.3: the workspace's size, which asks the same question,
+// does not know the type, so one limit serves both and fp32 loses 5% there.
 bool layer_norm_in_one(int64_t rows, int64_t cols) { return rows <= (cols > 4096 ? 1024 : 512); }
 
 template <bool F32, bool COLS>
